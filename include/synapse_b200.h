@@ -237,6 +237,148 @@ int syn_rope(const float* x, float* out, int n, int n_heads, int head_dim, const
              const float* freq_factors, int rope_mode, const float* yarn, void* stream);
 
 /* ------------------------------------------------------------------------
+ * KV caches in F16, Q8_0 or Q4_0, and decoding of token trees over them: a
+ * step that verifies several drafted continuations at once appends the
+ * drafted tokens' rows (syn_kv_append), attends with a tree mask
+ * (syn_tree_attention), picks a token at every node (syn_logits_process) and
+ * moves the accepted rows together (syn_kv_move). The reference has an F16
+ * cache, one-token attention and a bare argmax only (kernels/attention.hpp:
+ * 133-269, llama_decode.cpp:274); these entries have no counterpart there.
+ *
+ * A cache of one layer and sequence (K or V), max_ctx rows:
+ *   SYN_F16  : [max_ctx][n_kv][head_dim] binary16, the layout syn_attention
+ *              and a session's caches have (attention.hpp:133-143);
+ *   SYN_Q8_0 : int8 quants [n_kv][max_ctx][head_dim], then, at the next
+ *              256-byte boundary, binary16 scales [n_kv][max_ctx][head_dim/32];
+ *              a value is scale * quant (quant/q8.hpp:54-69 per 32 values);
+ *   SYN_Q4_0 : 4-bit quants [n_kv][max_ctx][head_dim/2 bytes], byte j of a
+ *              block of 32 holding value j (low) and j + 16 (high), then
+ *              scales as Q8_0; a value is scale * (quant - 8).
+ * head_dim is a multiple of 32 (F16: of 8) and at most 256. Sequence i's
+ * cache starts i * seq_stride bytes after sequence 0's, layer l's
+ * l * layer_stride after layer 0's; pointers and strides are multiples of
+ * 16. Rows outside [0, max_ctx) that a device array names are skipped.
+ * ---------------------------------------------------------------------- */
+typedef struct {
+    void* k;              /* layer 0, sequence 0 */
+    void* v;
+    size_t seq_stride;    /* bytes; unused with n_seq = 1 */
+    size_t layer_stride;  /* bytes; unused with n_layer = 1 */
+    int type;             /* SYN_F16 / SYN_Q8_0 / SYN_Q4_0, K and V alike */
+    int n_layer, n_seq, n_kv, head_dim, max_ctx;
+} syn_kv_cache;
+/* Bytes of one layer's K (or V) of one sequence, a multiple of 16; 0 for a
+ * type or shape that is not supported. */
+size_t syn_kv_cache_bytes(int type, int n_kv, int head_dim, int max_ctx);
+
+/* Append n tokens of every sequence: rows k, v (token i of sequence s at
+ * (s * n + i) * kv_stride floats) are rotated (K, when rope_table is given),
+ * quantised or rounded to the cache's type and stored in row slot[s * n + i].
+ * q, if given, is rotated into q_out by the same launch, in the layout
+ * syn_tree_attention takes. A token's RoPE position is pos[s * n + i]
+ * (NULL: its slot; in a tree the positions are the committed length plus the
+ * node's depth). Quantised types store finite values: an input beyond
+ * binary16's range is clamped to +-65504 and NaN stored as 0; F16 stores what
+ * the rounding gives. A token whose slot is outside the cache, or whose
+ * position is outside the table, is skipped whole (its q_out row too). Two
+ * tokens of a call must not share a slot of a sequence. */
+typedef struct {
+    const float* k;          /* [n_seq * n][n_kv * head_dim] */
+    const float* v;
+    const float* q;          /* NULL, or [n_seq * n][n_head * head_dim] */
+    float* q_out;            /* contiguous [n_seq * n][n_head * head_dim]; must not overlap q */
+    const int32_t* slot;     /* [n_seq * n] device */
+    const int32_t* pos;      /* NULL, or [n_seq * n] device */
+    const float* rope_table; /* NULL: no rotation; or syn_rope_table of table_len rows */
+    size_t kv_stride;        /* floats between tokens of k and of v (0: n_kv * head_dim) */
+    size_t q_stride;         /* floats between tokens of q (0: n_head * head_dim) */
+    int n, n_head, table_len;
+    int rope_mode;           /* 0 normal (Llama), 1 neox */
+} syn_kv_append_args;
+int syn_kv_append(const syn_kv_cache* c, int layer, const syn_kv_append_args* a, void* stream);
+
+/* Read n rows of every sequence back as values: row i of sequence s is cache
+ * row rows[s * n + i] (device), or first + i when rows is NULL. k_out, v_out
+ * (either may be NULL): [n_seq][n][n_kv][head_dim] of out_type SYN_F32 or
+ * SYN_F16, 16-byte aligned. Rows outside the cache read as zeros. */
+int syn_kv_read(const syn_kv_cache* c, int layer, const int32_t* rows, int first, int n, int out_type, void* k_out,
+                void* v_out, void* stream);
+
+/* Move rows together, in every layer: row path[s * path_ld + i] of sequence s
+ * becomes row begin[s] + i, for i < count[s] <= path_ld (device arrays). Each
+ * sequence's path must ascend with path[i] >= begin + i, as the nodes of a
+ * path through a tree appended at begin do. What a cache holds in the other
+ * rows stays. */
+int syn_kv_move(const syn_kv_cache* c, const int32_t* path, int path_ld, const int32_t* count, const int32_t* begin,
+                void* stream);
+
+/* Attention of n_tree tokens of every sequence over its cache:
+ *   out = softmax(scale * q K^T) V  over rows 0 .. len[s] - 1, which every
+ *   token sees, and of rows len[s] + j, j < n_tree, those whose bit j is set
+ *   in the token's mask words (mask NULL: those with j <= the token's index,
+ *   i.e. a causal chunk; n_tree = 1 without a mask is one-token decode, its
+ *   own row included).
+ * Query head h reads KV head h / (n_head / n_kv). Products use the binary16
+ * or block values of the cache as stored; q, the probabilities and every sum
+ * keep 22 bits or more (about 1e-6 relative). A token that sees nothing gets
+ * zeros. What masked rows hold, infinities and NaN included, reaches no
+ * output; a token that sees a row with a value that is not finite gets NaN in
+ * the heads that read it.
+ * len[s] is clamped to [0, max_len - n_tree]; max_len <= max_ctx bounds
+ * len[s] + n_tree and sizes the split of the context over the GPU.
+ * scratch: syn_tree_attention_scratch_bytes, 16-byte aligned, zeroed once
+ * before its first use (each call leaves it ready for the next, of any
+ * shape); calls whose GPU work overlaps need scratches of their own. */
+typedef struct {
+    const float* q;          /* [n_seq * n_tree][n_head * head_dim], rotated */
+    float* out;              /* contiguous [n_seq * n_tree][n_head * head_dim] */
+    const int32_t* len;      /* [n_seq] device: rows committed before the tree's */
+    const uint32_t* mask;    /* NULL, or [n_seq][n_tree][(n_tree + 31) / 32] device */
+    void* scratch;
+    size_t q_stride;         /* floats between tokens of q (0: n_head * head_dim) */
+    int n_tree, n_head, max_len;
+    float scale;
+} syn_tree_attention_args;
+size_t syn_tree_attention_scratch_bytes(int n_seq, int n_tree, int n_head, int n_kv, int head_dim, int max_len);
+int syn_tree_attention(const syn_kv_cache* c, int layer, const syn_tree_attention_args* a, void* stream);
+
+/* Logit processing of n_tree rows (tree nodes; 1 in plain decode) of n_seq
+ * sequences, row r = s * n_tree + i:
+ *   x = logits[r][t] + the sequence's bias of token t
+ *   c = occurrences of t in the sequence's history and in the drafted tokens
+ *       on the node's path (mask bits as in syn_tree_attention; the node's own
+ *       token is on its path)
+ *   if c > 0: x = (x > 0 ? x / repeat : x * repeat) - (c * frequency + presence)
+ *   x = -inf where the row's grammar mask has no bit t
+ *   pick[r] = the lowest t with the largest x, or -1 when no x is above -inf
+ *             (NaN is never picked).
+ * Everything but logits, out or pick, and the sizes may be NULL. Tokens
+ * outside the vocabulary count nowhere. A token that a sequence's bias list
+ * names twice gets both. Calls that overlap on the GPU need scratches of
+ * their own. */
+typedef struct {
+    const float* logits;
+    float* out;                 /* NULL: only picks; may be logits itself */
+    int32_t* pick;              /* NULL, or [n_seq * n_tree] */
+    size_t ld, out_ld;          /* floats between rows (0: n_vocab) */
+    const float* penalties;     /* [n_seq][3]: repeat, presence, frequency; NULL: 1, 0, 0 */
+    const int32_t* history;     /* [n_seq][history_ld] */
+    const int32_t* history_len; /* [n_seq], clamped to [0, history_ld] */
+    const int32_t* draft;       /* [n_seq][n_tree]: the nodes' tokens */
+    const uint32_t* mask;       /* NULL with draft: node i's path is nodes 0 .. i */
+    const int32_t* bias_begin;  /* [n_seq + 1]: sequence s has entries bias_begin[s] .. bias_begin[s + 1] - 1 */
+    const int32_t* bias_token;
+    const float* bias_value;
+    const uint32_t* allowed;    /* [n_seq * n_tree][allowed_ld]: bit t % 32 of word t / 32 */
+    size_t allowed_ld;          /* words between rows (0: (n_vocab + 31) / 32) */
+    void* scratch;              /* with pick: syn_logits_scratch_bytes, 8-byte aligned, zeroed once before its
+                                   first use (each call leaves it zero) */
+    int n_seq, n_tree, n_vocab, history_ld;
+} syn_logits_args;
+size_t syn_logits_scratch_bytes(int n_rows);
+int syn_logits_process(const syn_logits_args* a, void* stream);
+
+/* ------------------------------------------------------------------------
  * Element-wise ops (kernels/elementwise.hpp), each on n_tok rows.
  * ---------------------------------------------------------------------- */
 /* out = x / rms(x) * gamma (elementwise.hpp:208-232), then optionally quantized

@@ -133,6 +133,14 @@ def _declare(L):
         "syn_session_prefill": (i32, [vp, i32, vp, i32, ctypes.c_uint32, vp, vp]),
         "syn_session_step_batch": (i32, [vp, i32, vp, vp, vp, vp]),
         "syn_session_fill_kv_random": (i32, [vp, i32, ctypes.c_uint64]),
+        "syn_kv_cache_bytes": (sz, [i32, i32, i32, i32]),
+        "syn_kv_append": (i32, [vp, i32, vp, vp]),
+        "syn_kv_read": (i32, [vp, i32, vp, i32, i32, i32, vp, vp, vp]),
+        "syn_kv_move": (i32, [vp, vp, i32, vp, vp, vp]),
+        "syn_tree_attention_scratch_bytes": (sz, [i32, i32, i32, i32, i32, i32]),
+        "syn_tree_attention": (i32, [vp, i32, vp, vp]),
+        "syn_logits_scratch_bytes": (sz, [i32]),
+        "syn_logits_process": (i32, [vp, vp]),
     })
     for name, (res, args) in sig.items():
         fn = getattr(L, name)
@@ -370,6 +378,217 @@ def rope(x, pos, n_heads, head_dim, theta_scale, rope_mode=0, freq_factors=None,
     check(lib().syn_rope(_ptr(x), _ptr(out), n, n_heads, head_dim, _ptr(pos), theta_scale, _ptr(freq_factors),
                          rope_mode, None, _stream(stream)), "syn_rope")
     return out
+
+
+# ---------------------------------------------------------------------------
+# KV caches in F16 / Q8_0 / Q4_0 and decoding of token trees over them
+
+class KVCacheDesc(ctypes.Structure):
+    """syn_kv_cache."""
+    _fields_ = [("k", ctypes.c_void_p), ("v", ctypes.c_void_p), ("seq_stride", ctypes.c_size_t),
+                ("layer_stride", ctypes.c_size_t)] + \
+               [(n, ctypes.c_int) for n in ("type", "n_layer", "n_seq", "n_kv", "head_dim", "max_ctx")]
+
+
+class KVAppendArgs(ctypes.Structure):
+    """syn_kv_append_args."""
+    _fields_ = [(n, ctypes.c_void_p) for n in ("k", "v", "q", "q_out", "slot", "pos", "rope_table")] + \
+               [("kv_stride", ctypes.c_size_t), ("q_stride", ctypes.c_size_t)] + \
+               [(n, ctypes.c_int) for n in ("n", "n_head", "table_len", "rope_mode")]
+
+
+class TreeAttentionArgs(ctypes.Structure):
+    """syn_tree_attention_args."""
+    _fields_ = [(n, ctypes.c_void_p) for n in ("q", "out", "len", "mask", "scratch")] + \
+               [("q_stride", ctypes.c_size_t)] + [(n, ctypes.c_int) for n in ("n_tree", "n_head", "max_len")] + \
+               [("scale", ctypes.c_float)]
+
+
+class LogitsArgs(ctypes.Structure):
+    """syn_logits_args."""
+    _fields_ = [(n, ctypes.c_void_p) for n in ("logits", "out", "pick")] + \
+               [("ld", ctypes.c_size_t), ("out_ld", ctypes.c_size_t)] + \
+               [(n, ctypes.c_void_p) for n in ("penalties", "history", "history_len", "draft", "mask", "bias_begin",
+                                                "bias_token", "bias_value", "allowed")] + \
+               [("allowed_ld", ctypes.c_size_t), ("scratch", ctypes.c_void_p)] + \
+               [(n, ctypes.c_int) for n in ("n_seq", "n_tree", "n_vocab", "history_ld")]
+
+
+def kv_cache_bytes(type_, n_kv, head_dim, max_ctx):
+    """Bytes of one layer's K (or V) of one sequence; 0 for a type or shape that is not supported."""
+    return lib().syn_kv_cache_bytes(type_, n_kv, head_dim, max_ctx)
+
+
+class KVCache:
+    """K and V caches of n_layer layers and n_seq sequences in F16, Q8_0 or Q4_0 (syn_kv_cache)."""
+
+    def __init__(self, type_, n_layer, n_seq, n_kv, head_dim, max_ctx, device="cuda"):
+        n = kv_cache_bytes(type_, n_kv, head_dim, max_ctx)
+        if n == 0:
+            raise SynapseError(2, "syn_kv_cache_bytes")
+        data = _torch().zeros((n_layer, 2, n_seq, n), dtype=_torch().uint8, device=device)
+        self._describe(type_, data[:, 0], data[:, 1], n_kv, head_dim, max_ctx)
+
+    @classmethod
+    def over(cls, type_, k, v, n_kv, head_dim, max_ctx):
+        """A cache over a caller's byte tensors k and v: [n_seq][bytes] or [n_layer][n_seq][bytes], strided alike."""
+        self = cls.__new__(cls)
+        self._describe(type_, k, v, n_kv, head_dim, max_ctx)
+        return self
+
+    def _describe(self, type_, k, v, n_kv, head_dim, max_ctx):
+        if k.dim() == 2:
+            k, v = k[None], v[None]
+        if k.shape != v.shape or k.stride() != v.stride() or k.element_size() != 1 or v.element_size() != 1 or \
+                k.dim() != 3 or k.stride(2) != 1 or k.shape[2] < kv_cache_bytes(type_, n_kv, head_dim, max_ctx) or \
+                not k.is_cuda or k.device != v.device:
+            raise ValueError("k and v must be CUDA byte tensors [n_layer][n_seq][bytes] of one layout, large enough")
+        self.k, self.v, self.device = k, v, k.device
+        self.type, self.n_layer, self.n_seq = type_, k.shape[0], k.shape[1]
+        self.n_kv, self.head_dim, self.max_ctx = n_kv, head_dim, max_ctx
+        self.desc = KVCacheDesc(k.data_ptr(), v.data_ptr(), k.stride(1) if self.n_seq > 1 else 0,
+                                k.stride(0) if self.n_layer > 1 else 0, type_, self.n_layer, self.n_seq, n_kv,
+                                head_dim, max_ctx)
+        self.ref = ctypes.byref(self.desc)
+
+
+def _need(t, dtype, n, where):
+    """A contiguous CUDA tensor of dtype with n elements; its address (None for None)."""
+    if t is None:
+        return None
+    if t.dtype != dtype or not t.is_cuda or not t.is_contiguous() or (n is not None and t.numel() != n):
+        raise ValueError(f"{where}: needs a contiguous {dtype} CUDA tensor of {n} elements")
+    return t.data_ptr()
+
+
+def _rows(t, cols, n, where):
+    """Rows of cols floats whose rows may be strided: (address, floats between rows)."""
+    f32 = _torch().float32
+    if t.dtype != f32 or not t.is_cuda or t.dim() != 2 or t.shape[0] != n or t.shape[1] != cols or \
+            (cols > 1 and t.stride(1) != 1) or (n > 1 and t.stride(0) < cols):
+        raise ValueError(f"{where}: needs {n} float rows of {cols} on the GPU")
+    return t.data_ptr(), t.stride(0) if n > 1 else cols
+
+
+def kv_append(cache, k, v, slot, pos=None, rope_table=None, rope_mode=0, q=None, layer=0, stream=None):
+    """Append tokens' K and V rows [n_seq * n][n_kv * head_dim] at slots (int32, n_seq * n), K rotated when a
+    rope_table ([len][head_dim / 2][2]) is given; q [n_seq * n][n_head * head_dim], if given, is rotated too and
+    returned."""
+    torch = _torch()
+    tokens, hd = slot.numel(), cache.head_dim
+    kp, ks = _rows(k, cache.n_kv * hd, tokens, "kv_append k")
+    vp, vs = _rows(v, cache.n_kv * hd, tokens, "kv_append v")
+    if ks != vs or tokens % cache.n_seq:
+        raise ValueError("kv_append: k and v must be strided alike, with the same tokens for every sequence")
+    qp = qs = out = None
+    n_head = 0
+    if q is not None:
+        n_head = q.shape[1] // hd
+        qp, qs = _rows(q, n_head * hd, tokens, "kv_append q")
+        out = torch.empty((tokens, n_head * hd), dtype=torch.float32, device=q.device)
+    table_len = 0
+    if rope_table is not None:
+        table_len = rope_table.numel() // hd
+    a = KVAppendArgs(kp, vp, qp, out.data_ptr() if out is not None else None, _need(slot, torch.int32, tokens, "slot"),
+                     _need(pos, torch.int32, tokens, "pos"), _need(rope_table, torch.float32, table_len * hd, "rope_table"),
+                     ks, qs or 0, tokens // cache.n_seq, n_head, table_len, rope_mode)
+    check(lib().syn_kv_append(cache.ref, layer, ctypes.byref(a), _stream(stream)), "syn_kv_append")
+    return out
+
+
+def kv_read(cache, n, rows=None, first=0, dtype=None, layer=0, stream=None):
+    """n rows of every sequence as values, (k, v) [n_seq][n][n_kv][head_dim]: the cache rows named by `rows` (int32,
+    n_seq * n), or first, first + 1, ...; dtype torch.float32 (default) or torch.float16."""
+    torch = _torch()
+    dtype = dtype or torch.float32
+    if dtype not in (torch.float32, torch.float16):
+        raise ValueError("kv_read: dtype is torch.float32 or torch.float16")
+    k, v = torch.empty((2, cache.n_seq, n, cache.n_kv, cache.head_dim), dtype=dtype, device=cache.device)
+    check(lib().syn_kv_read(cache.ref, layer, _need(rows, torch.int32, cache.n_seq * n, "rows"), first, n,
+                            F16 if dtype == torch.float16 else F32, k.data_ptr(), v.data_ptr(), _stream(stream)),
+          "syn_kv_read")
+    return k, v
+
+
+def kv_move(cache, path, count, begin, stream=None):
+    """Rows path[s][i] (int32, ascending, >= begin[s] + i) of sequence s become rows begin[s] + i, i < count[s], in
+    every layer."""
+    torch = _torch()
+    ld = path.shape[-1]
+    check(lib().syn_kv_move(cache.ref, _need(path, torch.int32, cache.n_seq * ld, "path"), ld,
+                            _need(count, torch.int32, cache.n_seq, "count"),
+                            _need(begin, torch.int32, cache.n_seq, "begin"), _stream(stream)), "syn_kv_move")
+
+
+def tree_attention_scratch(cache, tree, n_head, max_len=None):
+    """A zeroed scratch for tree_attention calls of this shape; it may be kept for every later call on one stream."""
+    n = lib().syn_tree_attention_scratch_bytes(cache.n_seq, tree, n_head, cache.n_kv, cache.head_dim,
+                                               max_len or cache.max_ctx)
+    return _torch().zeros(max(n, 1), dtype=_torch().uint8, device=cache.device)
+
+
+def tree_attention(cache, q, len, n_head, scale, tree=1, mask=None, max_len=None, out=None, scratch=None, layer=0,
+                   stream=None):
+    """Attention of `tree` tokens of every sequence over rows 0 .. len[s] - 1 and the tree's own rows after them that
+    their mask bits name (None: a causal chunk); q [n_seq * tree][n_head * head_dim], rotated. See syn_tree_attention."""
+    torch = _torch()
+    cols, rows = n_head * cache.head_dim, cache.n_seq * tree
+    max_len = max_len or cache.max_ctx
+    qp, qs = _rows(q, cols, rows, "tree_attention q")
+    if out is None:
+        out = torch.empty((rows, cols), dtype=torch.float32, device=q.device)
+    need = lib().syn_tree_attention_scratch_bytes(cache.n_seq, tree, n_head, cache.n_kv, cache.head_dim, max_len)
+    if scratch is None:
+        scratch = torch.zeros(max(need, 1), dtype=torch.uint8, device=q.device)
+    elif scratch.numel() * scratch.element_size() < need:
+        raise ValueError(f"tree_attention: scratch of {need} bytes needed")
+    a = TreeAttentionArgs(qp, _need(out, torch.float32, rows * cols, "out"), _need(len, torch.int32, cache.n_seq, "len"),
+                          _need(mask, torch.int32, rows * ((tree + 31) // 32), "mask"), scratch.data_ptr(), qs, tree,
+                          n_head, max_len, scale)
+    check(lib().syn_tree_attention(cache.ref, layer, ctypes.byref(a), _stream(stream)), "syn_tree_attention")
+    return out
+
+
+def logits_scratch(n_rows, device="cuda"):
+    """A zeroed scratch for logits_process calls of up to n_rows rows on one stream."""
+    return _torch().zeros(max(lib().syn_logits_scratch_bytes(n_rows), 1), dtype=_torch().uint8, device=device)
+
+
+def logits_process(logits, n_seq, penalties=None, history=None, history_len=None, draft=None, mask=None, bias=None,
+                   allowed=None, out=None, pick=True, scratch=None, stream=None):
+    """Biases, penalties and a grammar mask on logits [n_seq * tree][n_vocab], and the pick of every row: (out, pick).
+    penalties [n_seq][3] (repeat, presence, frequency), history [n_seq][ld] with history_len [n_seq], the tree's
+    tokens draft [n_seq][tree] with mask words, bias (begin [n_seq + 1], tokens, values), allowed [rows][words]. out
+    may be logits itself; pick=False leaves the pick out. See syn_logits_process."""
+    torch = _torch()
+    rows, vocab = logits.shape
+    tree = rows // n_seq
+    if tree * n_seq != rows:
+        raise ValueError("logits_process: the same rows for every sequence")
+    xp, ld = _rows(logits, vocab, rows, "logits")
+    if out is None:
+        out = torch.empty((rows, vocab), dtype=torch.float32, device=logits.device)
+    op, out_ld = _rows(out, vocab, rows, "out")
+    picks = torch.empty(rows, dtype=torch.int32, device=logits.device) if pick else None
+    if pick and scratch is None:
+        scratch = logits_scratch(rows, logits.device)
+    if pick and scratch.numel() * scratch.element_size() < lib().syn_logits_scratch_bytes(rows):
+        raise ValueError("logits_process: the scratch is too small")
+    i32, words = torch.int32, (vocab + 31) // 32
+    begin, tokens, values = bias if bias is not None and bias[1].numel() else (None, None, None)
+    n = tokens.numel() if tokens is not None else None
+    if history is not None and history.dim() != 2:
+        raise ValueError("logits_process: history is [n_seq][ld]")
+    history_ld = history.shape[1] if history is not None else 0
+    a = LogitsArgs(xp, op, picks.data_ptr() if pick else None, ld, out_ld,
+                   _need(penalties, torch.float32, 3 * n_seq, "penalties"),
+                   _need(history, i32, n_seq * history_ld, "history"), _need(history_len, i32, n_seq, "history_len"),
+                   _need(draft, i32, rows, "draft"), _need(mask, i32, rows * ((tree + 31) // 32), "mask"),
+                   _need(begin, i32, n_seq + 1, "bias begin"), _need(tokens, i32, n, "bias tokens"),
+                   _need(values, torch.float32, n, "bias values"), _need(allowed, i32, rows * words, "allowed"), words,
+                   scratch.data_ptr() if pick else None, n_seq, tree, vocab, history_ld)
+    check(lib().syn_logits_process(ctypes.byref(a), _stream(stream)), "syn_logits_process")
+    return out, picks
 
 
 # ---------------------------------------------------------------------------

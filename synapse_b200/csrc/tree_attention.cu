@@ -1,0 +1,729 @@
+// Attention of a tree of drafted tokens over a KV cache (syn_tree_attention):
+// out = softmax(scale q K^T) V over the committed rows and the tree's own rows
+// that a token's mask names. n_tree = 1 is one-token decode.
+//
+// A KV head's work is one matrix product over the rows r = token * G + head of
+// its group (G = n_head / n_kv): M = n_tree * G rows against every position,
+// so the cache is read once for the whole tree.
+//
+// tree_attn_kernel: a CTA takes 16 or 32 of the M rows and a run of the
+// context. Its four warps take every fourth step of 16 positions, each with a
+// ring of its own in shared memory (16-byte asynchronous copies, no barrier
+// between the warps), and keep a running maximum, sum and output of their own
+// (one pass over K and V); the warps' results are joined at the end. With few
+// rows the context is split over CTAs so that all SMs read: each CTA leaves
+// (max, sum, output) in the scratch and the last one to arrive joins them in
+// split order.
+//
+// Precision: the products run on binary16 tensor-core instructions with float
+// accumulators. q is scaled by a power of two per row and split into two
+// binary16 terms (22 bits), and so are the probabilities; K and V enter as
+// stored. Quantised caches enter as integers (exact in binary16): a score is
+// the sum over blocks of scale * (q . quants); for V the block's scale is
+// m * 2^e, 2^e <= 2^9 applied to the integers (exact) and m (in [1, 2) for all
+// but extreme scales) to the float probabilities before they are split, so no value is rounded to binary16.
+#include "kv_cache.cuh"
+
+#include <algorithm>
+#include <mutex>
+#include <vector>
+
+using namespace syn;
+
+namespace {
+
+constexpr int kWarps = 4;
+constexpr int kStep = 16;            // positions per step of a warp
+constexpr float kPShift = 8.0f;      // probabilities carry 2^8, away from binary16's subnormals
+constexpr size_t kCounterBytes = 16384;  // arrival counters at the start of the scratch
+constexpr int kMaxTree = 1024;
+
+struct TreeParams {
+    KvView c;
+    const float* q;
+    float* out;
+    const int32_t* len;
+    const uint32_t* mask;
+    unsigned* counters;  // [n_seq][n_kv * row blocks]
+    float* parts;        // [n_seq][n_kv * row blocks][splits]: m[R], l[R], o[R][hd]
+    size_t q_stride;
+    int n_tree, n_head, group, rows, row_blocks, max_len, mask_words, splits;
+    float scale_log2;    // scale * log2(e)
+};
+
+__device__ __forceinline__ void cp16(uint32_t dst, const void* src, bool in) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(in ? 16 : 0) : "memory");
+}
+__device__ __forceinline__ void cp_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void cp_wait() {
+    asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+}
+__device__ __forceinline__ void ldsm4(uint32_t (&r)[4], uint32_t addr) {
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+                 : "r"(addr));
+}
+__device__ __forceinline__ void ldsm4t(uint32_t (&r)[4], uint32_t addr) {
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+                 : "r"(addr));
+}
+// C += A B, m16n8k16: lane = 4 g + t holds A[g | g + 8][2t.. | 2t + 8..], B[2t.. | 2t + 8..][g], C[g | g + 8][2t..].
+__device__ __forceinline__ void mma(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+    asm volatile(
+        "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+        : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ float ex2(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+__device__ __forceinline__ uint32_t bits(__half2 h) { return *reinterpret_cast<uint32_t*>(&h); }
+__device__ __forceinline__ __half2 half2_of(uint32_t u) { return *reinterpret_cast<__half2*>(&u); }
+// (x, y) as binary16 pairs hi + lo.
+__device__ __forceinline__ void split2(float x, float y, uint32_t& hi, uint32_t& lo) {
+    const __half2 h = __floats2half2_rn(x, y);
+    const float2 f = __half22float2(h);
+    hi = bits(h);
+    lo = bits(__floats2half2_rn(x - f.x, y - f.y));
+}
+// Bytes i and j of x as binary16 integers 1024 + byte.
+__device__ __forceinline__ __half2 bytes_h2(uint32_t x, uint32_t sel) { return half2_of(__byte_perm(x, 0x64646464u, sel)); }
+
+// Shared memory of one warp's stage: K rows, V rows (pitches keep the
+// fragment reads free of bank conflicts), then the scales of the 16 positions.
+template <int TYPE, int HDP>
+struct Stage {
+    static constexpr int row = TYPE == SYN_F16 ? HDP * 2 : TYPE == SYN_Q8_0 ? HDP : HDP / 2;  // bytes
+    static constexpr int k_pitch = row + (TYPE == SYN_Q8_0 ? 32 : 16);
+    static constexpr int v_pitch = row + 16;
+    static constexpr int nb = HDP / 32;
+    static constexpr int scales = TYPE == SYN_F16 ? 0 : kStep * nb * 2 + 16;  // K's (V's alike), from a 16-byte boundary
+    static constexpr int v_at = kStep * k_pitch;
+    static constexpr int sk_at = v_at + kStep * v_pitch;
+    static constexpr int sv_at = sk_at + scales;
+    static constexpr int bytes = sv_at + scales;
+};
+
+template <int TYPE, int HDP, int MT>
+struct Plan {
+    using S = Stage<TYPE, HDP>;
+    static constexpr int R = 16 * MT;                                // rows of a CTA
+    static constexpr int q_pitch = HDP * 2 + 16;
+    static constexpr int q_bytes = 2 * R * q_pitch;                  // hi and lo
+    static constexpr int stages = TYPE == SYN_F16 ? (HDP >= 256 ? 2 : 3) : 4;
+    static constexpr int ring = kWarps * stages * S::bytes;
+    static constexpr int o_pitch = HDP + 4;                          // floats
+    static constexpr int join = kWarps * R * (o_pitch + 2) * 4;      // the warps' results, over the ring
+    static constexpr int smem = q_bytes + (ring > join ? ring : join) + R * 4;  // + the rows' score factors
+};
+
+template <int TYPE, int HDP, int MT>
+__global__ void __launch_bounds__(kWarps * 32, 2) tree_attn_kernel(const TreeParams a) {
+    using S = Stage<TYPE, HDP>;
+    using P = Plan<TYPE, HDP, MT>;
+    constexpr int R = P::R, KS = HDP / 16, NB = HDP / 32;
+    constexpr bool kQuant = TYPE != SYN_F16;
+    constexpr bool kQReg = MT == 1 && HDP <= 128;
+    extern __shared__ __align__(128) unsigned char smem[];
+    unsigned char* ring = smem + P::q_bytes;
+    float* row_scale = reinterpret_cast<float*>(smem + P::smem - R * 4);
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
+    const int hd = a.c.hd;
+    const int kvh = blockIdx.y / a.row_blocks, rb = blockIdx.y - kvh * a.row_blocks, seq = blockIdx.z;
+    const int row0 = rb * R, rows = min(R, a.rows - row0);
+
+    pdl_launch_dependents();
+    pdl_wait();
+    const int len = min(max(a.len[seq], 0), a.max_len - a.n_tree);
+    const int total = len + a.n_tree;
+    const int steps = (total + kStep - 1) / kStep;
+    const int per = (steps + a.splits - 1) / a.splits;
+    const int active = (steps + per - 1) / per;  // splits that have steps
+    const int s0 = blockIdx.x * per, s1 = min(s0 + per, steps);
+    if (s0 >= steps) return;
+
+    // --- the ring -------------------------------------------------------------
+    const int nb = hd / 32;  // blocks of a row (quantised)
+    const char *kbase = a.c.k + size_t(seq) * a.c.seq_stride, *vbase = a.c.v + size_t(seq) * a.c.seq_stride;
+    // a position's K (V) row of this head, and the bytes between positions
+    const int row_bytes = TYPE == SYN_F16 ? hd * 2 : TYPE == SYN_Q8_0 ? hd : hd / 2;
+    const size_t pos_pitch = TYPE == SYN_F16 ? size_t(a.c.n_kv) * hd * 2 : size_t(row_bytes);
+    const size_t head_at = TYPE == SYN_F16 ? size_t(kvh) * hd * 2 : size_t(kvh) * a.c.max_ctx * row_bytes;
+    const size_t scale_at = a.c.scale_plane + size_t(kvh) * a.c.max_ctx * nb * 2;
+    const int scale_off = kQuant ? int(scale_at & 15) : 0;  // the same for every step: 16 positions are 32 nb bytes
+    unsigned char* my_ring = ring + warp * P::stages * S::bytes;
+    const uint32_t ring_s = smem_addr(my_ring);
+    auto load = [&](int step, int stage) {
+        const uint32_t st = ring_s + stage * S::bytes;
+        const int p0 = step * kStep;
+        const int chunks = row_bytes / 16;
+        constexpr int CP = S::row / 16;  // chunks of a full row
+#pragma unroll
+        for (int i = 0; i < kStep * CP / 32; ++i) {
+            const int r = (i * 32 + lane) / CP, c = (i * 32 + lane) % CP;
+            const bool in = p0 + r < total;
+            const size_t at = head_at + size_t(in ? p0 + r : 0) * pos_pitch + c * 16;
+            if (c < chunks) {
+                cp16(st + r * S::k_pitch + c * 16, kbase + at, in);
+                cp16(st + S::v_at + r * S::v_pitch + c * 16, vbase + at, in);
+            }
+        }
+        if (kQuant) {
+            // the run of scales from its 16-byte boundary; the last chunk holds at least one of its bytes
+            const int last = min(p0 + kStep, a.c.max_ctx);
+            const size_t at = (scale_at + size_t(p0) * nb * 2) & ~size_t(15);
+            const int n = (scale_off + (last - p0) * nb * 2 + 15) / 16;
+            constexpr int most = S::scales / 16;
+            const int which = lane / 16, c = lane % 16;
+            if (c < n) cp16(st + (which ? S::sv_at : S::sk_at) + c * 16, (which ? vbase : kbase) + at + c * 16, true);
+            if (most > 16 && c + 16 < n)
+                cp16(st + (which ? S::sv_at : S::sk_at) + (c + 16) * 16, (which ? vbase : kbase) + at + (c + 16) * 16, true);
+        }
+    };
+    if (hd != HDP) {  // dims past the head stay zero
+        for (int i = tid; i < P::ring / 16; i += kWarps * 32) reinterpret_cast<uint4*>(ring)[i] = make_uint4(0, 0, 0, 0);
+        __syncthreads();
+    }
+    int next = s0 + warp;  // the next step to request
+#pragma unroll
+    for (int i = 0; i < P::stages - 1; ++i) {
+        if (next < s1) load(next, i);
+        cp_commit();
+        next += kWarps;
+    }
+
+    // --- q: scaled to a row maximum in [2^8, 2^9), split, in the order of the K fragments -------
+    for (int r = warp; r < R; r += kWarps) {
+        const int row = row0 + r, tok = row / a.group, h = row - tok * a.group;
+        const bool in = r < rows;
+        const float* src = a.q + (size_t(seq) * a.n_tree + (in ? tok : 0)) * a.q_stride + size_t(kvh * a.group + (in ? h : 0)) * hd;
+        float x[NB], m = 0.0f;
+#pragma unroll
+        for (int b = 0; b < NB; ++b) {
+            const int d = 32 * b + lane;
+            x[b] = in && d < hd ? src[d] : 0.0f;
+            m = fmaxf(m, fabsf(x[b]));
+        }
+        m = warp_max(m);
+        // 2^e <= m < 2^(e+1); zero, subnormal and non-finite rows keep a factor of 1 * 2^8
+        const int e = int(__float_as_uint(m) >> 23);
+        const bool plain = e < 32 || e > 250;
+        const float up = plain ? 256.0f : __uint_as_float(uint32_t(254 + 8 - e) << 23);
+        const float down = plain ? 1.0f / 256.0f : __uint_as_float(uint32_t(e - 8) << 23);
+        if (lane == 0) row_scale[r] = a.scale_log2 * down;
+#pragma unroll
+        for (int b = 0; b < NB; ++b) {
+            // the k index of dim `lane` of the block in its two products of 16
+            int s = lane >> 4, k = lane & 15;
+            if (TYPE == SYN_Q8_0) {  // dim = 8 t + 4 s + e, e = 0..3: k = 2 t + (e & 1) + 8 (e >> 1)
+                s = (lane >> 2) & 1;
+                k = 2 * (lane >> 3) + (lane & 1) + 8 * ((lane >> 1) & 1);
+            } else if (TYPE == SYN_Q4_0) {  // dim = 16 s + 4 t + e
+                k = 2 * ((lane >> 2) & 3) + (lane & 1) + 8 * ((lane >> 1) & 1);
+            }
+            const float y = x[b] * up;
+            const __half hi = __float2half_rn(y);
+            const __half lo = __float2half_rn(y - __half2float(hi));
+            unsigned char* at = smem + r * P::q_pitch + (32 * b + 16 * s + k) * 2;
+            *reinterpret_cast<__half*>(at) = hi;
+            *reinterpret_cast<__half*>(at + R * P::q_pitch) = lo;
+        }
+    }
+    __syncthreads();
+
+    const uint32_t q_s = smem_addr(smem) + (lane & 15) * P::q_pitch + (lane >> 4) * 16;
+    uint32_t qh[kQReg ? KS : 1][4], ql[kQReg ? KS : 1][4];
+    if (kQReg) {
+#pragma unroll
+        for (int k = 0; k < KS; ++k) {
+            ldsm4(qh[k], q_s + k * 32);
+            ldsm4(ql[k], q_s + R * P::q_pitch + k * 32);
+        }
+    }
+    float rs[MT][2], m[MT][2], l[MT][2], o[MT][HDP / 8][4];
+    int tok[MT][2];
+#pragma unroll
+    for (int i = 0; i < MT; ++i) {
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+            rs[i][u] = row_scale[16 * i + 8 * u + g];
+            tok[i][u] = (row0 + 16 * i + 8 * u + g) / a.group;
+            m[i][u] = -INFINITY;
+            l[i][u] = 0.0f;
+        }
+#pragma unroll
+        for (int n = 0; n < HDP / 8; ++n)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) o[i][n][e] = 0.0f;
+    }
+
+    // --- the steps of this warp ----------------------------------------------------
+    int stage = 0;
+    for (int step = s0 + warp; step < s1; step += kWarps) {
+        cp_wait<P::stages - 2>();
+        __syncwarp();
+        {
+            int to = stage + P::stages - 1;
+            if (to >= P::stages) to -= P::stages;
+            if (next < s1) load(next, to);
+            cp_commit();
+            next += kWarps;
+        }
+        unsigned char* st = my_ring + stage * S::bytes;
+        const uint32_t st_s = ring_s + stage * S::bytes;
+        const int p0 = step * kStep;
+
+        // scores of 16 positions: n-tile u holds positions p0 + 8 u + {2t, 2t + 1}
+        float s[MT][2][4];
+#pragma unroll
+        for (int i = 0; i < MT; ++i)
+#pragma unroll
+            for (int u = 0; u < 2; ++u)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) s[i][u][e] = 0.0f;
+        float vm[kQuant ? NB : 1][4];   // V scales' mantissas of positions 2t, 2t + 1, 2t + 8, 2t + 9
+        uint32_t ve[kQuant ? NB : 1][2];  // and their powers of two, as binary16 pairs
+        if constexpr (!kQuant) {
+#pragma unroll
+            for (int k = 0; k < KS; ++k) {
+                uint32_t b[4];  // (n-tile 0: b0, b1), (n-tile 1: b0, b1)
+                ldsm4(b, st_s + ((lane & 7) + ((lane >> 4) << 3)) * S::k_pitch + k * 32 + ((lane >> 3) & 1) * 16);
+#pragma unroll
+                for (int i = 0; i < MT; ++i) {
+                    uint32_t ah[4], al[4];
+                    if (!kQReg) {
+                        ldsm4(ah, q_s + 16 * i * P::q_pitch + k * 32);
+                        ldsm4(al, q_s + (R + 16 * i) * P::q_pitch + k * 32);
+                    }
+                    mma(s[i][0], kQReg ? qh[kQReg ? k : 0] : ah, b[0], b[1]);
+                    mma(s[i][1], kQReg ? qh[kQReg ? k : 0] : ah, b[2], b[3]);
+                    mma(s[i][0], kQReg ? ql[kQReg ? k : 0] : al, b[0], b[1]);
+                    mma(s[i][1], kQReg ? ql[kQReg ? k : 0] : al, b[2], b[3]);
+                }
+            }
+        } else {
+            // the scales of this lane's positions; a position past the context has scales of 0, one whose
+            // V scale is not finite scores NaN (rows that do not see it mask that)
+            float kd[NB][4];
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                const int r = 2 * t + (j & 1) + 8 * (j >> 1);
+                const bool in = p0 + r < total;
+                const uint16_t* sk = reinterpret_cast<const uint16_t*>(st + S::sk_at + scale_off) + r * nb;
+                const uint16_t* sv = reinterpret_cast<const uint16_t*>(st + S::sv_at + scale_off) + r * nb;
+#pragma unroll
+                for (int b = 0; b < NB; ++b) {
+                    const bool ok = in && b < nb;
+                    const uint32_t dk = ok ? sk[b] : 0u, dv = ok ? sv[b] : 0u;
+                    kd[b][j] = f16_from_bits(uint16_t(dk));
+                    const bool finite = (dv & 0x7c00u) != 0x7c00u;
+                    if (!finite) kd[b][j] = __uint_as_float(0x7fffffffu);
+                    const uint32_t pow = min(max(dv & 0x7c00u, 0x0400u), 0x6000u);  // 2^-14 .. 2^9: 127 * 2^9 is finite
+                    const float inv = __uint_as_float(0x7f000000u - __float_as_uint(f16_from_bits(uint16_t(pow))));
+                    vm[b][j] = finite ? f16_from_bits(uint16_t(dv)) * inv : 0.0f;
+                    const uint32_t p = finite ? pow : 0x0400u;
+                    ve[b][j >> 1] = (j & 1) ? (ve[b][j >> 1] | p << 16) : p;
+                }
+            }
+#pragma unroll
+            for (int b = 0; b < NB; ++b) {
+                float c[MT][2][4];
+#pragma unroll
+                for (int i = 0; i < MT; ++i)
+#pragma unroll
+                    for (int u = 0; u < 2; ++u)
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) c[i][u][e] = 0.0f;
+                uint32_t w[2][2];  // [n-tile][product of 16 dims]: four quants as bytes
+#pragma unroll
+                for (int u = 0; u < 2; ++u) {
+                    const unsigned char* at = st + (8 * u + g) * S::k_pitch;
+                    if (TYPE == SYN_Q8_0) {
+                        const uint2 x = *reinterpret_cast<const uint2*>(at + 32 * b + 8 * t);
+                        w[u][0] = x.x ^ 0x80808080u;
+                        w[u][1] = x.y ^ 0x80808080u;
+                    } else {
+                        const uint32_t x = *reinterpret_cast<const uint32_t*>(at + 16 * b + 4 * t);
+                        w[u][0] = x & 0x0f0f0f0fu;
+                        w[u][1] = (x >> 4) & 0x0f0f0f0fu;
+                    }
+                }
+                const __half2 zero = half2_of(TYPE == SYN_Q8_0 ? 0x64806480u : 0x64086408u);  // 1024 + 128 | 8
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    uint32_t bb[2][2];
+#pragma unroll
+                    for (int u = 0; u < 2; ++u) {
+                        bb[u][0] = bits(__hsub2(bytes_h2(w[u][h], 0x4140), zero));
+                        bb[u][1] = bits(__hsub2(bytes_h2(w[u][h], 0x4342), zero));
+                    }
+#pragma unroll
+                    for (int i = 0; i < MT; ++i) {
+                        const int k = 2 * b + h;
+                        uint32_t ah[4], al[4];
+                        if (!kQReg) {
+                            ldsm4(ah, q_s + 16 * i * P::q_pitch + k * 32);
+                            ldsm4(al, q_s + (R + 16 * i) * P::q_pitch + k * 32);
+                        }
+                        mma(c[i][0], kQReg ? qh[kQReg ? k : 0] : ah, bb[0][0], bb[0][1]);
+                        mma(c[i][1], kQReg ? qh[kQReg ? k : 0] : ah, bb[1][0], bb[1][1]);
+                        mma(c[i][0], kQReg ? ql[kQReg ? k : 0] : al, bb[0][0], bb[0][1]);
+                        mma(c[i][1], kQReg ? ql[kQReg ? k : 0] : al, bb[1][0], bb[1][1]);
+                    }
+                }
+#pragma unroll
+                for (int i = 0; i < MT; ++i)
+#pragma unroll
+                    for (int u = 0; u < 2; ++u)
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) s[i][u][e] = fmaf(c[i][u][e], kd[b][2 * u + (e & 1)], s[i][u][e]);
+            }
+        }
+
+        // the tree's own rows: what a token does not see scores -inf
+        const bool edge = p0 + kStep > len;
+        if (!kQuant && edge) {
+            // V rows of the tree may hold values that are not finite where some token does not see them:
+            // zeroed here (0 * inf is NaN), and the position scores NaN for the tokens that do see it
+            unsigned bad = 0;
+            const int r = lane & 15;
+            if (p0 + r >= len && p0 + r < total) {
+                for (int c = lane >> 4; c < row_bytes / 16; c += 2) {
+                    uint16_t* x = reinterpret_cast<uint16_t*>(st + S::v_at + r * S::v_pitch + c * 16);
+#pragma unroll
+                    for (int e = 0; e < 8; ++e)
+                        if ((x[e] & 0x7c00u) == 0x7c00u) {
+                            x[e] = 0;
+                            bad = 1;
+                        }
+                }
+            }
+            unsigned flags = __ballot_sync(0xffffffffu, bad);
+            flags = (flags | flags >> 16) & 0xffffu;
+            __syncwarp();
+#pragma unroll
+            for (int i = 0; i < MT; ++i)
+#pragma unroll
+                for (int u = 0; u < 2; ++u)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e)
+                        if (flags >> (8 * u + 2 * t + (e & 1)) & 1u) s[i][u][e] = __uint_as_float(0x7fffffffu);
+        }
+#pragma unroll
+        for (int i = 0; i < MT; ++i)
+#pragma unroll
+            for (int u = 0; u < 2; ++u)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) s[i][u][e] *= rs[i][e >> 1];
+        if (edge) {
+#pragma unroll
+            for (int i = 0; i < MT; ++i)
+#pragma unroll
+                for (int u = 0; u < 2; ++u)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        const int j = p0 + 8 * u + 2 * t + (e & 1) - len, tk = tok[i][e >> 1];
+                        bool sees = j < 0;
+                        if (!sees && j < a.n_tree && tk < a.n_tree)
+                            sees = a.mask ? (a.mask[(size_t(seq) * a.n_tree + tk) * a.mask_words + (j >> 5)] >> (j & 31) & 1u)
+                                          : j <= tk;
+                        if (!sees) s[i][u][e] = -INFINITY;
+                    }
+        }
+
+        // running maximum, probabilities, sum
+        uint32_t ph[MT][4], pl[MT][4];
+        float p[MT][2][4];
+#pragma unroll
+        for (int i = 0; i < MT; ++i) {
+            bool grows = false;
+            float mn[2];
+#pragma unroll
+            for (int u = 0; u < 2; ++u) {
+                float x = fmaxf(fmaxf(s[i][0][2 * u], s[i][0][2 * u + 1]), fmaxf(s[i][1][2 * u], s[i][1][2 * u + 1]));
+                x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 1));
+                x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 2));
+                mn[u] = fmaxf(m[i][u], x);
+                grows |= mn[u] > m[i][u];
+            }
+            if (__any_sync(0xffffffffu, grows)) {
+                float f[2];
+#pragma unroll
+                for (int u = 0; u < 2; ++u) {
+                    f[u] = mn[u] > m[i][u] ? ex2(m[i][u] - mn[u]) : 1.0f;  // m = -inf: 0
+                    m[i][u] = mn[u];
+                    l[i][u] *= f[u];
+                }
+#pragma unroll
+                for (int n = 0; n < HDP / 8; ++n)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) o[i][n][e] *= f[e >> 1];
+            }
+#pragma unroll
+            for (int u = 0; u < 2; ++u)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    const float mm = m[i][e >> 1];
+                    p[i][u][e] = ex2(s[i][u][e] - (mm == -INFINITY ? 0.0f : mm) + kPShift);
+                    l[i][e >> 1] += p[i][u][e];
+                }
+        }
+
+        // out += p V
+        if constexpr (!kQuant) {
+#pragma unroll
+            for (int i = 0; i < MT; ++i)
+#pragma unroll
+                for (int u = 0; u < 2; ++u) {
+                    split2(p[i][u][0], p[i][u][1], ph[i][2 * u], pl[i][2 * u]);
+                    split2(p[i][u][2], p[i][u][3], ph[i][2 * u + 1], pl[i][2 * u + 1]);
+                }
+#pragma unroll
+            for (int n = 0; n < HDP / 16; ++n) {
+                uint32_t b[4];
+                ldsm4t(b, st_s + S::v_at + ((lane & 7) + ((lane >> 3) & 1) * 8) * S::v_pitch + n * 32 + (lane >> 4) * 16);
+#pragma unroll
+                for (int i = 0; i < MT; ++i) {
+                    mma(o[i][2 * n], ph[i], b[0], b[1]);
+                    mma(o[i][2 * n + 1], ph[i], b[2], b[3]);
+                    mma(o[i][2 * n], pl[i], b[0], b[1]);
+                    mma(o[i][2 * n + 1], pl[i], b[2], b[3]);
+                }
+            }
+        } else {
+            uint32_t r4[4];  // a block's bytes of 2 positions x 2 dims: (positions 0-7, 8-15) x (dims 0-15, 16-31)
+#pragma unroll
+            for (int b = 0; b < NB; ++b) {
+                if (TYPE == SYN_Q8_0)
+                    ldsm4t(r4, st_s + S::v_at + ((lane & 7) + ((lane >> 3) & 1) * 8) * S::v_pitch + b * 32 + (lane >> 4) * 16);
+                else if ((b & 1) == 0)  // two blocks of 16 bytes
+                    ldsm4t(r4, st_s + S::v_at + ((lane & 7) + ((lane >> 3) & 1) * 8) * S::v_pitch + b * 16 + (lane >> 4) * 16);
+#pragma unroll
+                for (int i = 0; i < MT; ++i)
+#pragma unroll
+                    for (int u = 0; u < 2; ++u) {
+                        split2(p[i][u][0] * vm[b][2 * u], p[i][u][1] * vm[b][2 * u + 1], ph[i][2 * u], pl[i][2 * u]);
+                        split2(p[i][u][2] * vm[b][2 * u], p[i][u][3] * vm[b][2 * u + 1], ph[i][2 * u + 1], pl[i][2 * u + 1]);
+                    }
+                const __half2 zero = half2_of(TYPE == SYN_Q8_0 ? 0x64806480u : 0x64086408u);
+                const __half2 e0 = half2_of(ve[b][0]), e1 = half2_of(ve[b][1]);
+                // n-tile 4 b + 2 half + odd: dims 32 b + 16 half + 2 n + odd
+#pragma unroll
+                for (int half = 0; half < 2; ++half) {
+                    uint32_t x0, x1;  // positions 2t, 2t + 1 | 2t + 8, 2t + 9: bytes (even, odd, even, odd)
+                    if (TYPE == SYN_Q8_0) {
+                        x0 = r4[2 * half] ^ 0x80808080u;
+                        x1 = r4[2 * half + 1] ^ 0x80808080u;
+                    } else {
+                        x0 = (r4[2 * (b & 1)] >> (4 * half)) & 0x0f0f0f0fu;
+                        x1 = (r4[2 * (b & 1) + 1] >> (4 * half)) & 0x0f0f0f0fu;
+                    }
+#pragma unroll
+                    for (int odd = 0; odd < 2; ++odd) {
+                        const uint32_t sel = odd ? 0x4341u : 0x4240u;
+                        const uint32_t b0 = bits(__hmul2(__hsub2(bytes_h2(x0, sel), zero), e0));
+                        const uint32_t b1 = bits(__hmul2(__hsub2(bytes_h2(x1, sel), zero), e1));
+#pragma unroll
+                        for (int i = 0; i < MT; ++i) {
+                            mma(o[i][4 * b + 2 * half + odd], ph[i], b0, b1);
+                            mma(o[i][4 * b + 2 * half + odd], pl[i], b0, b1);
+                        }
+                    }
+                }
+            }
+        }
+        if (++stage == P::stages) stage = 0;
+    }
+    cp_wait<0>();
+    __syncthreads();  // every warp is done with the ring
+
+    // --- the warps' results joined --------------------------------------------------
+    float* jo = reinterpret_cast<float*>(ring);       // [kWarps][R][o_pitch]
+    float* jm = jo + kWarps * R * P::o_pitch;          // [kWarps][R]
+    float* jl = jm + kWarps * R;
+#pragma unroll
+    for (int i = 0; i < MT; ++i)
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+            float sum = l[i][u];
+            sum += __shfl_xor_sync(0xffffffffu, sum, 1);
+            sum += __shfl_xor_sync(0xffffffffu, sum, 2);
+            const int r = 16 * i + 8 * u + g;
+            if (t == 0) {
+                jm[warp * R + r] = m[i][u];
+                jl[warp * R + r] = sum;
+            }
+            float* at = jo + (warp * R + r) * P::o_pitch;
+            if constexpr (!kQuant) {
+#pragma unroll
+                for (int n = 0; n < HDP / 8; ++n)
+                    *reinterpret_cast<float2*>(at + 8 * n + 2 * t) = make_float2(o[i][n][2 * u], o[i][n][2 * u + 1]);
+            } else {
+#pragma unroll
+                for (int n = 0; n < HDP / 16; ++n)  // (even, odd) n-tiles hold dims 4t, 4t + 2 and 4t + 1, 4t + 3
+                    *reinterpret_cast<float4*>(at + 16 * n + 4 * t) =
+                        make_float4(o[i][2 * n][2 * u], o[i][2 * n + 1][2 * u], o[i][2 * n][2 * u + 1], o[i][2 * n + 1][2 * u + 1]);
+            }
+        }
+    __syncthreads();
+    const int part_floats = R * (hd + 2);
+    const size_t unit = size_t(seq) * gridDim.y + blockIdx.y;
+    float* part = a.parts + (unit * a.splits + blockIdx.x) * part_floats;
+    for (int r = warp; r < rows; r += kWarps) {
+        float mx = -INFINITY;
+#pragma unroll
+        for (int w = 0; w < kWarps; ++w) mx = fmaxf(mx, jm[w * R + r]);
+        float f[kWarps], sum = 0.0f;
+#pragma unroll
+        for (int w = 0; w < kWarps; ++w) {
+            const float mw = jm[w * R + r];
+            f[w] = mw == -INFINITY ? (jl[w * R + r] != jl[w * R + r] ? 1.0f : 0.0f) : ex2(mw - mx);  // a NaN sum stays
+            sum += f[w] * jl[w * R + r];
+        }
+        const int row = row0 + r, tk = row / a.group, h = kvh * a.group + row - tk * a.group;
+        float* out = a.out + (size_t(seq) * a.n_tree + tk) * a.n_head * hd + size_t(h) * hd;
+        const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
+        for (int d = lane; d < hd; d += 32) {
+            float acc = 0.0f;
+#pragma unroll
+            for (int w = 0; w < kWarps; ++w) acc += f[w] * jo[(w * R + r) * P::o_pitch + d];
+            if (active == 1) out[d] = acc * inv;
+            else part[2 * R + r * hd + d] = acc;
+        }
+        if (active > 1 && lane == 0) {
+            part[r] = mx;
+            part[R + r] = sum;
+        }
+    }
+    if (active == 1) return;
+
+    // --- the last of the unit's CTAs joins the splits, in their order ------------------
+    __threadfence();
+    __syncthreads();
+    __shared__ unsigned arrived;
+    if (tid == 0) arrived = atomicAdd(a.counters + unit, 1u);
+    __syncthreads();
+    if (arrived != unsigned(active - 1)) return;
+    __threadfence();
+    if (tid == 0) a.counters[unit] = 0;  // ready for the next call
+    const float* parts = a.parts + unit * a.splits * part_floats;
+    for (int r = warp; r < rows; r += kWarps) {
+        float mx = -INFINITY;
+        for (int x = lane; x < active; x += 32) mx = fmaxf(mx, __ldcg(parts + size_t(x) * part_floats + r));
+        mx = warp_max(mx);
+        float acc[NB] = {}, sum = 0.0f;
+        for (int x = 0; x < active; ++x) {
+            const float* px = parts + size_t(x) * part_floats;
+            const float mw = __ldcg(px + r), lw = __ldcg(px + R + r);
+            const float f = mw == -INFINITY ? (lw != lw ? 1.0f : 0.0f) : ex2(mw - mx);
+            sum += f * lw;
+#pragma unroll
+            for (int b = 0; b < NB; ++b)
+                if (32 * b + lane < hd) acc[b] += f * __ldcg(px + 2 * R + r * hd + 32 * b + lane);
+        }
+        const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
+        const int row = row0 + r, tk = row / a.group, h = kvh * a.group + row - tk * a.group;
+        float* out = a.out + (size_t(seq) * a.n_tree + tk) * a.n_head * hd + size_t(h) * hd;
+#pragma unroll
+        for (int b = 0; b < NB; ++b)
+            if (32 * b + lane < hd) out[32 * b + lane] = acc[b] * inv;
+    }
+}
+
+// How a call is cut: rows of a CTA, CTAs over the rows, splits of the context.
+struct Cut {
+    int R, row_blocks, splits;
+    size_t units;
+};
+Cut cut_of(int n_seq, int n_tree, int n_head, int n_kv, int head_dim, int max_len) {
+    Cut c;
+    const int rows = n_tree * (n_head / n_kv);
+    c.R = rows > 16 && head_dim <= 128 ? 32 : 16;
+    c.row_blocks = (rows + c.R - 1) / c.R;
+    c.units = size_t(n_seq) * n_kv * c.row_blocks;
+    // two CTAs per SM; a split has at least two steps of every warp
+    const size_t target = size_t(2) * syn_num_sms();
+    const int most = (max_len + 2 * kWarps * kStep - 1) / (2 * kWarps * kStep);
+    c.splits = int(std::max<size_t>(1, std::min<size_t>(target / c.units, size_t(most))));
+    if (c.units * sizeof(unsigned) > kCounterBytes) c.splits = 1;
+    return c;
+}
+
+int opt_in(const void* kernel, size_t bytes) {
+    static std::mutex mu;
+    static std::vector<std::pair<const void*, int>> done;
+    int dev = 0;
+    int st = syn_cuda_status(cudaGetDevice(&dev));
+    if (st) return st;
+    std::lock_guard<std::mutex> lock(mu);
+    for (const auto& d : done)
+        if (d.first == kernel && d.second == dev) return SYN_OK;
+    st = syn_cuda_status(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, int(bytes)));
+    if (!st) done.push_back({kernel, dev});
+    return st;
+}
+
+template <int TYPE, int HDP, int MT>
+int launch(const TreeParams& a, cudaStream_t s) {
+    auto kernel = tree_attn_kernel<TYPE, HDP, MT>;
+    constexpr int smem = Plan<TYPE, HDP, MT>::smem;
+    static_assert(smem <= 227 * 1024, "shared memory of a CTA");
+    const int st = opt_in(reinterpret_cast<const void*>(kernel), smem);
+    if (st) return st;
+    const dim3 grid{unsigned(a.splits), unsigned(a.c.n_kv * a.row_blocks), unsigned(a.c.n_seq)};
+    return syn_launch(kernel, grid, kWarps * 32, smem, s, a);
+}
+
+template <int TYPE>
+int launch_type(const TreeParams& a, int R, cudaStream_t s) {
+    if (a.c.hd <= 64) return R == 32 ? launch<TYPE, 64, 2>(a, s) : launch<TYPE, 64, 1>(a, s);
+    if (a.c.hd <= 128) return R == 32 ? launch<TYPE, 128, 2>(a, s) : launch<TYPE, 128, 1>(a, s);
+    return launch<TYPE, 256, 1>(a, s);
+}
+
+}  // namespace
+
+extern "C" size_t syn_tree_attention_scratch_bytes(int n_seq, int n_tree, int n_head, int n_kv, int head_dim,
+                                                   int max_len) {
+    if (n_seq <= 0 || n_tree <= 0 || n_tree > kMaxTree || n_kv <= 0 || n_head <= 0 || n_head % n_kv || head_dim <= 0 ||
+        head_dim > 256 || max_len < n_tree)
+        return 0;
+    const Cut c = cut_of(n_seq, n_tree, n_head, n_kv, head_dim, max_len);
+    return kCounterBytes + (c.splits > 1 ? align256(c.units * c.splits * c.R * (size_t(head_dim) + 2) * 4) : 0);
+}
+
+extern "C" int syn_tree_attention(const syn_kv_cache* c, int layer, const syn_tree_attention_args* x, void* stream) {
+    int st = kv_check(c, layer);
+    if (st) return st;
+    if (!x || !x->q || !x->out || !x->len || !x->scratch) return SYN_ERR_INVALID;
+    if (x->n_head <= 0 || x->n_head % c->n_kv || x->n_tree <= 0) return SYN_ERR_INVALID;
+    if (x->max_len < x->n_tree || x->max_len > c->max_ctx) return SYN_ERR_INVALID;
+    if (x->n_tree > kMaxTree || c->n_seq > 65535) return SYN_ERR_UNSUPPORTED;
+    const size_t q_row = size_t(x->n_head) * c->head_dim;
+    if (x->q_stride && x->q_stride < q_row) return SYN_ERR_INVALID;
+    if (reinterpret_cast<uintptr_t>(x->scratch) & 15) return SYN_ERR_INVALID;
+    const Cut cut = cut_of(c->n_seq, x->n_tree, x->n_head, c->n_kv, c->head_dim, x->max_len);
+    if (size_t(c->n_kv) * cut.row_blocks > 65535) return SYN_ERR_UNSUPPORTED;
+    TreeParams a{};
+    a.c = kv_view(c, layer);
+    a.q = x->q; a.out = x->out; a.len = x->len; a.mask = x->mask;
+    a.counters = static_cast<unsigned*>(x->scratch);
+    a.parts = reinterpret_cast<float*>(static_cast<char*>(x->scratch) + kCounterBytes);
+    a.q_stride = x->q_stride ? x->q_stride : q_row;
+    a.n_tree = x->n_tree; a.n_head = x->n_head;
+    a.group = x->n_head / c->n_kv;
+    a.rows = x->n_tree * a.group;
+    a.row_blocks = cut.row_blocks;
+    a.max_len = x->max_len;
+    a.mask_words = (x->n_tree + 31) / 32;
+    a.splits = cut.splits;
+    a.scale_log2 = x->scale * 1.4426950408889634f;
+    cudaStream_t s = static_cast<cudaStream_t>(stream);
+    if (c->type == SYN_F16) return launch_type<SYN_F16>(a, cut.R, s);
+    if (c->type == SYN_Q8_0) return launch_type<SYN_Q8_0>(a, cut.R, s);
+    return launch_type<SYN_Q4_0>(a, cut.R, s);
+}
