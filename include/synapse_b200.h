@@ -331,7 +331,7 @@ int syn_kv_move(const syn_kv_cache* c, const int32_t* path, int path_ld, const i
  * shape); calls whose GPU work overlaps need scratches of their own. */
 typedef struct {
     const float* q;          /* [n_seq * n_tree][n_head * head_dim], rotated */
-    float* out;              /* contiguous [n_seq * n_tree][n_head * head_dim] */
+    float* out;              /* contiguous [n_seq * n_tree][n_head * head_dim], 16-byte aligned */
     const int32_t* len;      /* [n_seq] device: rows committed before the tree's */
     const uint32_t* mask;    /* NULL, or [n_seq][n_tree][(n_tree + 31) / 32] device */
     void* scratch;

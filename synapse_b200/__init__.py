@@ -162,11 +162,17 @@ def check(status, where):
 # ---------------------------------------------------------------------------
 # torch helpers (device memory and streams only)
 
+_torch_module = None
+
+
 def _torch():
-    import torch
-    if not torch.cuda.is_available():
-        raise RuntimeError("synapse_b200 needs a CUDA GPU (B200); there is no CPU path")
-    return torch
+    global _torch_module
+    if _torch_module is None:
+        import torch
+        if not torch.cuda.is_available():
+            raise RuntimeError("synapse_b200 needs a CUDA GPU (B200); there is no CPU path")
+        _torch_module = torch
+    return _torch_module
 
 
 def _ptr(t):

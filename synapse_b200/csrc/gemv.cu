@@ -1093,8 +1093,8 @@ extern "C" int syn_check_tp_wait(unsigned wait_us, int* errors) {
 extern "C" int syn_device_errors(void) {
     unsigned n = 0;
     if (cudaMemcpyFromSymbol(&n, g_gemv_timeouts, sizeof n) != cudaSuccess) return -1;
-    const int a = syn_attn_timeouts();
-    return a < 0 ? -1 : int(n) + a;
+    const int a = syn_attn_timeouts(), t = syn_tree_timeouts();
+    return a < 0 || t < 0 ? -1 : int(n) + a + t;
 }
 
 extern "C" int syn_gemv_f(int type, const void* w, int rows, int cols, const float* x, int n_tok, float* y,

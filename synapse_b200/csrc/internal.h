@@ -97,6 +97,7 @@ int syn_tp_step_begin(unsigned* epoch, cudaStream_t s);
 
 // Bounded waits of the attention kernels that gave up on the current device (-1: unreadable).
 int syn_attn_timeouts();
+int syn_tree_timeouts();  // the same of the tree attention kernel
 // Device addresses (current device) of the counters of bounded copy waits that
 // gave up in the GEMV and attention kernels, for a session to copy out after
 // every step; NULL if they cannot be looked up.

@@ -22,7 +22,7 @@
 // the sum over blocks of scale * (q . quants); for V the block's scale is
 // m * 2^e, 2^e <= 2^9 applied to the integers (exact) and m (in [1, 2) for all
 // but extreme scales) to the float probabilities before they are split, so no value is rounded to binary16.
-#include "kv_cache.cuh"
+#include "tree_attention.cuh"
 
 #include <algorithm>
 #include <mutex>
@@ -34,31 +34,7 @@ namespace {
 
 constexpr int kWarps = 4;
 constexpr int kStep = 16;            // positions per step of a warp
-constexpr float kPShift = 8.0f;      // probabilities carry 2^8, away from binary16's subnormals
 constexpr size_t kCounterBytes = 16384;  // arrival counters at the start of the scratch
-constexpr int kMaxTree = 1024;
-
-struct TreeParams {
-    KvView c;
-    const float* q;
-    float* out;
-    const int32_t* len;
-    const uint32_t* mask;
-    unsigned* counters;  // [n_seq][n_kv * row blocks]
-    float* parts;        // [n_seq][n_kv * row blocks][splits]: m[R], l[R], o[R][hd]
-    size_t q_stride;
-    int n_tree, n_head, group, rows, row_blocks, max_len, mask_words, splits;
-    float scale_log2;    // scale * log2(e)
-};
-
-__device__ __forceinline__ void cp16(uint32_t dst, const void* src, bool in) {
-    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(in ? 16 : 0) : "memory");
-}
-__device__ __forceinline__ void cp_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
-template <int N>
-__device__ __forceinline__ void cp_wait() {
-    asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
-}
 __device__ __forceinline__ void ldsm4(uint32_t (&r)[4], uint32_t addr) {
     asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
                  : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
@@ -76,23 +52,6 @@ __device__ __forceinline__ void mma(float (&c)[4], const uint32_t (&a)[4], uint3
         : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
         : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
-__device__ __forceinline__ float ex2(float x) {
-    float y;
-    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-    return y;
-}
-__device__ __forceinline__ uint32_t bits(__half2 h) { return *reinterpret_cast<uint32_t*>(&h); }
-__device__ __forceinline__ __half2 half2_of(uint32_t u) { return *reinterpret_cast<__half2*>(&u); }
-// (x, y) as binary16 pairs hi + lo.
-__device__ __forceinline__ void split2(float x, float y, uint32_t& hi, uint32_t& lo) {
-    const __half2 h = __floats2half2_rn(x, y);
-    const float2 f = __half22float2(h);
-    hi = bits(h);
-    lo = bits(__floats2half2_rn(x - f.x, y - f.y));
-}
-// Bytes i and j of x as binary16 integers 1024 + byte.
-__device__ __forceinline__ __half2 bytes_h2(uint32_t x, uint32_t sel) { return half2_of(__byte_perm(x, 0x64646464u, sel)); }
-
 // Shared memory of one warp's stage: K rows, V rows (pitches keep the
 // fragment reads free of bank conflicts), then the scales of the 16 positions.
 template <int TYPE, int HDP>
@@ -209,11 +168,8 @@ __global__ void __launch_bounds__(kWarps * 32, 2) tree_attn_kernel(const TreePar
             m = fmaxf(m, fabsf(x[b]));
         }
         m = warp_max(m);
-        // 2^e <= m < 2^(e+1); zero, subnormal and non-finite rows keep a factor of 1 * 2^8
-        const int e = int(__float_as_uint(m) >> 23);
-        const bool plain = e < 32 || e > 250;
-        const float up = plain ? 256.0f : __uint_as_float(uint32_t(254 + 8 - e) << 23);
-        const float down = plain ? 1.0f / 256.0f : __uint_as_float(uint32_t(e - 8) << 23);
+        float up, down;
+        q_factor(m, up, down);
         if (lane == 0) row_scale[r] = a.scale_log2 * down;
 #pragma unroll
         for (int b = 0; b < NB; ++b) {
@@ -426,11 +382,8 @@ __global__ void __launch_bounds__(kWarps * 32, 2) tree_attn_kernel(const TreePar
                 for (int u = 0; u < 2; ++u)
 #pragma unroll
                     for (int e = 0; e < 4; ++e) {
-                        const int j = p0 + 8 * u + 2 * t + (e & 1) - len, tk = tok[i][e >> 1];
-                        bool sees = j < 0;
-                        if (!sees && j < a.n_tree && tk < a.n_tree)
-                            sees = a.mask ? (a.mask[(size_t(seq) * a.n_tree + tk) * a.mask_words + (j >> 5)] >> (j & 31) & 1u)
-                                          : j <= tk;
+                        const int j = p0 + 8 * u + 2 * t + (e & 1) - len;
+                        const bool sees = j < 0 || tree_sees(a, seq, tok[i][e >> 1], j);
                         if (!sees) s[i][u][e] = -INFINITY;
                     }
         }
@@ -580,8 +533,7 @@ __global__ void __launch_bounds__(kWarps * 32, 2) tree_attn_kernel(const TreePar
         float f[kWarps], sum = 0.0f;
 #pragma unroll
         for (int w = 0; w < kWarps; ++w) {
-            const float mw = jm[w * R + r];
-            f[w] = mw == -INFINITY ? (jl[w * R + r] != jl[w * R + r] ? 1.0f : 0.0f) : ex2(mw - mx);  // a NaN sum stays
+            f[w] = part_weight(jm[w * R + r], jl[w * R + r], mx);
             sum += f[w] * jl[w * R + r];
         }
         const int row = row0 + r, tk = row / a.group, h = kvh * a.group + row - tk * a.group;
@@ -619,7 +571,7 @@ __global__ void __launch_bounds__(kWarps * 32, 2) tree_attn_kernel(const TreePar
         for (int x = 0; x < active; ++x) {
             const float* px = parts + size_t(x) * part_floats;
             const float mw = __ldcg(px + r), lw = __ldcg(px + R + r);
-            const float f = mw == -INFINITY ? (lw != lw ? 1.0f : 0.0f) : ex2(mw - mx);
+            const float f = part_weight(mw, lw, mx);
             sum += f * lw;
 #pragma unroll
             for (int b = 0; b < NB; ++b)
@@ -636,24 +588,62 @@ __global__ void __launch_bounds__(kWarps * 32, 2) tree_attn_kernel(const TreePar
 
 // How a call is cut: rows of a CTA, CTAs over the rows, splits of the context.
 struct Cut {
+    bool tc;
     int R, row_blocks, splits;
     size_t units;
 };
 Cut cut_of(int n_seq, int n_tree, int n_head, int n_kv, int head_dim, int max_len) {
     Cut c;
     const int rows = n_tree * (n_head / n_kv);
-    c.R = rows > 16 && head_dim <= 128 ? 32 : 16;
+    const size_t sms = size_t(syn_num_sms());
+    c.tc = rows > 16 && head_dim <= 128;
+    c.R = c.tc ? kTcRows : 16;
     c.row_blocks = (rows + c.R - 1) / c.R;
     c.units = size_t(n_seq) * n_kv * c.row_blocks;
-    // two CTAs per SM; a split has at least two steps of every warp
-    const size_t target = size_t(2) * syn_num_sms();
-    const int most = (max_len + 2 * kWarps * kStep - 1) / (2 * kWarps * kStep);
-    c.splits = int(std::max<size_t>(1, std::min<size_t>(target / c.units, size_t(most))));
+    if (c.tc) {
+        // one CTA per SM: the split of the tiles whose last wave ends first
+        const int tiles = (max_len + kTcTile - 1) / kTcTile;
+        size_t best = ~size_t(0);
+        c.splits = 1;
+        for (int n = 1; n <= std::min(tiles, 128); ++n) {
+            const size_t waves = (c.units * n + sms - 1) / sms, per = size_t(tiles + n - 1) / n;
+            const size_t cost = waves * (per + 8);  // a CTA's start and end take about 8 tiles
+            if (cost < best) {
+                best = cost;
+                c.splits = n;
+            }
+        }
+    } else {
+        // two CTAs per SM; a split has at least two steps of every warp
+        const int most = (max_len + 2 * kWarps * kStep - 1) / (2 * kWarps * kStep);
+        c.splits = int(std::max<size_t>(1, std::min<size_t>(2 * sms / c.units, size_t(most))));
+    }
     if (c.units * sizeof(unsigned) > kCounterBytes) c.splits = 1;
     return c;
 }
 
-int opt_in(const void* kernel, size_t bytes) {
+template <int TYPE, int HDP, int MT>
+int launch(const TreeParams& a, cudaStream_t s) {
+    auto kernel = tree_attn_kernel<TYPE, HDP, MT>;
+    constexpr int smem = Plan<TYPE, HDP, MT>::smem;
+    static_assert(smem <= 227 * 1024, "shared memory of a CTA");
+    const int st = syn_opt_in_smem(reinterpret_cast<const void*>(kernel), smem);
+    if (st) return st;
+    const dim3 grid{unsigned(a.splits), unsigned(a.c.n_kv * a.row_blocks), unsigned(a.c.n_seq)};
+    return syn_launch(kernel, grid, kWarps * 32, smem, s, a);
+}
+
+template <int TYPE>
+int launch_type(const TreeParams& a, cudaStream_t s) {
+    if (a.c.hd <= 64) return launch<TYPE, 64, 1>(a, s);
+    if (a.c.hd <= 128) return launch<TYPE, 128, 1>(a, s);
+    return launch<TYPE, 256, 1>(a, s);
+}
+
+}  // namespace
+
+// The dynamic shared memory opt-in of a kernel, once per device.
+int syn_opt_in_smem(const void* kernel, size_t bytes) {
     static std::mutex mu;
     static std::vector<std::pair<const void*, int>> done;
     int dev = 0;
@@ -666,26 +656,6 @@ int opt_in(const void* kernel, size_t bytes) {
     if (!st) done.push_back({kernel, dev});
     return st;
 }
-
-template <int TYPE, int HDP, int MT>
-int launch(const TreeParams& a, cudaStream_t s) {
-    auto kernel = tree_attn_kernel<TYPE, HDP, MT>;
-    constexpr int smem = Plan<TYPE, HDP, MT>::smem;
-    static_assert(smem <= 227 * 1024, "shared memory of a CTA");
-    const int st = opt_in(reinterpret_cast<const void*>(kernel), smem);
-    if (st) return st;
-    const dim3 grid{unsigned(a.splits), unsigned(a.c.n_kv * a.row_blocks), unsigned(a.c.n_seq)};
-    return syn_launch(kernel, grid, kWarps * 32, smem, s, a);
-}
-
-template <int TYPE>
-int launch_type(const TreeParams& a, int R, cudaStream_t s) {
-    if (a.c.hd <= 64) return R == 32 ? launch<TYPE, 64, 2>(a, s) : launch<TYPE, 64, 1>(a, s);
-    if (a.c.hd <= 128) return R == 32 ? launch<TYPE, 128, 2>(a, s) : launch<TYPE, 128, 1>(a, s);
-    return launch<TYPE, 256, 1>(a, s);
-}
-
-}  // namespace
 
 extern "C" size_t syn_tree_attention_scratch_bytes(int n_seq, int n_tree, int n_head, int n_kv, int head_dim,
                                                    int max_len) {
@@ -705,7 +675,7 @@ extern "C" int syn_tree_attention(const syn_kv_cache* c, int layer, const syn_tr
     if (x->n_tree > kMaxTree || c->n_seq > 65535) return SYN_ERR_UNSUPPORTED;
     const size_t q_row = size_t(x->n_head) * c->head_dim;
     if (x->q_stride && x->q_stride < q_row) return SYN_ERR_INVALID;
-    if (reinterpret_cast<uintptr_t>(x->scratch) & 15) return SYN_ERR_INVALID;
+    if ((reinterpret_cast<uintptr_t>(x->scratch) | reinterpret_cast<uintptr_t>(x->out)) & 15) return SYN_ERR_INVALID;
     const Cut cut = cut_of(c->n_seq, x->n_tree, x->n_head, c->n_kv, c->head_dim, x->max_len);
     if (size_t(c->n_kv) * cut.row_blocks > 65535) return SYN_ERR_UNSUPPORTED;
     TreeParams a{};
@@ -723,7 +693,8 @@ extern "C" int syn_tree_attention(const syn_kv_cache* c, int layer, const syn_tr
     a.splits = cut.splits;
     a.scale_log2 = x->scale * 1.4426950408889634f;
     cudaStream_t s = static_cast<cudaStream_t>(stream);
-    if (c->type == SYN_F16) return launch_type<SYN_F16>(a, cut.R, s);
-    if (c->type == SYN_Q8_0) return launch_type<SYN_Q8_0>(a, cut.R, s);
-    return launch_type<SYN_Q4_0>(a, cut.R, s);
+    if (cut.tc) return syn_tree_attention_tc(a, c->type, s);
+    if (c->type == SYN_F16) return launch_type<SYN_F16>(a, s);
+    if (c->type == SYN_Q8_0) return launch_type<SYN_Q8_0>(a, s);
+    return launch_type<SYN_Q4_0>(a, s);
 }

@@ -1,0 +1,596 @@
+// syn_tree_attention on tcgen05: a CTA takes 128 rows (token * G + head) of a
+// KV head and a run of the context in tiles of 64 positions.
+//
+// For a tile, S = Q K^T (128 x 64) and O = P V (128 x head_dim) are products
+// with the A operand in tensor memory (Q for the whole call; P where S was)
+// and the tile in shared memory. As in the other kernel q and the
+// probabilities are two binary16 terms each, so S takes two products and O
+// two; a quantised tile is also two terms (its scale, brought to a common
+// power of two per tile, times its integers: 18 bits), so S and O take three
+// (the product of the two low terms is under 2^-22). A tile's O is read from
+// tensor memory and added to float registers, because sums in the tensor
+// core's accumulators lose a little with every product.
+//
+// Warps: 0-3 softmax (a thread owns a row: no exchange between lanes), 4-7
+// and 8-11 the two halves of O, 12-15 fill the tiles (F16: asynchronous
+// copies; quantised: integers to binary16), 16 issues the products. Tensor
+// memory: Q high | Q low | two S (then P) | two O.
+//
+// Bound: the products take 16 (F16) or 24 cycles per position and KV head
+// whatever the number of rows up to 128, against 22 (F16), 12 (Q8_0) or 6
+// (Q4_0) for the cache's bytes at head_dim 128.
+#include "tcgen05.cuh"
+#include "tree_attention.cuh"
+
+using namespace syn;
+
+namespace {
+
+constexpr int kTcThreads = 17 * 32;
+constexpr uint64_t kTcWaitNs = 2000000000ull;  // a wait gives up after 2 s
+constexpr int kEdgeTiles = kMaxTree / kTcTile + 2;  // tiles that hold rows of the tree
+
+__device__ unsigned g_tree_timeouts = 0;  // bounded waits that gave up (syn_device_errors)
+
+template <int TYPE, int HDP>
+struct TcPlan {
+    static constexpr bool quant = TYPE != SYN_F16;
+    static constexpr int atom = kTcTile * 128;          // 64 positions x 64 dims
+    static constexpr int tile = atom * (HDP / 64);      // one term of K or V
+    static constexpr int k_lo = tile, v_hi = quant ? 2 * tile : tile;  // V's low term follows its high one
+    static constexpr int stage = quant ? 4 * tile : 2 * tile;
+    static constexpr int stages = quant ? (HDP == 64 ? 4 : 3) : 5;
+    static constexpr int smem = stages * stage + 1024;  // from a 1024-byte boundary
+    // tensor memory columns
+    static constexpr int q_hi = 0, q_lo = HDP / 2, s = HDP, o = HDP + 2 * kTcTile;
+    static_assert(o + 2 * HDP <= 512, "tensor memory");
+};
+
+struct TcShared {
+    uint64_t q_full, kv_full[5], kv_empty[5], s_full[2], p_full[4], o_full[2], o_empty[2], done;
+    unsigned long long bad[kEdgeTiles];  // positions of a tree tile that hold values that are not finite
+    float corr[4][kTcRows];              // a tile's factor of the rows' sums so far
+    float v_factor[4];                   // and of its O
+    float k_scale[8], v_scale[8];        // powers of two of a tile's terms
+    float m[kTcRows], l[kTcRows];
+    unsigned top[2][2][4];               // the fill warps' largest scales
+    uint32_t tmem;
+    unsigned arrived;
+    int abort;
+};
+
+// Waits for phase `parity`; false when it gave up, here or in another thread of the CTA.
+__device__ __forceinline__ bool tc_wait(uint64_t* bar, uint32_t parity, TcShared& sh) {
+    if (mbar_try_wait(bar, parity)) return true;
+    const uint64_t t0 = global_ns();
+    for (;;) {
+        if (mbar_try_wait(bar, parity)) return true;
+        if (*reinterpret_cast<volatile int*>(&sh.abort)) return false;
+        if (global_ns() - t0 > kTcWaitNs) {
+            *reinterpret_cast<volatile int*>(&sh.abort) = 1;
+            atomicAdd(&g_tree_timeouts, 1u);
+            return false;
+        }
+    }
+}
+__device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity, TcShared& sh) {
+    return __all_sync(0xffffffffu, tc_wait(bar, parity, sh));
+}
+
+// Byte offset of 16-byte chunk c (8 dims) of position p in a swizzled tile.
+__device__ __forceinline__ int tile_at(int p, int c) { return (c >> 3) * (kTcTile * 128) + p * 128 + (((c & 7) ^ (p & 7)) << 4); }
+
+// The tile's positions that token tk sees: bit p for the tree's row j0 + p (a committed row where that is negative).
+__device__ __forceinline__ unsigned long long tile_sees(const TreeParams& a, int seq, int tk, int j0) {
+    uint32_t w[3];
+    const int first = j0 >> 5, shift = j0 & 31;
+#pragma unroll
+    for (int i = 0; i < 3; ++i) {
+        const int wi = first + i, left = a.n_tree - 32 * wi;  // rows of the tree from this word on
+        if (wi < 0) {
+            w[i] = 0xffffffffu;
+        } else if (left <= 0 || tk >= a.n_tree) {
+            w[i] = 0;
+        } else {
+            const int most = a.mask ? left : min(left, tk + 1 - 32 * wi);
+            w[i] = most <= 0 ? 0u : a.mask ? __ldg(a.mask + (size_t(seq) * a.n_tree + tk) * a.mask_words + wi) : 0xffffffffu;
+            if (most > 0 && most < 32) w[i] &= (1u << most) - 1u;
+        }
+    }
+    return (unsigned long long)(__funnelshift_r(w[1], w[2], shift)) << 32 | __funnelshift_r(w[0], w[1], shift);
+}
+
+template <int TYPE, int HDP>
+__global__ void __launch_bounds__(kTcThreads, 1) tree_attn_tc_kernel(const TreeParams a) {
+    using P = TcPlan<TYPE, HDP>;
+    extern __shared__ unsigned char raw[];
+    __shared__ TcShared sh;
+    unsigned char* tiles = raw + ((1024 - (smem_addr(raw) & 1023)) & 1023);
+    const uint32_t tiles_s = smem_addr(tiles);
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    const int hd = a.c.hd;
+    const int kvh = blockIdx.y / a.row_blocks, rb = blockIdx.y - kvh * a.row_blocks, seq = blockIdx.z;
+    const int row0 = rb * kTcRows, rows = min(kTcRows, a.rows - row0);
+
+    pdl_launch_dependents();
+    pdl_wait();
+    const int len = min(max(a.len[seq], 0), a.max_len - a.n_tree);
+    const int total = len + a.n_tree;
+    const int n_tiles = (total + kTcTile - 1) / kTcTile;
+    const int per = (n_tiles + a.splits - 1) / a.splits;
+    const int active = (n_tiles + per - 1) / per;
+    const int t0 = blockIdx.x * per, n = min(per, n_tiles - t0);  // tiles t0 .. t0 + n - 1
+    if (n <= 0) return;
+    const int edge0 = len / kTcTile;  // the first tile with a row of the tree
+
+    if (tid == 0) {
+        mbar_init(&sh.q_full, 128);
+        for (int i = 0; i < P::stages; ++i) {
+            mbar_init(&sh.kv_full[i], 4);
+            mbar_init(&sh.kv_empty[i], 1);
+        }
+        for (int i = 0; i < 2; ++i) {
+            mbar_init(&sh.s_full[i], 1);
+            mbar_init(&sh.o_full[i], 1);
+            mbar_init(&sh.o_empty[i], 256);
+        }
+        for (int i = 0; i < 4; ++i) mbar_init(&sh.p_full[i], 128);
+        mbar_init(&sh.done, 1);
+        mbar_init_fence();
+        sh.abort = 0;
+    }
+    if (tid < kEdgeTiles) sh.bad[tid] = 0;
+    if (warp == 16) tmem_alloc_all(&sh.tmem);
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tm = sh.tmem;
+
+    if (warp < 4) {
+        // ---- softmax: thread = row -------------------------------------------------
+        const bool live = 32 * warp < rows;  // the warp has rows
+        const int r = tid, row = row0 + r;
+        const int tok = row / a.group;
+        const uint32_t lanes = tm + (uint32_t(32 * warp) << 16);
+        float c = 0.0f;
+        if (live) {
+            // the warp's 32 rows, a row at a time (lane = dims), split into the tile memory that the fill warps leave
+            // free until q_full; then each thread's row to tensor memory
+            constexpr int V = HDP / 32, pitch = HDP * 2 + 16;
+            unsigned char* mine = tiles + P::stage + warp * 64 * pitch;
+            const bool vec = V == 4 && ((reinterpret_cast<uintptr_t>(a.q) & 15) | (a.q_stride & 3)) == 0;
+            for (int i0 = 0; i0 < 32; i0 += 8) {
+                float x[8][V];
+#pragma unroll
+                for (int i = 0; i < 8; ++i) {
+                    const int rr = 32 * warp + i0 + i, qrow = row0 + rr, qt = qrow / a.group, qh = qrow - qt * a.group;
+                    const float* q = a.q + (size_t(seq) * a.n_tree + qt) * a.q_stride + size_t(kvh * a.group + qh) * hd + lane * V;
+#pragma unroll
+                    for (int e = 0; e < V; ++e) x[i][e] = 0.0f;
+                    if (rr < rows && lane * V < hd) {
+                        if constexpr (V == 4) {
+                            if (vec) {
+                                const float4 f = __ldg(reinterpret_cast<const float4*>(q));
+                                x[i][0] = f.x; x[i][1] = f.y; x[i][2] = f.z; x[i][3] = f.w;
+                            }
+                        }
+                        if (!vec)
+#pragma unroll
+                            for (int e = 0; e < V; ++e) x[i][e] = __ldg(q + e);
+                    }
+                }
+#pragma unroll
+                for (int i = 0; i < 8; ++i) {
+                    uint32_t top = 0;
+#pragma unroll
+                    for (int e = 0; e < V; ++e) top = max(top, __float_as_uint(fabsf(x[i][e])));
+                    float up, down;
+                    q_factor(__uint_as_float(__reduce_max_sync(0xffffffffu, top)), up, down);
+                    if (lane == i0 + i) c = a.scale_log2 * down;
+                    unsigned char* at = mine + (i0 + i) * 2 * pitch + lane * V * 2;
+#pragma unroll
+                    for (int e = 0; e < V; e += 2) {
+                        uint32_t hi, lo;
+                        split2(x[i][e] * up, x[i][e + 1] * up, hi, lo);
+                        *reinterpret_cast<uint32_t*>(at + 2 * e) = hi;
+                        *reinterpret_cast<uint32_t*>(at + pitch + 2 * e) = lo;
+                    }
+                }
+            }
+            __syncwarp();
+#pragma unroll
+            for (int b = 0; b < HDP / 16; ++b) {  // 16 columns: 32 dims of the high, then of the low term
+                const int term = b / (HDP / 32), at = b % (HDP / 32);
+                uint32_t w[16];
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    const uint4 x = *reinterpret_cast<const uint4*>(mine + (lane * 2 + term) * pitch + at * 64 + e * 16);
+                    w[4 * e] = x.x; w[4 * e + 1] = x.y; w[4 * e + 2] = x.z; w[4 * e + 3] = x.w;
+                }
+                tmem_st16(lanes + (term ? P::q_lo : P::q_hi) + 16 * at, w);
+            }
+            tmem_wait_st();
+        }
+        tc_fence_before();
+        mbar_arrive(&sh.q_full);
+        float m = -INFINITY, l = 0.0f;
+        for (int j = 0; j < n; ++j) {
+            const int t = t0 + j, st = j % P::stages;
+            const bool edge = t >= edge0;
+            bool ok = warp_wait(&sh.s_full[j & 1], uint32_t(j >> 1) & 1, sh);
+            if (ok && (P::quant || edge)) ok = warp_wait(&sh.kv_full[st], uint32_t(j / P::stages) & 1, sh);
+            if (!ok) break;
+            if (live) {
+                tc_fence_after();
+                uint32_t s[2][32];
+                tmem_ld32(s[0], lanes + P::s + (j & 1) * kTcTile);
+                tmem_ld32(s[1], lanes + P::s + (j & 1) * kTcTile + 32);
+                const float cc = P::quant ? c * sh.k_scale[j & 7] : c;
+                tmem_wait_ld();
+                float x = -INFINITY;
+                if (!edge) {
+#pragma unroll
+                    for (int u = 0; u < 2; ++u)
+#pragma unroll
+                        for (int e = 0; e < 32; ++e) {
+                            const float v = __uint_as_float(s[u][e]) * cc;
+                            s[u][e] = __float_as_uint(v);
+                            x = fmaxf(x, v);
+                        }
+                } else {
+                    const unsigned long long bad = sh.bad[t - edge0], sees = tile_sees(a, seq, tok, t * kTcTile - len);
+#pragma unroll
+                    for (int u = 0; u < 2; ++u)
+#pragma unroll
+                        for (int e = 0; e < 32; ++e) {
+                            const int p = 32 * u + e;
+                            float v = __uint_as_float(s[u][e]) * cc;
+                            if (bad >> p & 1ull) v = __uint_as_float(0x7fffffffu);
+                            if (!(sees >> p & 1ull)) v = -INFINITY;
+                            s[u][e] = __float_as_uint(v);
+                            x = fmaxf(x, v);
+                        }
+                }
+                const float mn = fmaxf(m, x);
+                sh.corr[j & 3][r] = mn > m ? ex2(m - mn) : 1.0f;  // m = -inf: 0
+                l *= mn > m ? ex2(m - mn) : 1.0f;
+                m = mn;
+                const float base = (m == -INFINITY ? 0.0f : m) - kPShift;
+                float sum[4] = {};
+#pragma unroll
+                for (int u = 0; u < 2; ++u) {
+                    uint32_t hi[16], lo[16];
+#pragma unroll
+                    for (int e = 0; e < 16; ++e) {
+                        const float p0 = ex2(__uint_as_float(s[u][2 * e]) - base), p1 = ex2(__uint_as_float(s[u][2 * e + 1]) - base);
+                        sum[e & 3] += p0 + p1;
+                        split2(p0, p1, hi[e], lo[e]);
+                    }
+                    tmem_st16(lanes + P::s + (j & 1) * kTcTile + 16 * u, hi);
+                    tmem_st16(lanes + P::s + (j & 1) * kTcTile + 32 + 16 * u, lo);
+                }
+                l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+                if (P::quant && tid == 0) sh.v_factor[j & 3] = sh.v_scale[j & 7];
+                tmem_wait_st();
+            }
+            tc_fence_before();
+            mbar_arrive(&sh.p_full[j & 3]);
+        }
+        sh.m[r] = m;
+        sh.l[r] = l;
+    } else if (warp < 12) {
+        // ---- O: thread = row, half of the dims -----------------------------------------
+        constexpr int W = HDP / 2;
+        const int half = (warp - 4) >> 2, r = (tid - 128) & 127;
+        const bool live = 32 * (warp & 3) < rows;
+        const uint32_t from = tm + (uint32_t(32 * (warp & 3)) << 16) + P::o + half * W;
+        float acc[W];
+#pragma unroll
+        for (int d = 0; d < W; ++d) acc[d] = 0.0f;
+        for (int j = 0; j < n; ++j) {
+            bool ok = warp_wait(&sh.p_full[j & 3], uint32_t(j >> 2) & 1, sh);
+            ok = ok && warp_wait(&sh.o_full[j & 1], uint32_t(j >> 1) & 1, sh);
+            if (!ok) break;
+            if (live) {
+                tc_fence_after();
+                const float f = sh.corr[j & 3][r], vf = P::quant ? sh.v_factor[j & 3] : 1.0f;
+#pragma unroll
+                for (int b = 0; b < W / 16; ++b) {
+                    uint32_t o[16];
+                    tmem_ld16(o, from + (j & 1) * HDP + 16 * b);
+                    tmem_wait_ld();
+#pragma unroll
+                    for (int e = 0; e < 16; ++e) {
+                        const float v = __uint_as_float(o[e]);
+                        acc[16 * b + e] = fmaf(acc[16 * b + e], f, P::quant ? v * vf : v);
+                    }
+                }
+            }
+            tc_fence_before();
+            mbar_arrive(&sh.o_empty[j & 1]);
+        }
+        asm volatile("bar.sync 2, 384;" ::: "memory");  // the softmax warps' m and l
+        const float l = sh.l[r];
+        if (live && r < rows && !*reinterpret_cast<volatile int*>(&sh.abort)) {
+            if (active == 1) {
+                const int row = row0 + r, tok = row / a.group, h = kvh * a.group + row - tok * a.group;
+                float* out = a.out + ((size_t(seq) * a.n_tree + tok) * a.n_head + h) * hd + half * W;
+                const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+#pragma unroll
+                for (int d = 0; d < W; d += 4)
+                    if (half * W + d < hd)
+                        *reinterpret_cast<float4*>(out + d) =
+                            make_float4(acc[d] * inv, acc[d + 1] * inv, acc[d + 2] * inv, acc[d + 3] * inv);
+            } else {  // m[128], l[128], o[hd][128]
+                float* part = a.parts + ((size_t(seq) * gridDim.y + blockIdx.y) * a.splits + blockIdx.x) * kTcRows * (hd + 2);
+                if (half == 0) {
+                    part[r] = sh.m[r];
+                    part[kTcRows + r] = l;
+                }
+#pragma unroll
+                for (int d = 0; d < W; ++d)
+                    if (half * W + d < hd) part[(2 + half * W + d) * kTcRows + r] = acc[d];
+            }
+        }
+    } else if (warp < 16) {
+        // ---- tiles ------------------------------------------------------------------------
+        const int ft = tid - 384;
+        const char *kb = a.c.k + size_t(seq) * a.c.seq_stride, *vb = a.c.v + size_t(seq) * a.c.seq_stride;
+        auto full = [&](int j) {
+            fence_async_shared();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&sh.kv_full[j % P::stages]);
+        };
+        if constexpr (!P::quant) {
+            constexpr int CP = HDP / 8, D = P::stages - 1;  // chunks of a row; tiles in flight
+            const size_t pitch = size_t(a.c.n_kv) * hd * 2, head = size_t(kvh) * hd * 2;
+            const int chunks = hd / 8;
+            int j = 0;
+            for (; j < n; ++j) {
+                const int st = j % P::stages, t = t0 + j, p0 = t * kTcTile;
+                if (j == 1 && !warp_wait(&sh.q_full, 0, sh)) break;
+                if (j >= P::stages && !warp_wait(&sh.kv_empty[st], uint32_t(j / P::stages - 1) & 1, sh)) break;
+                const uint32_t to = tiles_s + st * P::stage;
+#pragma unroll 8
+                for (int i = 0; i < kTcTile * CP / 128; ++i) {
+                    const int p = (i * 128 + ft) / CP, ch = (i * 128 + ft) % CP;
+                    const bool in = p0 + p < total && ch < chunks;  // dims past the head are zero
+                    const size_t at = in ? size_t(p0 + p) * pitch + head + ch * 16 : 0;
+                    const int off = tile_at(p, ch);
+                    cp16(to + off, kb + at, in);
+                    if (p0 + p < len) {
+                        cp16(to + P::v_hi + off, vb + at, in);
+                    } else {
+                        // a row of the tree: what is not finite becomes 0 (a probability of 0 times it would be
+                        // NaN) and its position scores NaN for the tokens that see it
+                        uint4 x = in ? *reinterpret_cast<const uint4*>(vb + at) : make_uint4(0, 0, 0, 0);
+                        uint32_t w[4] = {x.x, x.y, x.z, x.w};
+                        bool bad = false;
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) {
+                            if ((w[e] & 0x7c00u) == 0x7c00u) { w[e] &= 0xffff0000u; bad = true; }
+                            if ((w[e] & 0x7c000000u) == 0x7c000000u) { w[e] &= 0xffffu; bad = true; }
+                        }
+                        *reinterpret_cast<uint4*>(tiles + st * P::stage + P::v_hi + off) = make_uint4(w[0], w[1], w[2], w[3]);
+                        if (bad) atomicOr(&sh.bad[t - edge0], 1ull << p);
+                    }
+                }
+                cp_commit();
+                if (j >= D - 1) {
+                    cp_wait<D - 1>();
+                    full(j - (D - 1));
+                }
+            }
+            cp_wait<0>();
+            if (j == n)
+                for (int k = max(0, n - (D - 1)); k < n; ++k) full(k);
+        } else {
+            constexpr int VPC = TYPE == SYN_Q8_0 ? 16 : 32;          // values of 16 bytes of quants
+            constexpr int CP = HDP / VPC, N = kTcTile * CP / 128;   // chunks of a row; chunks of a thread
+            const int nb = hd / 32, chunks = hd / VPC;
+            const size_t head = size_t(kvh) * a.c.max_ctx;
+            const uint16_t *ks = reinterpret_cast<const uint16_t*>(kb + a.c.scale_plane), *vs = reinterpret_cast<const uint16_t*>(vb + a.c.scale_plane);
+            uint4 kq[N], vq[N];
+            uint32_t kd[N], vd[N];  // scale bits
+            auto fetch = [&](int t) {
+#pragma unroll
+                for (int i = 0; i < N; ++i) {
+                    const int p = (i * 128 + ft) / CP, ch = (i * 128 + ft) % CP, pos = t * kTcTile + p;
+                    kd[i] = vd[i] = 0;
+                    if (ch < chunks && pos < total) {
+                        const size_t rowi = head + pos, sc = rowi * nb + ch * VPC / 32, at = (rowi * chunks + ch) * 16;
+                        kq[i] = __ldg(reinterpret_cast<const uint4*>(kb + at));
+                        vq[i] = __ldg(reinterpret_cast<const uint4*>(vb + at));
+                        kd[i] = __ldg(ks + sc);
+                        vd[i] = __ldg(vs + sc);
+                    } else {
+                        kq[i] = vq[i] = make_uint4(0, 0, 0, 0);
+                    }
+                }
+            };
+            fetch(t0);
+            for (int j = 0; j < n; ++j) {
+                const int st = j % P::stages, t = t0 + j;
+                // a scale that is not finite: its position is bad in a tree tile (NaN for who sees it), NaN in others
+                uint32_t tk = 0, tv = 0;
+#pragma unroll
+                for (int i = 0; i < N; ++i) {
+                    const int p = (i * 128 + ft) / CP;
+                    const bool fk = (kd[i] & 0x7c00u) != 0x7c00u, fv = (vd[i] & 0x7c00u) != 0x7c00u;
+                    if (t * kTcTile + p >= len && !(fk && fv)) {
+                        kd[i] = vd[i] = 0;
+                        atomicOr(&sh.bad[t - edge0], 1ull << p);
+                    }
+                    if (fk) tk = max(tk, kd[i] & 0x7fffu);
+                    if (fv) tv = max(tv, vd[i] & 0x7fffu);
+                }
+                tk = __reduce_max_sync(0xffffffffu, tk);
+                tv = __reduce_max_sync(0xffffffffu, tv);
+                bool ok = j != 1 || warp_wait(&sh.q_full, 0, sh);
+                if (j >= P::stages) ok = ok && warp_wait(&sh.kv_empty[st], uint32_t(j / P::stages - 1) & 1, sh);
+                if (lane == 0) {
+                    sh.top[j & 1][0][warp - 12] = ok ? tk : ~0u;  // a wait that gave up ends all four warps
+                    sh.top[j & 1][1][warp - 12] = tv;
+                }
+                asm volatile("bar.sync 1, 128;" ::: "memory");
+                tk = max(max(sh.top[j & 1][0][0], sh.top[j & 1][0][1]), max(sh.top[j & 1][0][2], sh.top[j & 1][0][3]));
+                tv = max(max(sh.top[j & 1][1][0], sh.top[j & 1][1][1]), max(sh.top[j & 1][1][2], sh.top[j & 1][1][3]));
+                if (tk == ~0u) break;
+                // the largest scale to [2^8, 2^9): 127 of it is finite, and the low term reaches 2^-33 of it
+                const int ek = 23 - int(max(tk >> 10, 1u)), ev = 23 - int(max(tv >> 10, 1u));
+                const float upk = __uint_as_float(uint32_t(127 + ek) << 23), upv = __uint_as_float(uint32_t(127 + ev) << 23);
+                if (ft == 0) {
+                    sh.k_scale[j & 7] = __uint_as_float(uint32_t(127 - ek) << 23);
+                    sh.v_scale[j & 7] = __uint_as_float(uint32_t(127 - ev) << 23);
+                }
+                unsigned char* to = tiles + st * P::stage;
+                const __half2 zero = half2_of(TYPE == SYN_Q8_0 ? 0x64806480u : 0x64086408u);
+                auto put = [&](const uint4& q, __half2 d, int p, int ch, int hi_at, int lo_at) {
+                    const uint32_t w[4] = {q.x, q.y, q.z, q.w};
+#pragma unroll
+                    for (int part = 0; part < VPC / 8; ++part) {  // 8 dims: one chunk of each term
+                        uint32_t hi[4], lo[4];
+#pragma unroll
+                        for (int e = 0; e < 2; ++e) {
+                            uint32_t x;
+                            if (TYPE == SYN_Q8_0) x = w[2 * part + e] ^ 0x80808080u;
+                            else x = (w[2 * (part & 1) + e] >> (4 * (part >> 1))) & 0x0f0f0f0fu;
+#pragma unroll
+                            for (int o = 0; o < 2; ++o) {
+                                const __half2 v = __hsub2(bytes_h2(x, o ? 0x4342u : 0x4140u), zero);
+                                const __half2 y = __hmul2(v, d);
+                                hi[2 * e + o] = bits(y);
+                                lo[2 * e + o] = bits(__hfma2(v, d, __hneg2(y)));
+                            }
+                        }
+                        const int off = tile_at(p, ch * (VPC / 8) + part);
+                        *reinterpret_cast<uint4*>(to + hi_at + off) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
+                        *reinterpret_cast<uint4*>(to + lo_at + off) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
+                    }
+                };
+#pragma unroll
+                for (int i = 0; i < N; ++i) {
+                    const int p = (i * 128 + ft) / CP, ch = (i * 128 + ft) % CP;  // past the head: scales of 0
+                    put(kq[i], __float2half2_rn(f16_from_bits(uint16_t(kd[i])) * upk), p, ch, 0, P::k_lo);
+                    put(vq[i], __float2half2_rn(f16_from_bits(uint16_t(vd[i])) * upv), p, ch, P::v_hi, P::v_hi + P::tile);
+                }
+                if (j + 1 < n) fetch(t + 1);
+                full(j);
+            }
+        }
+    } else if (lane == 0) {
+        // ---- products ---------------------------------------------------------------------------
+        constexpr uint32_t ds = mma_desc(128, kTcTile, false), dv = mma_desc(128, HDP, true);
+        auto scores = [&](int j) {
+            const int st = j % P::stages;
+            if (!tc_wait(&sh.kv_full[st], uint32_t(j / P::stages) & 1, sh)) return false;
+            tc_fence_after();
+            const uint32_t k = tiles_s + st * P::stage, d = tm + P::s + (j & 1) * kTcTile;
+#pragma unroll
+            for (int term = 0; term < (P::quant ? 3 : 2); ++term) {  // hi hi, lo hi, hi lo
+                const uint32_t qa = tm + (term == 1 ? P::q_lo : P::q_hi), kt = k + (term == 2 ? P::k_lo : 0);
+#pragma unroll
+                for (int i = 0; i < HDP / 16; ++i)
+                    mma_ts(d, qa + 8 * i, smem_desc(kt + (i >> 2) * P::atom + (i & 3) * 32, 16, 1024), ds, term > 0 || i > 0);
+            }
+            mma_commit(&sh.s_full[j & 1]);
+            return true;
+        };
+        bool ok = tc_wait(&sh.q_full, 0, sh);
+        tc_fence_after();
+        ok = ok && scores(0);
+        for (int j = 0; ok && j < n; ++j) {
+            if (j + 1 < n && !scores(j + 1)) break;
+            if (!tc_wait(&sh.p_full[j & 3], uint32_t(j >> 2) & 1, sh)) break;
+            if (j >= 2 && !tc_wait(&sh.o_empty[j & 1], uint32_t((j >> 1) - 1) & 1, sh)) break;
+            tc_fence_after();
+            const int st = j % P::stages;
+            const uint32_t v = tiles_s + st * P::stage + P::v_hi, d = tm + P::o + (j & 1) * HDP, pa = tm + P::s + (j & 1) * kTcTile;
+#pragma unroll
+            for (int term = 0; term < (P::quant ? 3 : 2); ++term) {
+                const uint32_t pt = pa + (term == 1 ? 32 : 0), vt = v + (term == 2 ? P::tile : 0);
+#pragma unroll
+                for (int i = 0; i < kTcTile / 16; ++i)
+                    mma_ts(d, pt + 8 * i, smem_desc(vt + i * 2048, P::atom, 1024), dv, term > 0 || i > 0);
+            }
+            mma_commit(&sh.o_full[j & 1]);
+            mma_commit(&sh.kv_empty[st]);
+        }
+        // nothing of this CTA may be in flight when its tensor memory is freed
+        mma_commit(&sh.done);
+        mbar_wait_bounded(&sh.done, 0, kTcWaitNs);
+    }
+    __syncwarp();
+    if (warp < 4) asm volatile("bar.sync 2, 384;" ::: "memory");
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    if (warp == 16) tmem_free_all(tm);
+    if (active == 1 || sh.abort) return;
+
+    // ---- the last of the unit's CTAs joins the splits, in their order ------------------
+    __threadfence();
+    __syncthreads();
+    const size_t unit = size_t(seq) * gridDim.y + blockIdx.y;
+    if (tid == 0) sh.arrived = atomicAdd(a.counters + unit, 1u);
+    __syncthreads();
+    if (sh.arrived != unsigned(active - 1)) return;
+    __threadfence();
+    if (tid == 0) a.counters[unit] = 0;  // ready for the next call
+    const int part_floats = kTcRows * (hd + 2);
+    const float* parts = a.parts + unit * a.splits * part_floats;
+    float* weight = reinterpret_cast<float*>(tiles);  // [active][128], scaled by 1 / the row's sum
+    if (tid < rows) {
+        float top = -INFINITY, sum = 0.0f;
+        for (int x = 0; x < active; ++x) top = fmaxf(top, __ldcg(parts + size_t(x) * part_floats + tid));
+        for (int x = 0; x < active; ++x) {
+            const float l = __ldcg(parts + size_t(x) * part_floats + kTcRows + tid);
+            const float w = part_weight(__ldcg(parts + size_t(x) * part_floats + tid), l, top);
+            weight[x * kTcRows + tid] = w;
+            sum += w * l;
+        }
+        const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
+        for (int x = 0; x < active; ++x) weight[x * kTcRows + tid] *= inv;
+    }
+    __syncthreads();
+    for (int i = tid; i < rows * (hd / 4); i += kTcThreads) {
+        const int r = i % rows, d = i / rows * 4;
+        float acc[4] = {};
+#pragma unroll 4
+        for (int x = 0; x < active; ++x) {
+            const float* p = parts + size_t(x) * part_floats + (2 + d) * kTcRows + r;
+            const float w = weight[x * kTcRows + r];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) acc[e] = fmaf(w, __ldcg(p + e * kTcRows), acc[e]);
+        }
+        const int row = row0 + r, tok = row / a.group, h = kvh * a.group + row - tok * a.group;
+        *reinterpret_cast<float4*>(a.out + ((size_t(seq) * a.n_tree + tok) * a.n_head + h) * hd + d) =
+            make_float4(acc[0], acc[1], acc[2], acc[3]);
+    }
+}
+
+template <int TYPE, int HDP>
+int launch(const TreeParams& a, cudaStream_t s) {
+    auto kernel = tree_attn_tc_kernel<TYPE, HDP>;
+    constexpr int smem = TcPlan<TYPE, HDP>::smem;
+    static_assert(smem + sizeof(TcShared) <= 227 * 1024, "shared memory of a CTA");
+    const int st = syn_opt_in_smem(reinterpret_cast<const void*>(kernel), smem);
+    if (st) return st;
+    const dim3 grid{unsigned(a.splits), unsigned(a.c.n_kv * a.row_blocks), unsigned(a.c.n_seq)};
+    return syn_launch(kernel, grid, kTcThreads, smem, s, a);
+}
+
+}  // namespace
+
+int syn_tree_attention_tc(const TreeParams& a, int type, cudaStream_t s) {
+    if (a.c.hd <= 64)
+        return type == SYN_F16 ? launch<SYN_F16, 64>(a, s) : type == SYN_Q8_0 ? launch<SYN_Q8_0, 64>(a, s) : launch<SYN_Q4_0, 64>(a, s);
+    return type == SYN_F16 ? launch<SYN_F16, 128>(a, s) : type == SYN_Q8_0 ? launch<SYN_Q8_0, 128>(a, s) : launch<SYN_Q4_0, 128>(a, s);
+}
+
+// Bounded waits of the kernel that gave up on the current device (-1: unreadable).
+int syn_tree_timeouts() {
+    unsigned n = 0;
+    if (cudaMemcpyFromSymbol(&n, g_tree_timeouts, sizeof n) != cudaSuccess) return -1;
+    return int(n);
+}
