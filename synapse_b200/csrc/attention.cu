@@ -1314,29 +1314,13 @@ int opt_in(const void* kernel, size_t most) {
     return st;
 }
 
-// cuTensorMapEncodeTiled from the driver (looked up once; no libcuda link).
-PFN_cuTensorMapEncodeTiled_v12000 tensor_map_encoder() {
-    static PFN_cuTensorMapEncodeTiled_v12000 fn = nullptr;
-    static std::once_flag once;
-    std::call_once(once, [] {
-        void* p = nullptr;
-        cudaDriverEntryPointQueryResult q{};
-        if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &p, cudaEnableDefault, &q) == cudaSuccess &&
-            q == cudaDriverEntryPointSuccess)
-            fn = reinterpret_cast<PFN_cuTensorMapEncodeTiled_v12000>(p);
-        else
-            cudaGetLastError();
-    });
-    return fn;
-}
-
 // A K or V cache as a tensor of binary16: x = column (n_kv * head_dim), y =
 // position (max_len rows), z = query (cache_stride apart; absent when the
 // queries share one cache); boxes of box_x columns x box_y positions, read
 // into shared memory as they are (V) or in the 128-byte swizzle (K).
 int cache_tensor_map(const AttnParams& a, const uint16_t* base, unsigned box_x, unsigned box_y, bool swizzle,
                      CUtensorMap* m) {
-    const auto encode = tensor_map_encoder();
+    const auto encode = syn_tensor_map_encoder();
     if (!encode) {
         syn_set_error("cuTensorMapEncodeTiled is not available from the driver");
         return SYN_ERR_CUDA;

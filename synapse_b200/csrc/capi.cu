@@ -2,8 +2,12 @@
 // message is kept per thread for syn_last_error().
 #include "common.cuh"
 
+#include <cuda.h>
+#include <cudaTypedefs.h>
+
 #include <cstdio>
 #include <cstring>
+#include <mutex>
 
 namespace {
 thread_local char g_last_error[256] = "";
@@ -30,6 +34,22 @@ int syn_num_sms() {
     if (cudaGetDevice(&dev) != cudaSuccess) return 148;
     if (cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess || n <= 0) return 148;
     return n;
+}
+
+// cuTensorMapEncodeTiled from the driver (looked up once; no libcuda link).
+PFN_cuTensorMapEncodeTiled_v12000 syn_tensor_map_encoder() {
+    static PFN_cuTensorMapEncodeTiled_v12000 fn = nullptr;
+    static std::once_flag once;
+    std::call_once(once, [] {
+        void* p = nullptr;
+        cudaDriverEntryPointQueryResult q{};
+        if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &p, cudaEnableDefault, &q) == cudaSuccess &&
+            q == cudaDriverEntryPointSuccess)
+            fn = reinterpret_cast<PFN_cuTensorMapEncodeTiled_v12000>(p);
+        else
+            cudaGetLastError();
+    });
+    return fn;
 }
 
 extern "C" const char* syn_build_info(void) { return "synapse_b200 0.1 sm_100a"; }

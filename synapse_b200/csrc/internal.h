@@ -1,6 +1,8 @@
 // Entry points shared inside the library (not part of the public C ABI).
 #pragma once
 
+#include <cuda.h>
+#include <cudaTypedefs.h>
 #include <cuda_runtime.h>
 #include <stddef.h>
 #include <stdint.h>
@@ -55,6 +57,9 @@ void syn_set_pdl(int on);
 // The same, exported for microbenchmarks that time kernels captured the way
 // the session captures them.
 extern "C" void syn_set_programmatic_launch(int on);
+
+// cuTensorMapEncodeTiled from the driver; NULL when it is not there.
+PFN_cuTensorMapEncodeTiled_v12000 syn_tensor_map_encoder();
 
 // Sets the thread's last error message.
 void syn_set_error(const char* msg);

@@ -65,6 +65,12 @@ __device__ __forceinline__ uint64_t smem_desc(uint32_t addr, uint32_t lead, uint
 __host__ __device__ constexpr uint32_t mma_desc(int m, int n, bool b_mn_major) {
     return 1u << 4 | (b_mn_major ? 1u << 16 : 0u) | uint32_t(n >> 3) << 17 | uint32_t(m >> 4) << 24;
 }
+// One lane of a converged warp, always the same.
+__device__ __forceinline__ bool elect_one() {
+    uint32_t p;
+    asm volatile("{\n .reg .pred p;\n elect.sync _|p, 0xffffffff;\n selp.u32 %0, 1, 0, p;\n}\n" : "=r"(p));
+    return p != 0;
+}
 // D (TMEM) = A (TMEM) B (shared memory) [+ D], K = 16.
 __device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, bool accumulate) {
     asm volatile(

@@ -12,8 +12,8 @@
 // core's accumulators lose a little with every product.
 //
 // Warps: 0-3 softmax (a thread owns a row: no exchange between lanes), 4-7
-// and 8-11 the two halves of O, 12-15 fill the tiles (F16: asynchronous
-// copies; quantised: integers to binary16), 16 issues the products. Tensor
+// and 8-11 the two halves of O, 12-14 fill the tiles (F16: tensor copies;
+// quantised: integers to binary16), 15 issues the products. Tensor
 // memory: Q high | Q low | two S (then P) | two O.
 //
 // Bound: the products take 16 (F16) or 24 cycles per position and KV head
@@ -26,7 +26,8 @@ using namespace syn;
 
 namespace {
 
-constexpr int kTcThreads = 17 * 32;
+constexpr int kTcThreads = 16 * 32;
+constexpr int kFill = 96;  // threads that fill tiles
 constexpr uint64_t kTcWaitNs = 2000000000ull;  // a wait gives up after 2 s
 constexpr int kEdgeTiles = kMaxTree / kTcTile + 2;  // tiles that hold rows of the tree
 
@@ -46,6 +47,17 @@ struct TcPlan {
     static_assert(o + 2 * HDP <= 512, "tensor memory");
 };
 
+// The F16 caches as tensors (column, position, sequence), boxes of 64 columns x 64 positions under the 128-byte
+// swizzle; used where head_dim is a multiple of 64.
+struct TcMaps {
+    CUtensorMap k, v;
+};
+__device__ __forceinline__ void tma_load_tile(uint32_t dst, const CUtensorMap* map, int x, int y, int z, uint64_t* bar) {
+    asm volatile(
+        "cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], "
+        "[%5];" ::"r"(dst), "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(z), "r"(smem_addr(bar)) : "memory");
+}
+
 struct TcShared {
     uint64_t q_full, kv_full[5], kv_empty[5], s_full[2], p_full[4], o_full[2], o_empty[2], done;
     unsigned long long bad[kEdgeTiles];  // positions of a tree tile that hold values that are not finite
@@ -53,7 +65,7 @@ struct TcShared {
     float v_factor[4];                   // and of its O
     float k_scale[8], v_scale[8];        // powers of two of a tile's terms
     float m[kTcRows], l[kTcRows];
-    unsigned top[2][2][4];               // the fill warps' largest scales
+    unsigned top[2][2][3];               // the fill warps' largest scales
     uint32_t tmem;
     unsigned arrived;
     int abort;
@@ -101,7 +113,7 @@ __device__ __forceinline__ unsigned long long tile_sees(const TreeParams& a, int
 }
 
 template <int TYPE, int HDP>
-__global__ void __launch_bounds__(kTcThreads, 1) tree_attn_tc_kernel(const TreeParams a) {
+__global__ void __launch_bounds__(kTcThreads, 1) tree_attn_tc_kernel(const TreeParams a, const __grid_constant__ TcMaps maps) {
     using P = TcPlan<TYPE, HDP>;
     extern __shared__ unsigned char raw[];
     __shared__ TcShared sh;
@@ -126,7 +138,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) tree_attn_tc_kernel(const TreeP
     if (tid == 0) {
         mbar_init(&sh.q_full, 128);
         for (int i = 0; i < P::stages; ++i) {
-            mbar_init(&sh.kv_full[i], 4);
+            mbar_init(&sh.kv_full[i], kFill / 32);
             mbar_init(&sh.kv_empty[i], 1);
         }
         for (int i = 0; i < 2; ++i) {
@@ -140,7 +152,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) tree_attn_tc_kernel(const TreeP
         sh.abort = 0;
     }
     if (tid < kEdgeTiles) sh.bad[tid] = 0;
-    if (warp == 16) tmem_alloc_all(&sh.tmem);
+    if (warp == 15) tmem_alloc_all(&sh.tmem);
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
@@ -212,6 +224,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) tree_attn_tc_kernel(const TreeP
             tmem_wait_st();
         }
         tc_fence_before();
+        fence_async_shared();
         mbar_arrive(&sh.q_full);
         float m = -INFINITY, l = 0.0f;
         for (int j = 0; j < n; ++j) {
@@ -332,7 +345,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) tree_attn_tc_kernel(const TreeP
                     if (half * W + d < hd) part[(2 + half * W + d) * kTcRows + r] = acc[d];
             }
         }
-    } else if (warp < 16) {
+    } else if (warp < 15) {
         // ---- tiles ------------------------------------------------------------------------
         const int ft = tid - 384;
         const char *kb = a.c.k + size_t(seq) * a.c.seq_stride, *vb = a.c.v + size_t(seq) * a.c.seq_stride;
@@ -342,7 +355,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) tree_attn_tc_kernel(const TreeP
             if (lane == 0) mbar_arrive(&sh.kv_full[j % P::stages]);
         };
         if constexpr (!P::quant) {
-            constexpr int CP = HDP / 8, D = P::stages - 1;  // chunks of a row; tiles in flight
+            constexpr int CP = HDP / 8;  // chunks of a row
             const size_t pitch = size_t(a.c.n_kv) * hd * 2, head = size_t(kvh) * hd * 2;
             const int chunks = hd / 8;
             int j = 0;
@@ -350,20 +363,35 @@ __global__ void __launch_bounds__(kTcThreads, 1) tree_attn_tc_kernel(const TreeP
                 const int st = j % P::stages, t = t0 + j, p0 = t * kTcTile;
                 if (j == 1 && !warp_wait(&sh.q_full, 0, sh)) break;
                 if (j >= P::stages && !warp_wait(&sh.kv_empty[st], uint32_t(j / P::stages - 1) & 1, sh)) break;
-                const uint32_t to = tiles_s + st * P::stage;
-#pragma unroll 8
-                for (int i = 0; i < kTcTile * CP / 128; ++i) {
-                    const int p = (i * 128 + ft) / CP, ch = (i * 128 + ft) % CP;
+                if (t < edge0 && hd % 64 == 0) {
+                    if (lane == 0) {
+                        if (warp == 12) {
+                            const uint32_t to = tiles_s + st * P::stage;
+                            fence_async_shared();  // q was staged here
+                            mbar_expect_tx(&sh.kv_full[st], 2 * uint32_t(hd) * kTcTile * 2);
+                            for (int i = 0; i < hd / 64; ++i) {
+                                tma_load_tile(to + i * P::atom, &maps.k, kvh * hd + 64 * i, p0, seq, &sh.kv_full[st]);
+                                tma_load_tile(to + P::v_hi + i * P::atom, &maps.v, kvh * hd + 64 * i, p0, seq, &sh.kv_full[st]);
+                            }
+                        } else {
+                            mbar_arrive(&sh.kv_full[st]);
+                        }
+                    }
+                    continue;
+                }
+                unsigned char* to = tiles + st * P::stage;
+#pragma unroll 4
+                for (int i = ft; i < kTcTile * CP; i += kFill) {
+                    const int p = i / CP, ch = i % CP;
                     const bool in = p0 + p < total && ch < chunks;  // dims past the head are zero
                     const size_t at = in ? size_t(p0 + p) * pitch + head + ch * 16 : 0;
                     const int off = tile_at(p, ch);
-                    cp16(to + off, kb + at, in);
-                    if (p0 + p < len) {
-                        cp16(to + P::v_hi + off, vb + at, in);
-                    } else {
+                    const uint4 z = make_uint4(0, 0, 0, 0);
+                    *reinterpret_cast<uint4*>(to + off) = in ? *reinterpret_cast<const uint4*>(kb + at) : z;
+                    uint4 x = in ? *reinterpret_cast<const uint4*>(vb + at) : z;
+                    if (p0 + p >= len) {
                         // a row of the tree: what is not finite becomes 0 (a probability of 0 times it would be
                         // NaN) and its position scores NaN for the tokens that see it
-                        uint4 x = in ? *reinterpret_cast<const uint4*>(vb + at) : make_uint4(0, 0, 0, 0);
                         uint32_t w[4] = {x.x, x.y, x.z, x.w};
                         bool bad = false;
 #pragma unroll
@@ -371,22 +399,19 @@ __global__ void __launch_bounds__(kTcThreads, 1) tree_attn_tc_kernel(const TreeP
                             if ((w[e] & 0x7c00u) == 0x7c00u) { w[e] &= 0xffff0000u; bad = true; }
                             if ((w[e] & 0x7c000000u) == 0x7c000000u) { w[e] &= 0xffffu; bad = true; }
                         }
-                        *reinterpret_cast<uint4*>(tiles + st * P::stage + P::v_hi + off) = make_uint4(w[0], w[1], w[2], w[3]);
+                        x = make_uint4(w[0], w[1], w[2], w[3]);
                         if (bad) atomicOr(&sh.bad[t - edge0], 1ull << p);
                     }
+                    *reinterpret_cast<uint4*>(to + P::v_hi + off) = x;
                 }
-                cp_commit();
-                if (j >= D - 1) {
-                    cp_wait<D - 1>();
-                    full(j - (D - 1));
-                }
+                full(j);
             }
-            cp_wait<0>();
-            if (j == n)
-                for (int k = max(0, n - (D - 1)); k < n; ++k) full(k);
+            if (j < n)  // it gave up: its copies in flight land before it leaves
+                for (int k = max(0, j - P::stages); k < j; ++k)
+                    mbar_wait_bounded(&sh.kv_full[k % P::stages], uint32_t(k / P::stages) & 1, kTcWaitNs);
         } else {
             constexpr int VPC = TYPE == SYN_Q8_0 ? 16 : 32;          // values of 16 bytes of quants
-            constexpr int CP = HDP / VPC, N = kTcTile * CP / 128;   // chunks of a row; chunks of a thread
+            constexpr int CP = HDP / VPC, NC = kTcTile * CP, N = (NC + kFill - 1) / kFill;  // chunks of a row, of a tile, of a thread
             const int nb = hd / 32, chunks = hd / VPC;
             const size_t head = size_t(kvh) * a.c.max_ctx;
             const uint16_t *ks = reinterpret_cast<const uint16_t*>(kb + a.c.scale_plane), *vs = reinterpret_cast<const uint16_t*>(vb + a.c.scale_plane);
@@ -395,9 +420,9 @@ __global__ void __launch_bounds__(kTcThreads, 1) tree_attn_tc_kernel(const TreeP
             auto fetch = [&](int t) {
 #pragma unroll
                 for (int i = 0; i < N; ++i) {
-                    const int p = (i * 128 + ft) / CP, ch = (i * 128 + ft) % CP, pos = t * kTcTile + p;
+                    const int p = (i * kFill + ft) / CP, ch = (i * kFill + ft) % CP, pos = t * kTcTile + p;
                     kd[i] = vd[i] = 0;
-                    if (ch < chunks && pos < total) {
+                    if (ch < chunks && pos < total && i * kFill + ft < NC) {
                         const size_t rowi = head + pos, sc = rowi * nb + ch * VPC / 32, at = (rowi * chunks + ch) * 16;
                         kq[i] = __ldg(reinterpret_cast<const uint4*>(kb + at));
                         vq[i] = __ldg(reinterpret_cast<const uint4*>(vb + at));
@@ -415,9 +440,9 @@ __global__ void __launch_bounds__(kTcThreads, 1) tree_attn_tc_kernel(const TreeP
                 uint32_t tk = 0, tv = 0;
 #pragma unroll
                 for (int i = 0; i < N; ++i) {
-                    const int p = (i * 128 + ft) / CP;
+                    const int p = (i * kFill + ft) / CP;
                     const bool fk = (kd[i] & 0x7c00u) != 0x7c00u, fv = (vd[i] & 0x7c00u) != 0x7c00u;
-                    if (t * kTcTile + p >= len && !(fk && fv)) {
+                    if (t * kTcTile + p >= len && p < kTcTile && !(fk && fv)) {
                         kd[i] = vd[i] = 0;
                         atomicOr(&sh.bad[t - edge0], 1ull << p);
                     }
@@ -432,9 +457,9 @@ __global__ void __launch_bounds__(kTcThreads, 1) tree_attn_tc_kernel(const TreeP
                     sh.top[j & 1][0][warp - 12] = ok ? tk : ~0u;  // a wait that gave up ends all four warps
                     sh.top[j & 1][1][warp - 12] = tv;
                 }
-                asm volatile("bar.sync 1, 128;" ::: "memory");
-                tk = max(max(sh.top[j & 1][0][0], sh.top[j & 1][0][1]), max(sh.top[j & 1][0][2], sh.top[j & 1][0][3]));
-                tv = max(max(sh.top[j & 1][1][0], sh.top[j & 1][1][1]), max(sh.top[j & 1][1][2], sh.top[j & 1][1][3]));
+                asm volatile("bar.sync 1, 96;" ::: "memory");
+                tk = max(max(sh.top[j & 1][0][0], sh.top[j & 1][0][1]), sh.top[j & 1][0][2]);
+                tv = max(max(sh.top[j & 1][1][0], sh.top[j & 1][1][1]), sh.top[j & 1][1][2]);
                 if (tk == ~0u) break;
                 // the largest scale to [2^8, 2^9): 127 of it is finite, and the low term reaches 2^-33 of it
                 const int ek = 23 - int(max(tk >> 10, 1u)), ev = 23 - int(max(tv >> 10, 1u));
@@ -470,7 +495,8 @@ __global__ void __launch_bounds__(kTcThreads, 1) tree_attn_tc_kernel(const TreeP
                 };
 #pragma unroll
                 for (int i = 0; i < N; ++i) {
-                    const int p = (i * 128 + ft) / CP, ch = (i * 128 + ft) % CP;  // past the head: scales of 0
+                    const int p = (i * kFill + ft) / CP, ch = (i * kFill + ft) % CP;  // past the head: scales of 0
+                    if (NC % kFill && i * kFill + ft >= NC) break;
                     put(kq[i], __float2half2_rn(f16_from_bits(uint16_t(kd[i])) * upk), p, ch, 0, P::k_lo);
                     put(vq[i], __float2half2_rn(f16_from_bits(uint16_t(vd[i])) * upv), p, ch, P::v_hi, P::v_hi + P::tile);
                 }
@@ -478,46 +504,56 @@ __global__ void __launch_bounds__(kTcThreads, 1) tree_attn_tc_kernel(const TreeP
                 full(j);
             }
         }
-    } else if (lane == 0) {
-        // ---- products ---------------------------------------------------------------------------
+    } else {
+        // ---- products (the whole warp runs the loop, one lane issues) ---------------------------
         constexpr uint32_t ds = mma_desc(128, kTcTile, false), dv = mma_desc(128, HDP, true);
         auto scores = [&](int j) {
             const int st = j % P::stages;
-            if (!tc_wait(&sh.kv_full[st], uint32_t(j / P::stages) & 1, sh)) return false;
+            if (!warp_wait(&sh.kv_full[st], uint32_t(j / P::stages) & 1, sh)) return false;
             tc_fence_after();
-            const uint32_t k = tiles_s + st * P::stage, d = tm + P::s + (j & 1) * kTcTile;
+            const uint32_t d = tm + P::s + (j & 1) * kTcTile;
+            const uint64_t k = smem_desc(tiles_s + st * P::stage, 16, 1024);
+            if (elect_one()) {
 #pragma unroll
-            for (int term = 0; term < (P::quant ? 3 : 2); ++term) {  // hi hi, lo hi, hi lo
-                const uint32_t qa = tm + (term == 1 ? P::q_lo : P::q_hi), kt = k + (term == 2 ? P::k_lo : 0);
+                for (int term = 0; term < (P::quant ? 3 : 2); ++term) {  // hi hi, lo hi, hi lo
+                    const uint32_t qa = tm + (term == 1 ? P::q_lo : P::q_hi);
 #pragma unroll
-                for (int i = 0; i < HDP / 16; ++i)
-                    mma_ts(d, qa + 8 * i, smem_desc(kt + (i >> 2) * P::atom + (i & 3) * 32, 16, 1024), ds, term > 0 || i > 0);
+                    for (int i = 0; i < HDP / 16; ++i)
+                        mma_ts(d, qa + 8 * i, k + (((term == 2 ? P::k_lo : 0) + (i >> 2) * P::atom + (i & 3) * 32) >> 4), ds,
+                               term > 0 || i > 0);
+                }
+                mma_commit(&sh.s_full[j & 1]);
             }
-            mma_commit(&sh.s_full[j & 1]);
+            __syncwarp();
             return true;
         };
-        bool ok = tc_wait(&sh.q_full, 0, sh);
+        bool ok = warp_wait(&sh.q_full, 0, sh);
         tc_fence_after();
         ok = ok && scores(0);
         for (int j = 0; ok && j < n; ++j) {
             if (j + 1 < n && !scores(j + 1)) break;
-            if (!tc_wait(&sh.p_full[j & 3], uint32_t(j >> 2) & 1, sh)) break;
-            if (j >= 2 && !tc_wait(&sh.o_empty[j & 1], uint32_t((j >> 1) - 1) & 1, sh)) break;
+            if (!warp_wait(&sh.p_full[j & 3], uint32_t(j >> 2) & 1, sh)) break;
+            if (j >= 2 && !warp_wait(&sh.o_empty[j & 1], uint32_t((j >> 1) - 1) & 1, sh)) break;
             tc_fence_after();
             const int st = j % P::stages;
-            const uint32_t v = tiles_s + st * P::stage + P::v_hi, d = tm + P::o + (j & 1) * HDP, pa = tm + P::s + (j & 1) * kTcTile;
+            const uint32_t d = tm + P::o + (j & 1) * HDP, pa = tm + P::s + (j & 1) * kTcTile;
+            const uint64_t v = smem_desc(tiles_s + st * P::stage + P::v_hi, P::atom, 1024);
+            if (elect_one()) {
 #pragma unroll
-            for (int term = 0; term < (P::quant ? 3 : 2); ++term) {
-                const uint32_t pt = pa + (term == 1 ? 32 : 0), vt = v + (term == 2 ? P::tile : 0);
+                for (int term = 0; term < (P::quant ? 3 : 2); ++term) {
 #pragma unroll
-                for (int i = 0; i < kTcTile / 16; ++i)
-                    mma_ts(d, pt + 8 * i, smem_desc(vt + i * 2048, P::atom, 1024), dv, term > 0 || i > 0);
+                    for (int i = 0; i < kTcTile / 16; ++i)
+                        mma_ts(d, pa + (term == 1 ? 32 : 0) + 8 * i, v + (((term == 2 ? P::tile : 0) + i * 2048) >> 4), dv,
+                               term > 0 || i > 0);
+                }
+                mma_commit(&sh.o_full[j & 1]);
+                mma_commit(&sh.kv_empty[st]);
             }
-            mma_commit(&sh.o_full[j & 1]);
-            mma_commit(&sh.kv_empty[st]);
+            __syncwarp();
         }
         // nothing of this CTA may be in flight when its tensor memory is freed
-        mma_commit(&sh.done);
+        if (elect_one()) mma_commit(&sh.done);
+        __syncwarp();
         mbar_wait_bounded(&sh.done, 0, kTcWaitNs);
     }
     __syncwarp();
@@ -525,7 +561,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) tree_attn_tc_kernel(const TreeP
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
-    if (warp == 16) tmem_free_all(tm);
+    if (warp == 15) tmem_free_all(tm);
     if (active == 1 || sh.abort) return;
 
     // ---- the last of the unit's CTAs joins the splits, in their order ------------------
@@ -569,15 +605,40 @@ __global__ void __launch_bounds__(kTcThreads, 1) tree_attn_tc_kernel(const TreeP
     }
 }
 
+int cache_map(const TreeParams& a, const char* base, CUtensorMap* m) {
+    const auto encode = syn_tensor_map_encoder();
+    if (!encode) {
+        syn_set_error("cuTensorMapEncodeTiled is not available from the driver");
+        return SYN_ERR_CUDA;
+    }
+    const cuuint64_t row = cuuint64_t(a.c.n_kv) * a.c.hd;
+    const cuuint64_t dims[3] = {row, cuuint64_t(a.c.max_ctx), cuuint64_t(a.c.n_seq)};
+    const cuuint64_t strides[2] = {row * 2, a.c.n_seq > 1 ? cuuint64_t(a.c.seq_stride) : row * 2 * a.c.max_ctx};
+    const cuuint32_t box[3] = {64, kTcTile, 1}, estr[3] = {1, 1, 1};
+    const CUresult r = encode(m, CU_TENSOR_MAP_DATA_TYPE_UINT16, 3, const_cast<char*>(base), dims, strides, box, estr,
+                              CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                              CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    if (r != CUDA_SUCCESS) {
+        syn_set_error("cuTensorMapEncodeTiled rejected the KV cache geometry");
+        return SYN_ERR_INVALID;
+    }
+    return SYN_OK;
+}
+
 template <int TYPE, int HDP>
 int launch(const TreeParams& a, cudaStream_t s) {
     auto kernel = tree_attn_tc_kernel<TYPE, HDP>;
     constexpr int smem = TcPlan<TYPE, HDP>::smem;
     static_assert(smem + sizeof(TcShared) <= 227 * 1024, "shared memory of a CTA");
-    const int st = syn_opt_in_smem(reinterpret_cast<const void*>(kernel), smem);
+    int st = syn_opt_in_smem(reinterpret_cast<const void*>(kernel), smem);
     if (st) return st;
+    TcMaps maps{};
+    if (TYPE == SYN_F16 && a.c.hd % 64 == 0) {
+        if ((st = cache_map(a, a.c.k, &maps.k))) return st;
+        if ((st = cache_map(a, a.c.v, &maps.v))) return st;
+    }
     const dim3 grid{unsigned(a.splits), unsigned(a.c.n_kv * a.row_blocks), unsigned(a.c.n_seq)};
-    return syn_launch(kernel, grid, kTcThreads, smem, s, a);
+    return syn_launch(kernel, grid, kTcThreads, smem, s, a, maps);
 }
 
 }  // namespace
