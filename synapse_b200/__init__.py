@@ -527,10 +527,10 @@ def kv_move(cache, path, count, begin, stream=None):
 
 
 def tree_attention_scratch(cache, tree, n_head, max_len=None):
-    """A zeroed scratch for tree_attention calls of this shape; it may be kept for every later call on one stream."""
+    """A scratch for tree_attention calls of this shape; it may be kept for every later call on one stream."""
     n = lib().syn_tree_attention_scratch_bytes(cache.n_seq, tree, n_head, cache.n_kv, cache.head_dim,
                                                max_len or cache.max_ctx)
-    return _torch().zeros(max(n, 1), dtype=_torch().uint8, device=cache.device)
+    return empty_bytes(n, cache.device)
 
 
 def tree_attention(cache, q, len, n_head, scale, tree=1, mask=None, max_len=None, out=None, scratch=None, layer=0,
@@ -545,7 +545,7 @@ def tree_attention(cache, q, len, n_head, scale, tree=1, mask=None, max_len=None
         out = torch.empty((rows, cols), dtype=torch.float32, device=q.device)
     need = lib().syn_tree_attention_scratch_bytes(cache.n_seq, tree, n_head, cache.n_kv, cache.head_dim, max_len)
     if scratch is None:
-        scratch = torch.zeros(max(need, 1), dtype=torch.uint8, device=q.device)
+        scratch = empty_bytes(need, q.device)
     elif scratch.numel() * scratch.element_size() < need:
         raise ValueError(f"tree_attention: scratch of {need} bytes needed")
     a = TreeAttentionArgs(qp, _need(out, torch.float32, rows * cols, "out"), _need(len, torch.int32, cache.n_seq, "len"),

@@ -416,22 +416,28 @@ int syn_num_sms();
 int syn_pdl_enabled();
 void syn_set_pdl(int on);
 
-// Launch with the PDL attribute when enabled. Every kernel of this library
-// calls griddepcontrol.wait before it reads a predecessor's output or writes
-// any output, so a kernel may only start early, never read early.
+// Launch, with the PDL attribute if `early`.
 template <typename... KArgs, typename... Args>
-int syn_launch(void (*kernel)(KArgs...), dim3 grid, dim3 block, size_t smem, cudaStream_t s, Args&&... args) {
+int syn_launch_pdl(bool early, void (*kernel)(KArgs...), dim3 grid, dim3 block, size_t smem, cudaStream_t s, Args&&... args) {
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = grid;
     cfg.blockDim = block;
     cfg.dynamicSmemBytes = smem;
     cfg.stream = s;
     cudaLaunchAttribute attr[1];
-    if (syn_pdl_enabled()) {
+    if (early) {
         attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
         attr[0].val.programmaticStreamSerializationAllowed = 1;
         cfg.attrs = attr;
         cfg.numAttrs = 1;
     }
     return syn_cuda_status(cudaLaunchKernelEx(&cfg, kernel, static_cast<KArgs>(args)...));
+}
+
+// Launch with the PDL attribute when enabled. Every kernel of this library
+// calls griddepcontrol.wait before it reads a predecessor's output or writes
+// any output, so a kernel may only start early, never read early.
+template <typename... KArgs, typename... Args>
+int syn_launch(void (*kernel)(KArgs...), dim3 grid, dim3 block, size_t smem, cudaStream_t s, Args&&... args) {
+    return syn_launch_pdl(syn_pdl_enabled(), kernel, grid, block, smem, s, static_cast<Args&&>(args)...);
 }

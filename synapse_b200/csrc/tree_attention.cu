@@ -12,8 +12,8 @@
 // between the warps), and keep a running maximum, sum and output of their own
 // (one pass over K and V); the warps' results are joined at the end. With few
 // rows the context is split over CTAs so that all SMs read: each CTA leaves
-// (max, sum, output) in the scratch and the last one to arrive joins them in
-// split order.
+// (max, sum, output) in the scratch, and tree_join_kernel, which starts early
+// and waits for the first kernel to end, joins them in split order.
 //
 // Precision: the products run on binary16 tensor-core instructions with float
 // accumulators. q is scaled by a power of two per row and split into two
@@ -34,7 +34,6 @@ namespace {
 
 constexpr int kWarps = 4;
 constexpr int kStep = 16;            // positions per step of a warp
-constexpr size_t kCounterBytes = 16384;  // arrival counters at the start of the scratch
 __device__ __forceinline__ void ldsm4(uint32_t (&r)[4], uint32_t addr) {
     asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
                  : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
@@ -101,7 +100,6 @@ __global__ void __launch_bounds__(kWarps * 32, 2) tree_attn_kernel(const TreePar
     const int total = len + a.n_tree;
     const int steps = (total + kStep - 1) / kStep;
     const int per = (steps + a.splits - 1) / a.splits;
-    const int active = (steps + per - 1) / per;  // splits that have steps
     const int s0 = blockIdx.x * per, s1 = min(s0 + per, steps);
     if (s0 >= steps) return;
 
@@ -523,9 +521,7 @@ __global__ void __launch_bounds__(kWarps * 32, 2) tree_attn_kernel(const TreePar
             }
         }
     __syncthreads();
-    const int part_floats = R * (hd + 2);
-    const size_t unit = size_t(seq) * gridDim.y + blockIdx.y;
-    float* part = a.parts + (unit * a.splits + blockIdx.x) * part_floats;
+    const size_t part = ((size_t(seq) * gridDim.y + blockIdx.y) * a.splits + blockIdx.x) * R;
     for (int r = warp; r < rows; r += kWarps) {
         float mx = -INFINITY;
 #pragma unroll
@@ -537,53 +533,72 @@ __global__ void __launch_bounds__(kWarps * 32, 2) tree_attn_kernel(const TreePar
             sum += f[w] * jl[w * R + r];
         }
         const int row = row0 + r, tk = row / a.group, h = kvh * a.group + row - tk * a.group;
-        float* out = a.out + (size_t(seq) * a.n_tree + tk) * a.n_head * hd + size_t(h) * hd;
-        const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
+        const bool whole = a.splits == 1;
+        float* out = whole ? a.out + ((size_t(seq) * a.n_tree + tk) * a.n_head + h) * hd : a.part_o + (part + r) * hd;
+        const float inv = !whole ? 1.0f : sum == 0.0f ? 0.0f : 1.0f / sum;
         for (int d = lane; d < hd; d += 32) {
             float acc = 0.0f;
 #pragma unroll
             for (int w = 0; w < kWarps; ++w) acc += f[w] * jo[(w * R + r) * P::o_pitch + d];
-            if (active == 1) out[d] = acc * inv;
-            else part[2 * R + r * hd + d] = acc;
+            out[d] = acc * inv;
         }
-        if (active > 1 && lane == 0) {
-            part[r] = mx;
-            part[R + r] = sum;
-        }
+        if (!whole && lane == 0) a.part_ml[part + r] = make_float2(mx, sum);
     }
-    if (active == 1) return;
+}
 
-    // --- the last of the unit's CTAs joins the splits, in their order ------------------
-    __threadfence();
-    __syncthreads();
-    __shared__ unsigned arrived;
-    if (tid == 0) arrived = atomicAdd(a.counters + unit, 1u);
-    __syncthreads();
-    if (arrived != unsigned(active - 1)) return;
-    __threadfence();
-    if (tid == 0) a.counters[unit] = 0;  // ready for the next call
-    const float* parts = a.parts + unit * a.splits * part_floats;
-    for (int r = warp; r < rows; r += kWarps) {
-        float mx = -INFINITY;
-        for (int x = lane; x < active; x += 32) mx = fmaxf(mx, __ldcg(parts + size_t(x) * part_floats + r));
-        mx = warp_max(mx);
-        float acc[NB] = {}, sum = 0.0f;
-        for (int x = 0; x < active; ++x) {
-            const float* px = parts + size_t(x) * part_floats;
-            const float mw = __ldcg(px + r), lw = __ldcg(px + R + r);
-            const float f = part_weight(mw, lw, mx);
-            sum += f * lw;
+// Joins a call's splits, in their order: a warp per row (token, head).
+__global__ void __launch_bounds__(128) tree_join_kernel(const TreeParams a, int R, int step) {
+    pdl_wait();
+    const int lane = threadIdx.x & 31, hd = a.c.hd;
+    const size_t id = size_t(blockIdx.x) * 4 + (threadIdx.x >> 5);  // row of all rows
+    if (id >= size_t(a.c.n_seq) * a.c.n_kv * a.rows) return;
+    const int row = int(id % a.rows), kvh = int(id / a.rows % a.c.n_kv), seq = int(id / a.rows / a.c.n_kv);
+    const int rb = row / R, r = row - rb * R;
+    // the splits that had steps
+    const int len = min(max(a.len[seq], 0), a.max_len - a.n_tree);
+    const int steps = (len + a.n_tree + step - 1) / step, per = (steps + a.splits - 1) / a.splits;
+    const int active = (steps + per - 1) / per;
+    const size_t first = (size_t(seq) * a.c.n_kv + kvh) * a.row_blocks + rb;
+    const float2* ml = a.part_ml + first * a.splits * R + r;
+    const float* o = a.part_o + (first * a.splits * R + r) * hd;
+    float top = -INFINITY;
+    for (int x = lane; x < active; x += 32) top = fmaxf(top, __ldcg(ml + size_t(x) * R).x);
+    top = warp_max(top);
+    const bool in = 4 * lane < hd, in2 = 128 + 4 * lane < hd;
+    float4 acc = make_float4(0, 0, 0, 0), acc2 = acc;
+    float sum = 0.0f;
+    auto add = [](float4& c, float f, const float4& v) {
+        c.x = fmaf(f, v.x, c.x); c.y = fmaf(f, v.y, c.y); c.z = fmaf(f, v.z, c.z); c.w = fmaf(f, v.w, c.w);
+    };
+    for (int x0 = 0; x0 < active; x0 += 32) {
+        const float2 s = x0 + lane < active ? __ldcg(ml + size_t(x0 + lane) * R) : make_float2(-INFINITY, 0.0f);
+        const float w = part_weight(s.x, s.y, top);
+        sum += warp_sum(w * s.y);
+        const int n = min(32, active - x0);
+        for (int i0 = 0; i0 < n; i0 += 8) {
+            float4 v[8], v2[8];
 #pragma unroll
-            for (int b = 0; b < NB; ++b)
-                if (32 * b + lane < hd) acc[b] += f * __ldcg(px + 2 * R + r * hd + 32 * b + lane);
+            for (int i = 0; i < 8; ++i) {
+                const float4* p = reinterpret_cast<const float4*>(o + size_t(x0 + i0 + i) * R * hd);
+                v[i] = v2[i] = make_float4(0, 0, 0, 0);
+                if (i0 + i < n && in) v[i] = __ldcg(p + lane);
+                if (i0 + i < n && in2) v2[i] = __ldcg(p + 32 + lane);
+            }
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                const float f = __shfl_sync(0xffffffffu, w, (i0 + i) & 31);
+                if (i0 + i < n) {
+                    add(acc, f, v[i]);
+                    if (hd > 128) add(acc2, f, v2[i]);
+                }
+            }
         }
-        const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
-        const int row = row0 + r, tk = row / a.group, h = kvh * a.group + row - tk * a.group;
-        float* out = a.out + (size_t(seq) * a.n_tree + tk) * a.n_head * hd + size_t(h) * hd;
-#pragma unroll
-        for (int b = 0; b < NB; ++b)
-            if (32 * b + lane < hd) out[32 * b + lane] = acc[b] * inv;
     }
+    const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
+    const int tk = row / a.group, h = kvh * a.group + row - tk * a.group;
+    float4* out = reinterpret_cast<float4*>(a.out + ((size_t(seq) * a.n_tree + tk) * a.n_head + h) * hd);
+    if (in) out[lane] = make_float4(acc.x * inv, acc.y * inv, acc.z * inv, acc.w * inv);
+    if (in2) out[32 + lane] = make_float4(acc2.x * inv, acc2.y * inv, acc2.z * inv, acc2.w * inv);
 }
 
 // How a call is cut: rows of a CTA, CTAs over the rows, splits of the context.
@@ -618,7 +633,6 @@ Cut cut_of(int n_seq, int n_tree, int n_head, int n_kv, int head_dim, int max_le
         const int most = (max_len + 2 * kWarps * kStep - 1) / (2 * kWarps * kStep);
         c.splits = int(std::max<size_t>(1, std::min<size_t>(2 * sms / c.units, size_t(most))));
     }
-    if (c.units * sizeof(unsigned) > kCounterBytes) c.splits = 1;
     return c;
 }
 
@@ -663,7 +677,7 @@ extern "C" size_t syn_tree_attention_scratch_bytes(int n_seq, int n_tree, int n_
         head_dim > 256 || max_len < n_tree)
         return 0;
     const Cut c = cut_of(n_seq, n_tree, n_head, n_kv, head_dim, max_len);
-    return kCounterBytes + (c.splits > 1 ? align256(c.units * c.splits * c.R * (size_t(head_dim) + 2) * 4) : 0);
+    return c.splits > 1 ? align256(c.units * c.splits * c.R * 8) + align256(c.units * c.splits * c.R * size_t(head_dim) * 4) : 256;
 }
 
 extern "C" int syn_tree_attention(const syn_kv_cache* c, int layer, const syn_tree_attention_args* x, void* stream) {
@@ -681,8 +695,8 @@ extern "C" int syn_tree_attention(const syn_kv_cache* c, int layer, const syn_tr
     TreeParams a{};
     a.c = kv_view(c, layer);
     a.q = x->q; a.out = x->out; a.len = x->len; a.mask = x->mask;
-    a.counters = static_cast<unsigned*>(x->scratch);
-    a.parts = reinterpret_cast<float*>(static_cast<char*>(x->scratch) + kCounterBytes);
+    a.part_ml = static_cast<float2*>(x->scratch);
+    a.part_o = reinterpret_cast<float*>(static_cast<char*>(x->scratch) + align256(cut.units * cut.splits * cut.R * 8));
     a.q_stride = x->q_stride ? x->q_stride : q_row;
     a.n_tree = x->n_tree; a.n_head = x->n_head;
     a.group = x->n_head / c->n_kv;
@@ -693,8 +707,11 @@ extern "C" int syn_tree_attention(const syn_kv_cache* c, int layer, const syn_tr
     a.splits = cut.splits;
     a.scale_log2 = x->scale * 1.4426950408889634f;
     cudaStream_t s = static_cast<cudaStream_t>(stream);
-    if (cut.tc) return syn_tree_attention_tc(a, c->type, s);
-    if (c->type == SYN_F16) return launch_type<SYN_F16>(a, s);
-    if (c->type == SYN_Q8_0) return launch_type<SYN_Q8_0>(a, s);
-    return launch_type<SYN_Q4_0>(a, s);
+    if (cut.tc) st = syn_tree_attention_tc(a, c->type, s);
+    else if (c->type == SYN_F16) st = launch_type<SYN_F16>(a, s);
+    else if (c->type == SYN_Q8_0) st = launch_type<SYN_Q8_0>(a, s);
+    else st = launch_type<SYN_Q4_0>(a, s);
+    if (st || cut.splits == 1) return st;
+    const size_t rows = size_t(c->n_seq) * c->n_kv * a.rows;
+    return syn_launch_pdl(true, tree_join_kernel, unsigned((rows + 3) / 4), 128, 0, s, a, cut.R, cut.tc ? kTcTile : kStep);
 }

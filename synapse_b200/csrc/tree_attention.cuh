@@ -14,8 +14,8 @@ struct TreeParams {
     float* out;
     const int32_t* len;
     const uint32_t* mask;
-    unsigned* counters;  // [n_seq][n_kv * row blocks]
-    float* parts;        // [n_seq][n_kv * row blocks][splits]: m[R], l[R], o[R * hd]
+    float2* part_ml;     // [n_seq][n_kv * row blocks][splits][R]: a part's maximum and sum of a row
+    float* part_o;       // [n_seq][n_kv * row blocks][splits][R][hd]: its output, not divided
     size_t q_stride;
     int n_tree, n_head, group, rows, row_blocks, max_len, mask_words, splits;
     float scale_log2;    // scale * log2(e)

@@ -12,8 +12,8 @@
 // core's accumulators lose a little with every product.
 //
 // Warps: 0-3 softmax (a thread owns a row: no exchange between lanes), 4-7
-// and 8-11 the two halves of O, 12-14 fill the tiles (F16: tensor copies;
-// quantised: integers to binary16), 15 issues the products. Tensor
+// and 8-11 the two halves of O, 12-17 fill the tiles (F16: tensor copies;
+// quantised: integers to binary16), 18 issues the products. Tensor
 // memory: Q high | Q low | two S (then P) | two O.
 //
 // Bound: the products take 16 (F16) or 24 cycles per position and KV head
@@ -26,8 +26,8 @@ using namespace syn;
 
 namespace {
 
-constexpr int kTcThreads = 16 * 32;
-constexpr int kFill = 96;  // threads that fill tiles
+constexpr int kFillWarps = 6, kMmaWarp = 12 + kFillWarps, kTcThreads = (kMmaWarp + 1) * 32;
+constexpr int kFill = 32 * kFillWarps;  // threads that fill tiles
 constexpr uint64_t kTcWaitNs = 2000000000ull;  // a wait gives up after 2 s
 constexpr int kEdgeTiles = kMaxTree / kTcTile + 2;  // tiles that hold rows of the tree
 
@@ -65,9 +65,9 @@ struct TcShared {
     float v_factor[4];                   // and of its O
     float k_scale[8], v_scale[8];        // powers of two of a tile's terms
     float m[kTcRows], l[kTcRows];
-    unsigned top[2][2][3];               // the fill warps' largest scales
+    float q_scale[kTcRows];              // the rows' factor of a product's scores
+    unsigned top[2][kFillWarps];                  // the fill warps' largest scales, of K and of V
     uint32_t tmem;
-    unsigned arrived;
     int abort;
 };
 
@@ -130,7 +130,6 @@ __global__ void __launch_bounds__(kTcThreads, 1) tree_attn_tc_kernel(const TreeP
     const int total = len + a.n_tree;
     const int n_tiles = (total + kTcTile - 1) / kTcTile;
     const int per = (n_tiles + a.splits - 1) / a.splits;
-    const int active = (n_tiles + per - 1) / per;
     const int t0 = blockIdx.x * per, n = min(per, n_tiles - t0);  // tiles t0 .. t0 + n - 1
     if (n <= 0) return;
     const int edge0 = len / kTcTile;  // the first tile with a row of the tree
@@ -138,7 +137,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) tree_attn_tc_kernel(const TreeP
     if (tid == 0) {
         mbar_init(&sh.q_full, 128);
         for (int i = 0; i < P::stages; ++i) {
-            mbar_init(&sh.kv_full[i], kFill / 32);
+            mbar_init(&sh.kv_full[i], kFillWarps);
             mbar_init(&sh.kv_empty[i], 1);
         }
         for (int i = 0; i < 2; ++i) {
@@ -152,7 +151,51 @@ __global__ void __launch_bounds__(kTcThreads, 1) tree_attn_tc_kernel(const TreeP
         sh.abort = 0;
     }
     if (tid < kEdgeTiles) sh.bad[tid] = 0;
-    if (warp == 15) tmem_alloc_all(&sh.tmem);
+    if (warp == kMmaWarp) tmem_alloc_all(&sh.tmem);
+    // q: a warp takes 8 rows (lane = dims), split into the tile memory that the fill warps leave free until q_full
+    constexpr int kQPitch = HDP * 2 + 16;
+    unsigned char* q_stage = tiles + P::stage;  // [row][high | low]
+    if (warp < kTcRows / 8) {
+        constexpr int V = HDP / 32;
+        const bool vec = V == 4 && ((reinterpret_cast<uintptr_t>(a.q) & 15) | (a.q_stride & 3)) == 0;
+        float x[8][V];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            const int r = 8 * warp + i, row = row0 + r, tok = row / a.group, h = row - tok * a.group;
+            const float* q = a.q + (size_t(seq) * a.n_tree + tok) * a.q_stride + size_t(kvh * a.group + h) * hd + lane * V;
+#pragma unroll
+            for (int e = 0; e < V; ++e) x[i][e] = 0.0f;
+            if (r < rows && lane * V < hd) {
+                if constexpr (V == 4) {
+                    if (vec) {
+                        const float4 f = __ldg(reinterpret_cast<const float4*>(q));
+                        x[i][0] = f.x; x[i][1] = f.y; x[i][2] = f.z; x[i][3] = f.w;
+                    }
+                }
+                if (!vec)
+#pragma unroll
+                    for (int e = 0; e < V; ++e) x[i][e] = __ldg(q + e);
+            }
+        }
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            const int r = 8 * warp + i;
+            uint32_t top = 0;
+#pragma unroll
+            for (int e = 0; e < V; ++e) top = max(top, __float_as_uint(fabsf(x[i][e])));
+            float up, down;
+            q_factor(__uint_as_float(__reduce_max_sync(0xffffffffu, top)), up, down);
+            if (lane == 0) sh.q_scale[r] = a.scale_log2 * down;
+            unsigned char* at = q_stage + r * 2 * kQPitch + lane * V * 2;
+#pragma unroll
+            for (int e = 0; e < V; e += 2) {
+                uint32_t hi, lo;
+                split2(x[i][e] * up, x[i][e + 1] * up, hi, lo);
+                *reinterpret_cast<uint32_t*>(at + 2 * e) = hi;
+                *reinterpret_cast<uint32_t*>(at + kQPitch + 2 * e) = lo;
+            }
+        }
+    }
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
@@ -164,59 +207,15 @@ __global__ void __launch_bounds__(kTcThreads, 1) tree_attn_tc_kernel(const TreeP
         const int r = tid, row = row0 + r;
         const int tok = row / a.group;
         const uint32_t lanes = tm + (uint32_t(32 * warp) << 16);
-        float c = 0.0f;
+        const float c = sh.q_scale[r];
         if (live) {
-            // the warp's 32 rows, a row at a time (lane = dims), split into the tile memory that the fill warps leave
-            // free until q_full; then each thread's row to tensor memory
-            constexpr int V = HDP / 32, pitch = HDP * 2 + 16;
-            unsigned char* mine = tiles + P::stage + warp * 64 * pitch;
-            const bool vec = V == 4 && ((reinterpret_cast<uintptr_t>(a.q) & 15) | (a.q_stride & 3)) == 0;
-            for (int i0 = 0; i0 < 32; i0 += 8) {
-                float x[8][V];
-#pragma unroll
-                for (int i = 0; i < 8; ++i) {
-                    const int rr = 32 * warp + i0 + i, qrow = row0 + rr, qt = qrow / a.group, qh = qrow - qt * a.group;
-                    const float* q = a.q + (size_t(seq) * a.n_tree + qt) * a.q_stride + size_t(kvh * a.group + qh) * hd + lane * V;
-#pragma unroll
-                    for (int e = 0; e < V; ++e) x[i][e] = 0.0f;
-                    if (rr < rows && lane * V < hd) {
-                        if constexpr (V == 4) {
-                            if (vec) {
-                                const float4 f = __ldg(reinterpret_cast<const float4*>(q));
-                                x[i][0] = f.x; x[i][1] = f.y; x[i][2] = f.z; x[i][3] = f.w;
-                            }
-                        }
-                        if (!vec)
-#pragma unroll
-                            for (int e = 0; e < V; ++e) x[i][e] = __ldg(q + e);
-                    }
-                }
-#pragma unroll
-                for (int i = 0; i < 8; ++i) {
-                    uint32_t top = 0;
-#pragma unroll
-                    for (int e = 0; e < V; ++e) top = max(top, __float_as_uint(fabsf(x[i][e])));
-                    float up, down;
-                    q_factor(__uint_as_float(__reduce_max_sync(0xffffffffu, top)), up, down);
-                    if (lane == i0 + i) c = a.scale_log2 * down;
-                    unsigned char* at = mine + (i0 + i) * 2 * pitch + lane * V * 2;
-#pragma unroll
-                    for (int e = 0; e < V; e += 2) {
-                        uint32_t hi, lo;
-                        split2(x[i][e] * up, x[i][e + 1] * up, hi, lo);
-                        *reinterpret_cast<uint32_t*>(at + 2 * e) = hi;
-                        *reinterpret_cast<uint32_t*>(at + pitch + 2 * e) = lo;
-                    }
-                }
-            }
-            __syncwarp();
 #pragma unroll
             for (int b = 0; b < HDP / 16; ++b) {  // 16 columns: 32 dims of the high, then of the low term
                 const int term = b / (HDP / 32), at = b % (HDP / 32);
                 uint32_t w[16];
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
-                    const uint4 x = *reinterpret_cast<const uint4*>(mine + (lane * 2 + term) * pitch + at * 64 + e * 16);
+                    const uint4 x = *reinterpret_cast<const uint4*>(q_stage + (r * 2 + term) * kQPitch + at * 64 + e * 16);
                     w[4 * e] = x.x; w[4 * e + 1] = x.y; w[4 * e + 2] = x.z; w[4 * e + 3] = x.w;
                 }
                 tmem_st16(lanes + (term ? P::q_lo : P::q_hi) + 16 * at, w);
@@ -271,16 +270,17 @@ __global__ void __launch_bounds__(kTcThreads, 1) tree_attn_tc_kernel(const TreeP
                 const float base = (m == -INFINITY ? 0.0f : m) - kPShift;
                 float sum[4] = {};
 #pragma unroll
-                for (int u = 0; u < 2; ++u) {
-                    uint32_t hi[16], lo[16];
+                for (int u = 0; u < 4; ++u) {
+                    uint32_t hi[8], lo[8];
 #pragma unroll
-                    for (int e = 0; e < 16; ++e) {
-                        const float p0 = ex2(__uint_as_float(s[u][2 * e]) - base), p1 = ex2(__uint_as_float(s[u][2 * e + 1]) - base);
+                    for (int e = 0; e < 8; ++e) {
+                        const int at = 16 * (u & 1) + 2 * e;
+                        const float p0 = ex2(__uint_as_float(s[u >> 1][at]) - base), p1 = ex2(__uint_as_float(s[u >> 1][at + 1]) - base);
                         sum[e & 3] += p0 + p1;
                         split2(p0, p1, hi[e], lo[e]);
                     }
-                    tmem_st16(lanes + P::s + (j & 1) * kTcTile + 16 * u, hi);
-                    tmem_st16(lanes + P::s + (j & 1) * kTcTile + 32 + 16 * u, lo);
+                    tmem_st8(lanes + P::s + (j & 1) * kTcTile + 8 * u, hi);
+                    tmem_st8(lanes + P::s + (j & 1) * kTcTile + 32 + 8 * u, lo);
                 }
                 l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
                 if (P::quant && tid == 0) sh.v_factor[j & 3] = sh.v_scale[j & 7];
@@ -325,27 +325,19 @@ __global__ void __launch_bounds__(kTcThreads, 1) tree_attn_tc_kernel(const TreeP
         asm volatile("bar.sync 2, 384;" ::: "memory");  // the softmax warps' m and l
         const float l = sh.l[r];
         if (live && r < rows && !*reinterpret_cast<volatile int*>(&sh.abort)) {
-            if (active == 1) {
-                const int row = row0 + r, tok = row / a.group, h = kvh * a.group + row - tok * a.group;
-                float* out = a.out + ((size_t(seq) * a.n_tree + tok) * a.n_head + h) * hd + half * W;
-                const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+            const bool whole = a.splits == 1;
+            const int row = row0 + r, tok = row / a.group, h = kvh * a.group + row - tok * a.group;
+            const size_t part = ((size_t(seq) * gridDim.y + blockIdx.y) * a.splits + blockIdx.x) * kTcRows + r;
+            float* out = whole ? a.out + ((size_t(seq) * a.n_tree + tok) * a.n_head + h) * hd : a.part_o + part * hd;
+            const float inv = !whole ? 1.0f : l == 0.0f ? 0.0f : 1.0f / l;
 #pragma unroll
-                for (int d = 0; d < W; d += 4)
-                    if (half * W + d < hd)
-                        *reinterpret_cast<float4*>(out + d) =
-                            make_float4(acc[d] * inv, acc[d + 1] * inv, acc[d + 2] * inv, acc[d + 3] * inv);
-            } else {  // m[128], l[128], o[hd][128]
-                float* part = a.parts + ((size_t(seq) * gridDim.y + blockIdx.y) * a.splits + blockIdx.x) * kTcRows * (hd + 2);
-                if (half == 0) {
-                    part[r] = sh.m[r];
-                    part[kTcRows + r] = l;
-                }
-#pragma unroll
-                for (int d = 0; d < W; ++d)
-                    if (half * W + d < hd) part[(2 + half * W + d) * kTcRows + r] = acc[d];
-            }
+            for (int d = 0; d < W; d += 4)
+                if (half * W + d < hd)
+                    *reinterpret_cast<float4*>(out + half * W + d) =
+                        make_float4(acc[d] * inv, acc[d + 1] * inv, acc[d + 2] * inv, acc[d + 3] * inv);
+            if (!whole && half == 0) a.part_ml[part] = make_float2(sh.m[r], l);
         }
-    } else if (warp < 15) {
+    } else if (warp < kMmaWarp) {
         // ---- tiles ------------------------------------------------------------------------
         const int ft = tid - 384;
         const char *kb = a.c.k + size_t(seq) * a.c.seq_stride, *vb = a.c.v + size_t(seq) * a.c.seq_stride;
@@ -415,92 +407,106 @@ __global__ void __launch_bounds__(kTcThreads, 1) tree_attn_tc_kernel(const TreeP
             const int nb = hd / 32, chunks = hd / VPC;
             const size_t head = size_t(kvh) * a.c.max_ctx;
             const uint16_t *ks = reinterpret_cast<const uint16_t*>(kb + a.c.scale_plane), *vs = reinterpret_cast<const uint16_t*>(vb + a.c.scale_plane);
-            uint4 kq[N], vq[N];
-            uint32_t kd[N], vd[N];  // scale bits
-            auto fetch = [&](int t) {
+            // a thread's chunks of K and of V: V's load while K is converted, the next K's while V is
+            struct Half {
+                uint4 q[N];
+                uint32_t d[N];  // scale bits
+            } kh, vh;
+            auto fetch = [&](Half& h, const char* base, const uint16_t* scales, int t) {
 #pragma unroll
                 for (int i = 0; i < N; ++i) {
                     const int p = (i * kFill + ft) / CP, ch = (i * kFill + ft) % CP, pos = t * kTcTile + p;
-                    kd[i] = vd[i] = 0;
+                    h.d[i] = 0;
+                    h.q[i] = make_uint4(0, 0, 0, 0);
                     if (ch < chunks && pos < total && i * kFill + ft < NC) {
-                        const size_t rowi = head + pos, sc = rowi * nb + ch * VPC / 32, at = (rowi * chunks + ch) * 16;
-                        kq[i] = __ldg(reinterpret_cast<const uint4*>(kb + at));
-                        vq[i] = __ldg(reinterpret_cast<const uint4*>(vb + at));
-                        kd[i] = __ldg(ks + sc);
-                        vd[i] = __ldg(vs + sc);
-                    } else {
-                        kq[i] = vq[i] = make_uint4(0, 0, 0, 0);
+                        const size_t rowi = head + pos;
+                        h.q[i] = __ldg(reinterpret_cast<const uint4*>(base + (rowi * chunks + ch) * 16));
+                        h.d[i] = __ldg(scales + rowi * nb + ch * VPC / 32);
                     }
                 }
             };
-            fetch(t0);
-            for (int j = 0; j < n; ++j) {
-                const int st = j % P::stages, t = t0 + j;
-                // a scale that is not finite: its position is bad in a tree tile (NaN for who sees it), NaN in others
-                uint32_t tk = 0, tv = 0;
+            // Converts a half of tile t into its two terms at `to`; the scale of the tile's integers goes to *scale.
+            // False when a wait has given up (in any of the warps).
+            auto convert = [&](Half& h, int which, bool ok, int j, unsigned char* to, float* scale) {
+                const int t = t0 + j;
+                uint32_t top = 0;
 #pragma unroll
                 for (int i = 0; i < N; ++i) {
+                    // a scale that is not finite: a tree row's position is bad (NaN for who sees it), others are NaN
                     const int p = (i * kFill + ft) / CP;
-                    const bool fk = (kd[i] & 0x7c00u) != 0x7c00u, fv = (vd[i] & 0x7c00u) != 0x7c00u;
-                    if (t * kTcTile + p >= len && p < kTcTile && !(fk && fv)) {
-                        kd[i] = vd[i] = 0;
+                    const bool finite = (h.d[i] & 0x7c00u) != 0x7c00u;
+                    if (!finite && t * kTcTile + p >= len) {
+                        h.d[i] = 0;
                         atomicOr(&sh.bad[t - edge0], 1ull << p);
                     }
-                    if (fk) tk = max(tk, kd[i] & 0x7fffu);
-                    if (fv) tv = max(tv, vd[i] & 0x7fffu);
+                    if (finite) top = max(top, h.d[i] & 0x7fffu);
                 }
-                tk = __reduce_max_sync(0xffffffffu, tk);
-                tv = __reduce_max_sync(0xffffffffu, tv);
-                bool ok = j != 1 || warp_wait(&sh.q_full, 0, sh);
-                if (j >= P::stages) ok = ok && warp_wait(&sh.kv_empty[st], uint32_t(j / P::stages - 1) & 1, sh);
-                if (lane == 0) {
-                    sh.top[j & 1][0][warp - 12] = ok ? tk : ~0u;  // a wait that gave up ends all four warps
-                    sh.top[j & 1][1][warp - 12] = tv;
-                }
-                asm volatile("bar.sync 1, 96;" ::: "memory");
-                tk = max(max(sh.top[j & 1][0][0], sh.top[j & 1][0][1]), sh.top[j & 1][0][2]);
-                tv = max(max(sh.top[j & 1][1][0], sh.top[j & 1][1][1]), sh.top[j & 1][1][2]);
-                if (tk == ~0u) break;
+                top = __reduce_max_sync(0xffffffffu, top);
+                if (lane == 0) sh.top[which][warp - 12] = ok ? top : ~0u;
+                asm volatile("bar.sync 1, %0;" ::"n"(kFill) : "memory");
+#pragma unroll
+                for (int w = 0; w < kFillWarps; ++w) top = max(top, sh.top[which][w]);
+                if (top == ~0u) return false;
                 // the largest scale to [2^8, 2^9): 127 of it is finite, and the low term reaches 2^-33 of it
-                const int ek = 23 - int(max(tk >> 10, 1u)), ev = 23 - int(max(tv >> 10, 1u));
-                const float upk = __uint_as_float(uint32_t(127 + ek) << 23), upv = __uint_as_float(uint32_t(127 + ev) << 23);
-                if (ft == 0) {
-                    sh.k_scale[j & 7] = __uint_as_float(uint32_t(127 - ek) << 23);
-                    sh.v_scale[j & 7] = __uint_as_float(uint32_t(127 - ev) << 23);
-                }
-                unsigned char* to = tiles + st * P::stage;
+                const int e = 23 - int(max(top >> 10, 1u));
+                const float up = __uint_as_float(uint32_t(127 + e) << 23);
+                if (ft == 0) *scale = __uint_as_float(uint32_t(127 - e) << 23);
                 const __half2 zero = half2_of(TYPE == SYN_Q8_0 ? 0x64806480u : 0x64086408u);
-                auto put = [&](const uint4& q, __half2 d, int p, int ch, int hi_at, int lo_at) {
-                    const uint32_t w[4] = {q.x, q.y, q.z, q.w};
-#pragma unroll
-                    for (int part = 0; part < VPC / 8; ++part) {  // 8 dims: one chunk of each term
-                        uint32_t hi[4], lo[4];
-#pragma unroll
-                        for (int e = 0; e < 2; ++e) {
-                            uint32_t x;
-                            if (TYPE == SYN_Q8_0) x = w[2 * part + e] ^ 0x80808080u;
-                            else x = (w[2 * (part & 1) + e] >> (4 * (part >> 1))) & 0x0f0f0f0fu;
-#pragma unroll
-                            for (int o = 0; o < 2; ++o) {
-                                const __half2 v = __hsub2(bytes_h2(x, o ? 0x4342u : 0x4140u), zero);
-                                const __half2 y = __hmul2(v, d);
-                                hi[2 * e + o] = bits(y);
-                                lo[2 * e + o] = bits(__hfma2(v, d, __hneg2(y)));
-                            }
-                        }
-                        const int off = tile_at(p, ch * (VPC / 8) + part);
-                        *reinterpret_cast<uint4*>(to + hi_at + off) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
-                        *reinterpret_cast<uint4*>(to + lo_at + off) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
-                    }
-                };
 #pragma unroll
                 for (int i = 0; i < N; ++i) {
                     const int p = (i * kFill + ft) / CP, ch = (i * kFill + ft) % CP;  // past the head: scales of 0
                     if (NC % kFill && i * kFill + ft >= NC) break;
-                    put(kq[i], __float2half2_rn(f16_from_bits(uint16_t(kd[i])) * upk), p, ch, 0, P::k_lo);
-                    put(vq[i], __float2half2_rn(f16_from_bits(uint16_t(vd[i])) * upv), p, ch, P::v_hi, P::v_hi + P::tile);
+                    const __half2 d = __float2half2_rn(f16_from_bits(uint16_t(h.d[i])) * up);
+                    // neighbouring threads store different 16-byte columns of the swizzled rows at a time: those of
+                    // the second 64 dims take the block's chunks in another order
+                    const int c0 = ch * (VPC / 8), turn = (c0 >> 3) * (VPC / 16);
+                    unsigned char* rowp = to + (c0 >> 3) * P::atom + p * 128;
+                    const int col = (((c0 ^ p) & 7) ^ turn) << 4;
+                    uint32_t w[4] = {h.q[i].x, h.q[i].y, h.q[i].z, h.q[i].w};
+                    if (TYPE == SYN_Q8_0) {
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) w[e] ^= 0x80808080u;
+                        if (turn) {
+                            const uint32_t x = w[0], y = w[1];
+                            w[0] = w[2]; w[1] = w[3]; w[2] = x; w[3] = y;
+                        }
+                    } else if (turn) {
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) w[e] = w[e] >> 4 | w[e] << 28;  // the high nibbles first
+                    }
+#pragma unroll
+                    for (int k = 0; k < VPC / 8; ++k) {  // 8 dims: one chunk of each term
+                        uint32_t hi[4], lo[4];
+#pragma unroll
+                        for (int e2 = 0; e2 < 2; ++e2) {
+                            uint32_t x = w[2 * (k & 1) + e2];
+                            if (TYPE == SYN_Q4_0) x = (k >> 1 ? (turn ? x << 4 | x >> 28 : x >> 4) : x) & 0x0f0f0f0fu;
+#pragma unroll
+                            for (int o = 0; o < 2; ++o) {
+                                const __half2 v = __hsub2(bytes_h2(x, o ? 0x4342u : 0x4140u), zero);
+                                const __half2 y = __hmul2(v, d);
+                                hi[2 * e2 + o] = bits(y);
+                                lo[2 * e2 + o] = bits(__hfma2(v, d, __hneg2(y)));
+                            }
+                        }
+                        unsigned char* at = rowp + (col ^ (k << 4));
+                        *reinterpret_cast<uint4*>(at) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
+                        *reinterpret_cast<uint4*>(at + P::tile) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
+                    }
                 }
-                if (j + 1 < n) fetch(t + 1);
+                return true;
+            };
+            fetch(kh, kb, ks, t0);
+            fetch(vh, vb, vs, t0);
+            for (int j = 0; j < n; ++j) {
+                const int st = j % P::stages, t = t0 + j;
+                bool ok = j != 1 || warp_wait(&sh.q_full, 0, sh);
+                if (j >= P::stages) ok = ok && warp_wait(&sh.kv_empty[st], uint32_t(j / P::stages - 1) & 1, sh);
+                unsigned char* to = tiles + st * P::stage;
+                if (!convert(kh, 0, ok, j, to, &sh.k_scale[j & 7])) break;
+                if (j + 1 < n) fetch(kh, kb, ks, t + 1);
+                convert(vh, 1, true, j, to + P::v_hi, &sh.v_scale[j & 7]);
+                if (j + 1 < n) fetch(vh, vb, vs, t + 1);
                 full(j);
             }
         }
@@ -561,48 +567,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) tree_attn_tc_kernel(const TreeP
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
-    if (warp == 15) tmem_free_all(tm);
-    if (active == 1 || sh.abort) return;
-
-    // ---- the last of the unit's CTAs joins the splits, in their order ------------------
-    __threadfence();
-    __syncthreads();
-    const size_t unit = size_t(seq) * gridDim.y + blockIdx.y;
-    if (tid == 0) sh.arrived = atomicAdd(a.counters + unit, 1u);
-    __syncthreads();
-    if (sh.arrived != unsigned(active - 1)) return;
-    __threadfence();
-    if (tid == 0) a.counters[unit] = 0;  // ready for the next call
-    const int part_floats = kTcRows * (hd + 2);
-    const float* parts = a.parts + unit * a.splits * part_floats;
-    float* weight = reinterpret_cast<float*>(tiles);  // [active][128], scaled by 1 / the row's sum
-    if (tid < rows) {
-        float top = -INFINITY, sum = 0.0f;
-        for (int x = 0; x < active; ++x) top = fmaxf(top, __ldcg(parts + size_t(x) * part_floats + tid));
-        for (int x = 0; x < active; ++x) {
-            const float l = __ldcg(parts + size_t(x) * part_floats + kTcRows + tid);
-            const float w = part_weight(__ldcg(parts + size_t(x) * part_floats + tid), l, top);
-            weight[x * kTcRows + tid] = w;
-            sum += w * l;
-        }
-        const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
-        for (int x = 0; x < active; ++x) weight[x * kTcRows + tid] *= inv;
-    }
-    __syncthreads();
-    for (int i = tid; i < rows * (hd / 4); i += kTcThreads) {
-        const int r = i % rows, d = i / rows * 4;
-        float acc[4] = {};
-#pragma unroll 4
-        for (int x = 0; x < active; ++x) {
-            const float* p = parts + size_t(x) * part_floats + (2 + d) * kTcRows + r;
-            const float w = weight[x * kTcRows + r];
-#pragma unroll
-            for (int e = 0; e < 4; ++e) acc[e] = fmaf(w, __ldcg(p + e * kTcRows), acc[e]);
-        }
-        const int row = row0 + r, tok = row / a.group, h = kvh * a.group + row - tok * a.group;
-        *reinterpret_cast<float4*>(a.out + ((size_t(seq) * a.n_tree + tok) * a.n_head + h) * hd + d) =
-            make_float4(acc[0], acc[1], acc[2], acc[3]);
-    }
+    if (warp == kMmaWarp) tmem_free_all(tm);
 }
 
 int cache_map(const TreeParams& a, const char* base, CUtensorMap* m) {
