@@ -286,7 +286,7 @@ typedef struct {
     const float* k;          /* [n_seq * n][n_kv * head_dim] */
     const float* v;
     const float* q;          /* NULL, or [n_seq * n][n_head * head_dim] */
-    float* q_out;            /* contiguous [n_seq * n][n_head * head_dim]; must not overlap q */
+    float* q_out;            /* contiguous [n_seq * n][n_head * head_dim], 16-byte aligned; must not overlap q */
     const int32_t* slot;     /* [n_seq * n] device */
     const int32_t* pos;      /* NULL, or [n_seq * n] device */
     const float* rope_table; /* NULL: no rotation; or syn_rope_table of table_len rows */

@@ -8,6 +8,7 @@ package on a machine without the built library raises, and calling a kernel
 without a GPU raises.
 """
 import ctypes
+import functools
 import os
 
 import numpy as np
@@ -459,21 +460,37 @@ class KVCache:
 
 
 def _need(t, dtype, n, where):
-    """A contiguous CUDA tensor of dtype with n elements; its address (None for None)."""
+    """The address of a contiguous CUDA tensor of dtype with n elements (None for None)."""
     if t is None:
         return None
-    if t.dtype != dtype or not t.is_cuda or not t.is_contiguous() or (n is not None and t.numel() != n):
+    if t.dtype != dtype or not t.is_cuda or t.numel() != n or not t.is_contiguous():
         raise ValueError(f"{where}: needs a contiguous {dtype} CUDA tensor of {n} elements")
     return t.data_ptr()
 
 
-def _rows(t, cols, n, where):
+def _rows(t, f32, cols, n, where):
     """Rows of cols floats whose rows may be strided: (address, floats between rows)."""
-    f32 = _torch().float32
-    if t.dtype != f32 or not t.is_cuda or t.dim() != 2 or t.shape[0] != n or t.shape[1] != cols or \
-            (cols > 1 and t.stride(1) != 1) or (n > 1 and t.stride(0) < cols):
+    if t.dtype != f32 or not t.is_cuda or t.shape != (n, cols):
         raise ValueError(f"{where}: needs {n} float rows of {cols} on the GPU")
-    return t.data_ptr(), t.stride(0) if n > 1 else cols
+    if t.is_contiguous():
+        return t.data_ptr(), cols
+    ld = t.stride(0) if n > 1 else cols
+    if (cols > 1 and t.stride(1) != 1) or ld < cols:
+        raise ValueError(f"{where}: rows must be contiguous and apart")
+    return t.data_ptr(), ld
+
+
+def _on(stream, device):
+    """The handle of a stream (None: the device's current one)."""
+    if stream is not None:
+        return stream.cuda_stream
+    return _torch()._C._cuda_getCurrentRawStream(device.index)
+
+
+@functools.lru_cache(maxsize=256)
+def _tree_scratch_bytes(n_seq, tree, n_head, n_kv, head_dim, max_len, device):
+    with _torch().cuda.device(device):  # the split depends on the device's SMs
+        return lib().syn_tree_attention_scratch_bytes(n_seq, tree, n_head, n_kv, head_dim, max_len)
 
 
 def kv_append(cache, k, v, slot, pos=None, rope_table=None, rope_mode=0, q=None, layer=0, stream=None):
@@ -481,24 +498,24 @@ def kv_append(cache, k, v, slot, pos=None, rope_table=None, rope_mode=0, q=None,
     rope_table ([len][head_dim / 2][2]) is given; q [n_seq * n][n_head * head_dim], if given, is rotated too and
     returned."""
     torch = _torch()
+    f32, i32 = torch.float32, torch.int32
     tokens, hd = slot.numel(), cache.head_dim
-    kp, ks = _rows(k, cache.n_kv * hd, tokens, "kv_append k")
-    vp, vs = _rows(v, cache.n_kv * hd, tokens, "kv_append v")
+    kp, ks = _rows(k, f32, cache.n_kv * hd, tokens, "kv_append k")
+    vp, vs = _rows(v, f32, cache.n_kv * hd, tokens, "kv_append v")
     if ks != vs or tokens % cache.n_seq:
         raise ValueError("kv_append: k and v must be strided alike, with the same tokens for every sequence")
-    qp = qs = out = None
-    n_head = 0
+    qp = op = out = None
+    n_head = qs = 0
     if q is not None:
         n_head = q.shape[1] // hd
-        qp, qs = _rows(q, n_head * hd, tokens, "kv_append q")
-        out = torch.empty((tokens, n_head * hd), dtype=torch.float32, device=q.device)
-    table_len = 0
-    if rope_table is not None:
-        table_len = rope_table.numel() // hd
-    a = KVAppendArgs(kp, vp, qp, out.data_ptr() if out is not None else None, _need(slot, torch.int32, tokens, "slot"),
-                     _need(pos, torch.int32, tokens, "pos"), _need(rope_table, torch.float32, table_len * hd, "rope_table"),
-                     ks, qs or 0, tokens // cache.n_seq, n_head, table_len, rope_mode)
-    check(lib().syn_kv_append(cache.ref, layer, ctypes.byref(a), _stream(stream)), "syn_kv_append")
+        qp, qs = _rows(q, f32, n_head * hd, tokens, "kv_append q")
+        out = q.new_empty((tokens, n_head * hd))
+        op = out.data_ptr()
+    table_len = rope_table.numel() // hd if rope_table is not None else 0
+    a = KVAppendArgs(kp, vp, qp, op, _need(slot, i32, tokens, "slot"), _need(pos, i32, tokens, "pos"),
+                     _need(rope_table, f32, table_len * hd, "rope_table"), ks, qs, tokens // cache.n_seq, n_head,
+                     table_len, rope_mode)
+    check(lib().syn_kv_append(cache.ref, layer, ctypes.byref(a), _on(stream, cache.device)), "syn_kv_append")
     return out
 
 
@@ -509,28 +526,26 @@ def kv_read(cache, n, rows=None, first=0, dtype=None, layer=0, stream=None):
     dtype = dtype or torch.float32
     if dtype not in (torch.float32, torch.float16):
         raise ValueError("kv_read: dtype is torch.float32 or torch.float16")
-    k, v = torch.empty((2, cache.n_seq, n, cache.n_kv, cache.head_dim), dtype=dtype, device=cache.device)
+    shape = (cache.n_seq, n, cache.n_kv, cache.head_dim)
+    k, v = cache.k.new_empty(shape, dtype=dtype), cache.k.new_empty(shape, dtype=dtype)
     check(lib().syn_kv_read(cache.ref, layer, _need(rows, torch.int32, cache.n_seq * n, "rows"), first, n,
-                            F16 if dtype == torch.float16 else F32, k.data_ptr(), v.data_ptr(), _stream(stream)),
-          "syn_kv_read")
+                            F16 if dtype == torch.float16 else F32, k.data_ptr(), v.data_ptr(),
+                            _on(stream, cache.device)), "syn_kv_read")
     return k, v
 
 
 def kv_move(cache, path, count, begin, stream=None):
     """Rows path[s][i] (int32, ascending, >= begin[s] + i) of sequence s become rows begin[s] + i, i < count[s], in
     every layer."""
-    torch = _torch()
-    ld = path.shape[-1]
-    check(lib().syn_kv_move(cache.ref, _need(path, torch.int32, cache.n_seq * ld, "path"), ld,
-                            _need(count, torch.int32, cache.n_seq, "count"),
-                            _need(begin, torch.int32, cache.n_seq, "begin"), _stream(stream)), "syn_kv_move")
+    i32, n, ld = _torch().int32, cache.n_seq, path.shape[-1]
+    check(lib().syn_kv_move(cache.ref, _need(path, i32, n * ld, "path"), ld, _need(count, i32, n, "count"),
+                            _need(begin, i32, n, "begin"), _on(stream, cache.device)), "syn_kv_move")
 
 
 def tree_attention_scratch(cache, tree, n_head, max_len=None):
     """A scratch for tree_attention calls of this shape; it may be kept for every later call on one stream."""
-    n = lib().syn_tree_attention_scratch_bytes(cache.n_seq, tree, n_head, cache.n_kv, cache.head_dim,
-                                               max_len or cache.max_ctx)
-    return empty_bytes(n, cache.device)
+    return empty_bytes(_tree_scratch_bytes(cache.n_seq, tree, n_head, cache.n_kv, cache.head_dim,
+                                           max_len or cache.max_ctx, cache.device), cache.device)
 
 
 def tree_attention(cache, q, len, n_head, scale, tree=1, mask=None, max_len=None, out=None, scratch=None, layer=0,
@@ -538,20 +553,22 @@ def tree_attention(cache, q, len, n_head, scale, tree=1, mask=None, max_len=None
     """Attention of `tree` tokens of every sequence over rows 0 .. len[s] - 1 and the tree's own rows after them that
     their mask bits name (None: a causal chunk); q [n_seq * tree][n_head * head_dim], rotated. See syn_tree_attention."""
     torch = _torch()
+    f32, i32 = torch.float32, torch.int32
     cols, rows = n_head * cache.head_dim, cache.n_seq * tree
     max_len = max_len or cache.max_ctx
-    qp, qs = _rows(q, cols, rows, "tree_attention q")
+    qp, qs = _rows(q, f32, cols, rows, "tree_attention q")
     if out is None:
-        out = torch.empty((rows, cols), dtype=torch.float32, device=q.device)
-    need = lib().syn_tree_attention_scratch_bytes(cache.n_seq, tree, n_head, cache.n_kv, cache.head_dim, max_len)
+        out = q.new_empty((rows, cols))
+    need = _tree_scratch_bytes(cache.n_seq, tree, n_head, cache.n_kv, cache.head_dim, max_len, cache.device)
     if scratch is None:
         scratch = empty_bytes(need, q.device)
     elif scratch.numel() * scratch.element_size() < need:
         raise ValueError(f"tree_attention: scratch of {need} bytes needed")
-    a = TreeAttentionArgs(qp, _need(out, torch.float32, rows * cols, "out"), _need(len, torch.int32, cache.n_seq, "len"),
-                          _need(mask, torch.int32, rows * ((tree + 31) // 32), "mask"), scratch.data_ptr(), qs, tree,
-                          n_head, max_len, scale)
-    check(lib().syn_tree_attention(cache.ref, layer, ctypes.byref(a), _stream(stream)), "syn_tree_attention")
+    a = TreeAttentionArgs(qp, _need(out, f32, rows * cols, "out"), _need(len, i32, cache.n_seq, "len"),
+                          _need(mask, i32, rows * ((tree + 31) // 32), "mask"), scratch.data_ptr(), qs, tree, n_head,
+                          max_len, scale)
+    check(lib().syn_tree_attention(cache.ref, layer, ctypes.byref(a), _on(stream, cache.device)),
+          "syn_tree_attention")
     return out
 
 
@@ -567,33 +584,38 @@ def logits_process(logits, n_seq, penalties=None, history=None, history_len=None
     tokens draft [n_seq][tree] with mask words, bias (begin [n_seq + 1], tokens, values), allowed [rows][words]. out
     may be logits itself; pick=False leaves the pick out. See syn_logits_process."""
     torch = _torch()
+    f32, i32 = torch.float32, torch.int32
     rows, vocab = logits.shape
     tree = rows // n_seq
     if tree * n_seq != rows:
         raise ValueError("logits_process: the same rows for every sequence")
-    xp, ld = _rows(logits, vocab, rows, "logits")
+    xp, ld = _rows(logits, f32, vocab, rows, "logits")
     if out is None:
-        out = torch.empty((rows, vocab), dtype=torch.float32, device=logits.device)
-    op, out_ld = _rows(out, vocab, rows, "out")
-    picks = torch.empty(rows, dtype=torch.int32, device=logits.device) if pick else None
-    if pick and scratch is None:
-        scratch = logits_scratch(rows, logits.device)
-    if pick and scratch.numel() * scratch.element_size() < lib().syn_logits_scratch_bytes(rows):
-        raise ValueError("logits_process: the scratch is too small")
-    i32, words = torch.int32, (vocab + 31) // 32
+        out = logits.new_empty((rows, vocab))
+    op, out_ld = _rows(out, f32, vocab, rows, "out")
+    picks = pp = sp = None
+    if pick:
+        picks = logits.new_empty(rows, dtype=i32)
+        if scratch is None:
+            scratch = logits_scratch(rows, logits.device)
+        elif scratch.numel() * scratch.element_size() < (12 * rows + 255) // 256 * 256:  # syn_logits_scratch_bytes
+            raise ValueError("logits_process: the scratch is too small")
+        pp, sp = picks.data_ptr(), scratch.data_ptr()
+    words = (vocab + 31) // 32
     begin, tokens, values = bias if bias is not None and bias[1].numel() else (None, None, None)
-    n = tokens.numel() if tokens is not None else None
-    if history is not None and history.dim() != 2:
-        raise ValueError("logits_process: history is [n_seq][ld]")
-    history_ld = history.shape[1] if history is not None else 0
-    a = LogitsArgs(xp, op, picks.data_ptr() if pick else None, ld, out_ld,
-                   _need(penalties, torch.float32, 3 * n_seq, "penalties"),
+    n = tokens.numel() if tokens is not None else 0
+    history_ld = 0
+    if history is not None:
+        if history.dim() != 2:
+            raise ValueError("logits_process: history is [n_seq][ld]")
+        history_ld = history.shape[1]
+    a = LogitsArgs(xp, op, pp, ld, out_ld, _need(penalties, f32, 3 * n_seq, "penalties"),
                    _need(history, i32, n_seq * history_ld, "history"), _need(history_len, i32, n_seq, "history_len"),
                    _need(draft, i32, rows, "draft"), _need(mask, i32, rows * ((tree + 31) // 32), "mask"),
                    _need(begin, i32, n_seq + 1, "bias begin"), _need(tokens, i32, n, "bias tokens"),
-                   _need(values, torch.float32, n, "bias values"), _need(allowed, i32, rows * words, "allowed"), words,
-                   scratch.data_ptr() if pick else None, n_seq, tree, vocab, history_ld)
-    check(lib().syn_logits_process(ctypes.byref(a), _stream(stream)), "syn_logits_process")
+                   _need(values, f32, n, "bias values"), _need(allowed, i32, rows * words, "allowed"), words, sp,
+                   n_seq, tree, vocab, history_ld)
+    check(lib().syn_logits_process(ctypes.byref(a), _on(stream, logits.device)), "syn_logits_process")
     return out, picks
 
 

@@ -8,6 +8,8 @@
 #include <cstdio>
 #include <cstring>
 #include <mutex>
+#include <utility>
+#include <vector>
 
 namespace {
 thread_local char g_last_error[256] = "";
@@ -50,6 +52,21 @@ PFN_cuTensorMapEncodeTiled_v12000 syn_tensor_map_encoder() {
             cudaGetLastError();
     });
     return fn;
+}
+
+// The dynamic shared memory opt-in of a kernel, once per device.
+int syn_opt_in_smem(const void* kernel, size_t bytes) {
+    static std::mutex mu;
+    static std::vector<std::pair<const void*, int>> done;
+    int dev = 0;
+    int st = syn_cuda_status(cudaGetDevice(&dev));
+    if (st) return st;
+    std::lock_guard<std::mutex> lock(mu);
+    for (const auto& d : done)
+        if (d.first == kernel && d.second == dev) return SYN_OK;
+    st = syn_cuda_status(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, int(bytes)));
+    if (!st) done.push_back({kernel, dev});
+    return st;
 }
 
 extern "C" const char* syn_build_info(void) { return "synapse_b200 0.1 sm_100a"; }

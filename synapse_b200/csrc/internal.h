@@ -61,6 +61,9 @@ extern "C" void syn_set_programmatic_launch(int on);
 // cuTensorMapEncodeTiled from the driver; NULL when it is not there.
 PFN_cuTensorMapEncodeTiled_v12000 syn_tensor_map_encoder();
 
+// The dynamic shared memory opt-in of a kernel, once per device.
+int syn_opt_in_smem(const void* kernel, size_t bytes);
+
 // Sets the thread's last error message.
 void syn_set_error(const char* msg);
 

@@ -16,88 +16,111 @@ struct AppendParams {
     const int32_t *slot, *pos;
     const float2* table;
     size_t kv_stride, q_stride;
-    int n, n_head, table_len, blocks_per_head;
+    int n, n_head, table_len;
     int neox;
 };
 
-// Q4_0 of one block of 32 values, one per lane: d = (the value of largest
-// magnitude, the first of equals) / -8, q = min(15, int(x / d + 8.5)); the
-// quant and the scale's bits.
-__device__ __forceinline__ int quantize_q4_lane(float x, uint16_t& dh) {
-    const uint32_t a = __float_as_uint(fabsf(x));
-    const uint32_t amax = __reduce_max_sync(0xffffffffu, a);
-    const int first = __ffs(__ballot_sync(0xffffffffu, a == amax)) - 1;
-    const float d = __fdiv_rn(__shfl_sync(0xffffffffu, x, first), -8.0f);
-    dh = f16_bits(d);
-    const float id = __fdiv_rn(1.0f, d);
-    // a scale that rounds to zero stores zeros (and 1 / d may not be finite)
-    return (dh & 0x7fff) ? min(15, int(__fadd_rn(__fmul_rn(x, id), 8.5f))) : 8;
-}
-
-// A warp takes blocks of 32 dims of a token's rows: n_head heads of q, then
-// n_kv of K, then n_kv of V, blocks_per_head each; lane = dim.
-template <int TYPE>
+// A thread takes 4 dims of a token's rows: n_head heads of q, then n_kv of K,
+// then n_kv of V; 8 neighbouring lanes hold a block of 32. VEC: rows and
+// strides allow 16-byte loads.
+template <int TYPE, bool VEC>
 __global__ void __launch_bounds__(256) kv_append_kernel(AppendParams a) {
     pdl_launch_dependents();
     pdl_wait();
-    const int lane = threadIdx.x & 31;
-    const int hd = a.c.hd, bph = a.blocks_per_head;
-    const int heads = (a.q ? a.n_head : 0) + 2 * a.c.n_kv;
+    const int hd = a.c.hd, quads = hd / 4, half = hd / 2;
+    const int nq = a.q ? a.n_head : 0, heads = nq + 2 * a.c.n_kv;
     const int tok = blockIdx.x;  // s * n + i
     const int slot = a.slot[tok];
     const int pos = a.pos ? a.pos[tok] : slot;
     if (slot < 0 || slot >= a.c.max_ctx) return;
     if (a.table && (pos < 0 || pos >= a.table_len)) return;
-    const int s = tok / a.n;
-    const int w0 = blockIdx.y * (blockDim.x >> 5) + (threadIdx.x >> 5), step = gridDim.y * (blockDim.x >> 5);
-    for (int w = w0; w < heads * bph; w += step) {
-        int h = w / bph;
-        const int b = w - h * bph, dim = b * 32 + lane;
-        const int nq = a.q ? a.n_head : 0;
+    const int s = tok / a.n, lane = threadIdx.x & 31;
+    auto load4 = [](const float* p) {
+        if (VEC) return *reinterpret_cast<const float4*>(p);
+        return make_float4(p[0], p[1], p[2], p[3]);
+    };
+    const float2* cs = a.table ? a.table + size_t(pos) * half : nullptr;
+    const int n = heads * quads;
+    for (int w = blockIdx.y * blockDim.x + (threadIdx.x & ~31); w < n; w += gridDim.y * blockDim.x) {
+        const int id = min(w + lane, n - 1);  // the last warp's spare lanes repeat the last quad and store nothing
+        const bool in = w + lane < n;
+        int h = id / quads;
+        const int d = (id - h * quads) * 4;
         const int kind = h < nq ? 0 : h < nq + a.c.n_kv ? 1 : 2;  // q, K, V
         h -= kind == 0 ? 0 : kind == 1 ? nq : nq + a.c.n_kv;
         const float* row = kind == 0 ? a.q + size_t(tok) * a.q_stride : (kind == 1 ? a.k : a.v) + size_t(tok) * a.kv_stride;
         row += size_t(h) * hd;
-        const bool in = dim < hd;
-        float x = in ? row[dim] : 0.0f;
-        if (kind != 2 && a.table) {
-            const int half = hd / 2;
-            const bool second = a.neox ? dim >= half : (dim & 1);
-            const int other = a.neox ? (second ? dim - half : dim + half) : dim ^ 1;
-            const int pair = a.neox ? (second ? dim - half : dim) : dim >> 1;
-            if (in) {
-                const float y = row[other];
-                const float2 cs = __ldg(a.table + size_t(pos) * half + pair);
-                // first: x c - y s; second: y s + x c (y is the first)
-                x = second ? __fadd_rn(__fmul_rn(y, cs.y), __fmul_rn(x, cs.x))
-                           : __fsub_rn(__fmul_rn(x, cs.x), __fmul_rn(y, cs.y));
+        const float4 v = load4(row + d);
+        float x[4] = {v.x, v.y, v.z, v.w};
+        if (kind != 2 && cs) {
+            if (a.neox) {  // pairs (i, i + hd / 2)
+                const bool second = d >= half;
+                const float4 o = load4(row + (second ? d - half : d + half));
+                const float y[4] = {o.x, o.y, o.z, o.w};
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    const float2 t = __ldg(cs + (second ? d - half : d) + e);
+                    x[e] = second ? __fadd_rn(__fmul_rn(y[e], t.y), __fmul_rn(x[e], t.x))
+                                  : __fsub_rn(__fmul_rn(x[e], t.x), __fmul_rn(y[e], t.y));
+                }
+            } else {  // pairs (2 i, 2 i + 1)
+#pragma unroll
+                for (int e = 0; e < 4; e += 2) {
+                    const float2 t = __ldg(cs + (d + e) / 2);
+                    const float y = x[e];
+                    x[e] = __fsub_rn(__fmul_rn(y, t.x), __fmul_rn(x[e + 1], t.y));
+                    x[e + 1] = __fadd_rn(__fmul_rn(y, t.y), __fmul_rn(x[e + 1], t.x));
+                }
             }
         }
-        if (kind == 0) {
-            if (in) a.q_out[(size_t(tok) * a.n_head + h) * hd + dim] = x;
-            continue;
-        }
         char* base = (kind == 1 ? a.c.k : a.c.v) + size_t(s) * a.c.seq_stride;
-        if (TYPE == SYN_F16) {
-            if (in) reinterpret_cast<uint16_t*>(base)[(size_t(slot) * a.c.n_kv + h) * hd + dim] = f16_bits(x);
-            continue;
+        if (kind == 0) {
+            if (in) *reinterpret_cast<float4*>(a.q_out + (size_t(tok) * a.n_head + h) * hd + d) = make_float4(x[0], x[1], x[2], x[3]);
+        } else if (TYPE == SYN_F16) {
+            const uint2 bits = make_uint2(uint32_t(f16_bits(x[0])) | uint32_t(f16_bits(x[1])) << 16,
+                                          uint32_t(f16_bits(x[2])) | uint32_t(f16_bits(x[3])) << 16);
+            if (in) *reinterpret_cast<uint2*>(reinterpret_cast<uint16_t*>(base) + (size_t(slot) * a.c.n_kv + h) * hd + d) = bits;
         }
+        if (TYPE == SYN_F16 || __all_sync(0xffffffffu, kind == 0)) continue;
         // quantised rows hold finite values only: clamped to binary16's range, NaN as 0
-        x = x != x ? 0.0f : fminf(fmaxf(x, -65504.0f), 65504.0f);
-        const size_t block = (size_t(h) * a.c.max_ctx + slot) * bph + b;
+        uint32_t top = 0;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            x[e] = x[e] != x[e] ? 0.0f : fminf(fmaxf(x[e], -65504.0f), 65504.0f);
+            top = max(top, __float_as_uint(fabsf(x[e])));
+        }
+        const uint32_t mine = top;
+#pragma unroll
+        for (int o = 1; o < 8; o <<= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
+        const size_t block = (size_t(h) * a.c.max_ctx + slot) * (hd / QK) + d / QK;
         uint16_t* scale = reinterpret_cast<uint16_t*>(base + a.c.scale_plane) + block;
         if (TYPE == SYN_Q8_0) {
-            const float d = __fdiv_rn(__uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(fabsf(x)))), 127.0f);
-            const uint16_t dh = f16_bits(d);
-            const int q = dh ? int(roundf(__fmul_rn(x, __fdiv_rn(1.0f, d)))) : 0;
-            reinterpret_cast<int8_t*>(base)[block * 32 + lane] = int8_t(q);
-            if (lane == 0) *scale = dh;
+            const float dd = __fdiv_rn(__uint_as_float(top), 127.0f), id8 = __fdiv_rn(1.0f, dd);
+            const uint16_t dh = f16_bits(dd);
+            uint32_t word = 0;  // a scale that rounds to zero stores zeros (and 1 / d may not be finite)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) word |= (dh ? uint32_t(int(roundf(__fmul_rn(x[e], id8)))) & 255u : 0u) << (8 * e);
+            if (in && kind != 0) {
+                *reinterpret_cast<uint32_t*>(base + block * 32 + (d & 31)) = word;
+                if ((lane & 7) == 0) *scale = dh;
+            }
         } else {
-            uint16_t dh;
-            const int q = quantize_q4_lane(x, dh);
-            const int hi = __shfl_down_sync(0xffffffffu, q, 16);
-            if (lane < 16) reinterpret_cast<uint8_t*>(base)[block * 16 + lane] = uint8_t(q | (hi << 4));
-            if (lane == 0) *scale = dh;
+            // d = (the value of largest magnitude, the first of equals) / -8, q = min(15, int(x / d + 8.5))
+            float first = 0.0f;
+#pragma unroll
+            for (int e = 3; e >= 0; --e)
+                if (__float_as_uint(fabsf(x[e])) == top) first = x[e];
+            const unsigned who = __ballot_sync(0xffffffffu, mine == top) >> (lane & 24) & 255u;
+            first = __shfl_sync(0xffffffffu, first, (lane & 24) + __ffs(who) - 1);
+            const float dd = __fdiv_rn(first, -8.0f), id4 = __fdiv_rn(1.0f, dd);
+            const uint16_t dh = f16_bits(dd);
+            uint32_t word = 0;
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+                word |= uint32_t((dh & 0x7fff) ? min(15, int(__fadd_rn(__fmul_rn(x[e], id4), 8.5f))) : 8) << (8 * e);
+            const uint32_t high = __shfl_down_sync(0xffffffffu, word, 4);
+            if (in && kind != 0 && (lane & 4) == 0) *reinterpret_cast<uint32_t*>(base + block * 16 + (d & 15)) = word | high << 4;
+            if (in && kind != 0 && (lane & 7) == 0) *scale = dh;
         }
     }
 }
@@ -107,68 +130,82 @@ struct ReadParams {
     KvView c;
     const int32_t* rows;
     void *k_out, *v_out;
-    size_t items;  // units of all rows of K (V alike)
-    int first, n, units, f16;
+    int first, n, units;
 };
 
-template <bool F16OUT>
-__device__ __forceinline__ void store8(void* out, size_t at, const float (&f)[8]) {
-    if (F16OUT) {
-        uint32_t h[4];
-#pragma unroll
-        for (int e = 0; e < 4; ++e) h[e] = uint32_t(f16_bits(f[2 * e])) | uint32_t(f16_bits(f[2 * e + 1])) << 16;
-        *reinterpret_cast<uint4*>(static_cast<uint16_t*>(out) + at) = make_uint4(h[0], h[1], h[2], h[3]);
-    } else {
-        float4* o = reinterpret_cast<float4*>(static_cast<float*>(out) + at);
-        o[0] = make_float4(f[0], f[1], f[2], f[3]);
-        o[1] = make_float4(f[4], f[5], f[6], f[7]);
-    }
-}
+constexpr int kReadRows = 4;  // rows of a thread, loaded together
 
-// A thread takes one unit of 8 values of a row: consecutive threads take the
-// units of one (row, head), then the next heads of the row.
+// A CTA takes kReadRows * (256 / units) rows of one head of K or V of a
+// sequence; a thread one unit (16 bytes of the output: 8 or 4 values) of
+// kReadRows of them, so that a warp's stores are whole lines.
 template <int TYPE, bool F16OUT>
 __global__ void __launch_bounds__(256) kv_read_kernel(ReadParams a) {
     pdl_launch_dependents();
     pdl_wait();
-    const int hd = a.c.hd, upr = hd / 8;
-    const char* plane = blockIdx.y ? a.c.v : a.c.k;
-    void* out = blockIdx.y ? a.v_out : a.k_out;
-    for (size_t i = size_t(blockIdx.x) * blockDim.x + threadIdx.x; i < a.items; i += size_t(gridDim.x) * blockDim.x) {
-        const int u = int(i % upr);
-        const size_t rh = i / upr;
-        const int h = int(rh % a.c.n_kv);
-        const size_t r = rh / a.c.n_kv;  // s * n + row
-        const int s = int(r / a.n);
-        const int row = a.rows ? a.rows[r] : a.first + int(r - size_t(s) * a.n);
-        float f[8] = {};
-        if (row >= 0 && row < a.c.max_ctx) {
-            const char* base = plane + size_t(s) * a.c.seq_stride;
+    constexpr int V = F16OUT ? 8 : 4;
+    const int hd = a.c.hd, h = blockIdx.y, s = blockIdx.z >> 1;
+    const char* base = ((blockIdx.z & 1) ? a.c.v : a.c.k) + size_t(s) * a.c.seq_stride;
+    void* out = (blockIdx.z & 1) ? a.v_out : a.k_out;
+    const int per = 256 / a.units, r0 = threadIdx.x / a.units, u = threadIdx.x - r0 * a.units;
+    if (!out || r0 >= per) return;
+    const int i0 = blockIdx.x * per * kReadRows + r0;
+    uint32_t x[kReadRows][V / (TYPE == SYN_F16 ? 2 : 4)];
+    uint16_t d[kReadRows];
+    auto load = [](auto& to, const char* p) {
+        constexpr int n = sizeof(to) / 4;
+        if constexpr (n == 4) {
+            const uint4 v = __ldg(reinterpret_cast<const uint4*>(p));
+            to[0] = v.x; to[1] = v.y; to[2] = v.z; to[3] = v.w;
+        } else if constexpr (n == 2) {
+            const uint2 v = __ldg(reinterpret_cast<const uint2*>(p));
+            to[0] = v.x; to[1] = v.y;
+        } else {
+            to[0] = __ldg(reinterpret_cast<const uint32_t*>(p));
+        }
+    };
+#pragma unroll
+    for (int j = 0; j < kReadRows; ++j) {
+        const int i = i0 + j * per;
+        const int row = i >= a.n ? -1 : a.rows ? __ldg(a.rows + size_t(s) * a.n + i) : a.first + i;
+        d[j] = 0;  // with a scale of 0 any quants are 0
+#pragma unroll
+        for (auto& w : x[j]) w = 0;
+        if (row < 0 || row >= a.c.max_ctx) continue;
+        if (TYPE == SYN_F16) {
+            load(x[j], base + ((size_t(row) * a.c.n_kv + h) * hd + u * V) * 2);
+        } else {
+            const size_t block = (size_t(h) * a.c.max_ctx + row) * (hd / QK) + u * V / QK;
+            const int in = u * V % QK;  // Q4_0: byte j of a block holds values j and j + 16
+            load(x[j], base + (TYPE == SYN_Q8_0 ? block * 32 + in : block * 16 + in % 16));
+            d[j] = __ldg(reinterpret_cast<const uint16_t*>(base + a.c.scale_plane) + block);
+        }
+    }
+    const bool high = TYPE == SYN_Q4_0 && u * V % QK >= 16;
+#pragma unroll
+    for (int j = 0; j < kReadRows; ++j) {
+        const int i = i0 + j * per;
+        if (i >= a.n) continue;
+        const size_t at = ((size_t(s) * a.n + i) * a.c.n_kv + h) * hd + u * V;
+        const float scale = f16_from_bits(d[j]);
+        float f[V];
+#pragma unroll
+        for (int e = 0; e < V; ++e) {
             if (TYPE == SYN_F16) {
-                const uint4 x = __ldg(reinterpret_cast<const uint4*>(base + ((size_t(row) * a.c.n_kv + h) * hd + u * 8) * 2));
-                const uint32_t w[4] = {x.x, x.y, x.z, x.w};
-#pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    f[2 * e] = f16_from_bits(uint16_t(w[e]));
-                    f[2 * e + 1] = f16_from_bits(uint16_t(w[e] >> 16));
-                }
+                f[e] = f16_from_bits(uint16_t(x[j][e >> 1] >> (16 * (e & 1))));
             } else {
-                const int b = u >> 2, part = u & 3;
-                const size_t block = (size_t(h) * a.c.max_ctx + row) * (hd / QK) + b;
-                const float d = f16_from_bits(__ldg(reinterpret_cast<const uint16_t*>(base + a.c.scale_plane) + block));
-                // Q4_0: values 0-15 are the block's low nibbles, 16-31 the high ones
-                const uint2 x = __ldg(reinterpret_cast<const uint2*>(
-                    base + (TYPE == SYN_Q8_0 ? block * 32 + part * 8 : block * 16 + (part & 1) * 8)));
-                const uint32_t w[2] = {x.x, x.y};
-#pragma unroll
-                for (int e = 0; e < 8; ++e) {
-                    const uint32_t byte = w[e >> 2] >> (8 * (e & 3)) & 255u;
-                    const int q = TYPE == SYN_Q8_0 ? int(int8_t(byte)) : int(part < 2 ? byte & 15u : byte >> 4) - 8;
-                    f[e] = __fmul_rn(float(q), d);
-                }
+                const uint32_t byte = x[j][e >> 2] >> (8 * (e & 3));
+                const int q = TYPE == SYN_Q8_0 ? int(int8_t(byte)) : int((high ? byte >> 4 : byte) & 15u) - 8;
+                f[e] = __fmul_rn(float(q), scale);
             }
         }
-        store8<F16OUT>(out, i * 8, f);
+        if constexpr (F16OUT) {
+            uint32_t w[4];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) w[e] = uint32_t(f16_bits(f[2 * e])) | uint32_t(f16_bits(f[2 * e + 1])) << 16;
+            *reinterpret_cast<uint4*>(static_cast<uint16_t*>(out) + at) = make_uint4(w[0], w[1], w[2], w[3]);
+        } else {
+            *reinterpret_cast<float4*>(static_cast<float*>(out) + at) = make_float4(f[0], f[1], f[2], f[3]);
+        }
     }
 }
 
@@ -259,18 +296,21 @@ extern "C" int syn_kv_append(const syn_kv_cache* c, int layer, const syn_kv_appe
     if (x->q && x->q == x->q_out) return SYN_ERR_INVALID;  // pairs read each other's element
     a.n = x->n; a.n_head = x->q ? x->n_head : 0;
     a.table_len = x->table_len;
-    a.blocks_per_head = (c->head_dim + 31) / 32;
     a.neox = x->rope_mode;
     const size_t tokens = size_t(c->n_seq) * x->n;
     if (tokens > 0x7fffffff) return SYN_ERR_UNSUPPORTED;
-    const int tasks = (a.n_head + 2 * c->n_kv) * a.blocks_per_head;
-    // few tokens: a warp per task; many: a CTA of 8 warps per token
-    const unsigned y = tokens < 64 ? unsigned((tasks + 7) / 8) : 1u;
+    const int quads = (a.n_head + 2 * c->n_kv) * (c->head_dim / 4);
+    // few tokens: a thread per quad; many: a CTA per token
+    const unsigned y = tokens < 256 ? unsigned((quads + 255) / 256) : 1u;
     const dim3 grid{unsigned(tokens), y, 1};
+    const bool vec = aligned(x->k, 16) && aligned(x->v, 16) && aligned(x->q, 16) && a.kv_stride % 4 == 0 && a.q_stride % 4 == 0;
+    if (x->q && !aligned(x->q_out, 16)) return SYN_ERR_INVALID;
     cudaStream_t s = static_cast<cudaStream_t>(stream);
-    if (c->type == SYN_F16) return syn_launch(kv_append_kernel<SYN_F16>, grid, 256, 0, s, a);
-    if (c->type == SYN_Q8_0) return syn_launch(kv_append_kernel<SYN_Q8_0>, grid, 256, 0, s, a);
-    return syn_launch(kv_append_kernel<SYN_Q4_0>, grid, 256, 0, s, a);
+    if (c->type == SYN_F16)
+        return vec ? syn_launch(kv_append_kernel<SYN_F16, true>, grid, 256, 0, s, a) : syn_launch(kv_append_kernel<SYN_F16, false>, grid, 256, 0, s, a);
+    if (c->type == SYN_Q8_0)
+        return vec ? syn_launch(kv_append_kernel<SYN_Q8_0, true>, grid, 256, 0, s, a) : syn_launch(kv_append_kernel<SYN_Q8_0, false>, grid, 256, 0, s, a);
+    return vec ? syn_launch(kv_append_kernel<SYN_Q4_0, true>, grid, 256, 0, s, a) : syn_launch(kv_append_kernel<SYN_Q4_0, false>, grid, 256, 0, s, a);
 }
 
 extern "C" int syn_kv_read(const syn_kv_cache* c, int layer, const int32_t* rows, int first, int n, int out_type,
@@ -283,13 +323,13 @@ extern "C" int syn_kv_read(const syn_kv_cache* c, int layer, const int32_t* rows
     if (!aligned(k_out, 16) || !aligned(v_out, 16)) return SYN_ERR_INVALID;
     ReadParams a{};
     a.c = kv_view(c, layer);
-    if (!k_out) a.c.k = a.c.v;  // one output: plane 0 is V
-    a.k_out = k_out ? k_out : v_out;
+    a.k_out = k_out;
     a.v_out = v_out;
     a.rows = rows; a.first = first; a.n = n;
-    a.items = size_t(c->n_seq) * n * c->n_kv * (c->head_dim / 8);
-    const size_t blocks = (a.items + 255) / 256;
-    const dim3 grid{unsigned(blocks < 0x7fffffff ? blocks : 0x7fffffff), k_out && v_out ? 2u : 1u, 1};
+    a.units = c->head_dim / (out_type == SYN_F16 ? 8 : 4);
+    const int per = 256 / a.units * kReadRows;
+    if (c->n_kv > 65535 || c->n_seq > 32767) return SYN_ERR_UNSUPPORTED;
+    const dim3 grid{unsigned((size_t(n) + per - 1) / per), unsigned(c->n_kv), unsigned(2 * c->n_seq)};
     cudaStream_t s = static_cast<cudaStream_t>(stream);
     const bool h = out_type == SYN_F16;
     switch (c->type) {

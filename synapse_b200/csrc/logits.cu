@@ -5,12 +5,19 @@
 // Bound by memory: each logit is read and written once. A CTA takes a chunk
 // of the vocabulary for the rows (tree nodes) of one sequence. It first
 // counts the sequence's history and sums its biases for the chunk's tokens in
-// shared memory (integer counts: the order of the atomics changes nothing),
-// with a bit per token that has either, so that the rows' pass reads the
-// counts only where there is something. A node's own path adds to the counts
-// before its row and is taken off after it, where a drafted token falls into
-// the chunk at all. The picks are joined by a 64-bit maximum of (ordered
-// value, lowest index), which does not depend on the order of arrival.
+// shared memory (integer counts: the order of the atomics changes nothing)
+// with a bit for every token that has either or that the tree has drafted.
+// Then, row by row, a thread holds vectors of the row; for its marked tokens it
+// computes the penalties (with the node's path added to their counts) in a loop
+// over them, before the mask, the store and the maximum. Which of a thread's
+// values are marked is the same in every row.
+// Measured for 256 rows of 128256, histories of up to 4096, with a grammar:
+// every value tested where it is held, 107 us (nearly every warp meets a marked
+// token and takes the long way for each of a vector's values); marked tokens
+// done afterwards in global memory, 111 us; marked tokens handed to a thread
+// each through shared memory, 74 us (two barriers a row). The picks are joined
+// by a 64-bit maximum of (ordered value, lowest index), which does not depend on
+// the order of arrival.
 #include "common.cuh"
 
 #include <algorithm>
@@ -21,7 +28,7 @@ namespace {
 
 constexpr int kThreads = 256;
 constexpr int kMaxTree = 1024;
-constexpr int kMaxRows = 64;  // rows (nodes) of one CTA
+constexpr int kMaxRows = 8;  // rows (nodes) of one CTA: few enough that the CTAs' number evens out over the SMs
 
 struct LogitParams {
     const float* x;
@@ -39,14 +46,27 @@ struct LogitParams {
     int n_tree, n_vocab, history_ld, rows_per_cta;
 };
 
+// Counts: 32 bits in the short chunks, 16 (two to a word) in the long ones,
+// whose CTAs then fit an SM four at a time; the host gives histories that
+// could pass 16 bits to the short chunks.
 template <int CHUNK>
 struct Shared {
-    int count[CHUNK];
+    static constexpr bool wide = CHUNK <= 1024;
+    unsigned count[wide ? CHUNK : CHUNK / 2];
     float bias[CHUNK];
-    unsigned touched[CHUNK / 32];  // tokens that may have a count or a bias
+    float x[CHUNK];                   // a thread's own vectors, where it indexes them
+    unsigned touched[CHUNK / 32];     // the tokens that may have a count or a bias
+    unsigned drafted[CHUNK / 32];     // those some node of the tree has
     unsigned long long best[kMaxRows];
-    unsigned short mine[kMaxTree];  // drafted tokens in this chunk, by node
+    unsigned short mine[kMaxTree];    // the nodes whose tokens are in this chunk
     int n_mine;
+    __device__ __forceinline__ void add(int at) {
+        if (wide) atomicAdd(&count[at], 1u);
+        else atomicAdd(&count[at >> 1], 1u << (16 * (at & 1)));
+    }
+    __device__ __forceinline__ int counted(int at) const {
+        return wide ? int(count[at]) : int(count[at >> 1] >> (16 * (at & 1)) & 0xffffu);
+    }
 };
 
 // A float's bits in the order of the floats; 0 for NaN and -inf.
@@ -55,17 +75,25 @@ __device__ __forceinline__ uint32_t ordered(float x) {
     return x > -INFINITY ? (b & 0x80000000u ? ~b : b | 0x80000000u) : 0u;
 }
 
+// A vector that is read once: not kept in L1, whose space in flight loads need.
+__device__ __forceinline__ float4 load_once(const float* p) {
+    float4 v;
+    asm volatile("ld.global.L1::no_allocate.v4.f32 {%0,%1,%2,%3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "l"(p) : "memory");
+    return v;
+}
+
 template <int CHUNK, int VEC>
-__global__ void __launch_bounds__(kThreads) logits_kernel(const LogitParams a) {
+__global__ void __launch_bounds__(kThreads, 4) logits_kernel(const LogitParams a) {
     extern __shared__ __align__(16) unsigned char raw[];
     Shared<CHUNK>& sh = *reinterpret_cast<Shared<CHUNK>*>(raw);
+    constexpr int kPer = CHUNK / (VEC * kThreads);  // vectors of a thread
     const int tid = threadIdx.x, lane = tid & 31;
-    const int seq = blockIdx.z, v0 = blockIdx.x * CHUNK;
+    const int seq = blockIdx.z, v0 = blockIdx.x * CHUNK, span = min(CHUNK, a.n_vocab - v0);
     const int i0 = blockIdx.y * a.rows_per_cta, n_rows = min(a.rows_per_cta, a.n_tree - i0);
     for (int i = tid; i < CHUNK; i += kThreads) {
-        sh.count[i] = 0;
+        if (i < int(sizeof(sh.count) / 4)) sh.count[i] = 0;
         sh.bias[i] = 0.0f;
-        if (i < CHUNK / 32) sh.touched[i] = 0;
+        if (i < CHUNK / 32) sh.touched[i] = sh.drafted[i] = 0;
     }
     for (int i = tid; i < n_rows; i += kThreads) sh.best[i] = 0;
     if (tid == 0) sh.n_mine = 0;
@@ -73,23 +101,50 @@ __global__ void __launch_bounds__(kThreads) logits_kernel(const LogitParams a) {
     pdl_launch_dependents();
     pdl_wait();
 
+    constexpr unsigned kAll = (1u << VEC) - 1u;
+    const int words = (a.n_tree + 31) / 32;
+    const bool full = span == CHUNK;
+    float f[kPer][VEC];
+    unsigned allowed = ~0u;  // a word of the grammar in each of the first kPer * VEC lanes
+    auto load = [&](int i) {
+        const size_t row = size_t(seq) * a.n_tree + i0 + i;
+        const float* x = a.x + row * a.ld + v0 + tid * VEC;
+        if (VEC == 4 && full) {
+#pragma unroll
+            for (int k = 0; k < kPer; ++k) {
+                const float4 v = load_once(x + k * kThreads * VEC);
+                f[k][0] = v.x; f[k][1 % VEC] = v.y; f[k][2 % VEC] = v.z; f[k][3 % VEC] = v.w;
+            }
+        } else {
+#pragma unroll
+            for (int k = 0; k < kPer; ++k)
+#pragma unroll
+                for (int e = 0; e < VEC; ++e) {
+                    const int at = (k * kThreads + tid) * VEC + e;
+                    f[k][e] = at < span ? x[k * kThreads * VEC + e] : -INFINITY;
+                }
+        }
+        if (a.allowed && lane < kPer * VEC) {  // the warp's vectors k cover VEC words from k * 8 VEC + warp * VEC on
+            const int w = lane / VEC * (kThreads * VEC / 32) + (tid >> 5) * VEC + lane % VEC;
+            if (32 * w < span) allowed = __ldg(a.allowed + row * a.allowed_ld + (v0 >> 5) + w);
+        }
+    };
+    load(0);  // on its way while the counts are made
+
     auto touch = [&](int at) { atomicOr(&sh.touched[at >> 5], 1u << (at & 31)); };
-    const int span = min(CHUNK, a.n_vocab - v0);
     if (a.history) {
         const int n = min(a.history_len[seq], a.history_ld);
         const int32_t* h = a.history + size_t(seq) * a.history_ld;
-        for (int i = tid; i < n; i += 4 * kThreads) {
-            int tok[4];
+        for (int i = tid; i < n; i += 8 * kThreads) {
+            int tok[8];
 #pragma unroll
-            for (int j = 0; j < 4; ++j) tok[j] = i + j * kThreads < n ? __ldg(h + i + j * kThreads) : -1;
+            for (int j = 0; j < 8; ++j) tok[j] = i + j * kThreads < n ? __ldg(h + i + j * kThreads) : -1;
 #pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                const int at = tok[j] - v0;
-                if (tok[j] >= v0 && at < span) {
-                    atomicAdd(&sh.count[at], 1);
-                    touch(at);
+            for (int j = 0; j < 8; ++j)
+                if (tok[j] >= v0 && tok[j] - v0 < span) {
+                    sh.add(tok[j] - v0);
+                    touch(tok[j] - v0);
                 }
-            }
         }
     }
     if (a.bias_begin) {
@@ -109,93 +164,94 @@ __global__ void __launch_bounds__(kThreads) logits_kernel(const LogitParams a) {
             if (tok >= v0 && tok - v0 < span) {
                 sh.mine[atomicAdd(&sh.n_mine, 1)] = static_cast<unsigned short>(j);
                 touch(tok - v0);
+                atomicOr(&sh.drafted[(tok - v0) >> 5], 1u << ((tok - v0) & 31));
             }
         }
     __syncthreads();
     const int n_mine = sh.n_mine;
-    const int words = (a.n_tree + 31) / 32;
     const float repeat = a.penalties ? a.penalties[3 * seq] : 1.0f;
     const float presence = a.penalties ? a.penalties[3 * seq + 1] : 0.0f;
     const float frequency = a.penalties ? a.penalties[3 * seq + 2] : 0.0f;
+    unsigned some = 0;  // which of this thread's values may change
+#pragma unroll
+    for (int k = 0; k < kPer; ++k) {
+        const int at = (k * kThreads + tid) * VEC;
+        some |= (sh.touched[at >> 5] >> (at & 31) & kAll) << (k * VEC);
+    }
 
-    constexpr int kPer = CHUNK / (VEC * kThreads);  // vectors of a thread
     for (int i = 0; i < n_rows; ++i) {
         const int node = i0 + i;
         const size_t row = size_t(seq) * a.n_tree + node;
-        auto path = [&](int sign) {
-            for (int k = tid; k < n_mine; k += kThreads) {
-                const int j = sh.mine[k];
-                const bool on = a.mask ? a.mask[row * words + (j >> 5)] >> (j & 31) & 1u : j <= node;
-                if (on) atomicAdd(&sh.count[draft[j] - v0], sign);
+        if (some) {  // through shared memory, for their indexes are not known to the compiler
+            float* x = sh.x + tid * VEC;
+#pragma unroll
+            for (int k = 0; k < kPer; ++k) {
+                if constexpr (VEC == 4) *reinterpret_cast<float4*>(x + k * kThreads * VEC) = make_float4(f[k][0], f[k][1], f[k][2], f[k][3]);
+                else x[k * kThreads] = f[k][0];
             }
-            __syncthreads();
-        };
-        const float* x = a.x + row * a.ld + v0;
-        float f[kPer][VEC];
-#pragma unroll
-        for (int k = 0; k < kPer; ++k) {
-            const int at = (k * kThreads + tid) * VEC;
-            const bool whole = VEC == 4 && at + 3 < span;
-            if constexpr (VEC == 4) {
-                if (whole) {
-                    const float4 v = *reinterpret_cast<const float4*>(x + at);
-                    f[k][0] = v.x; f[k][1] = v.y; f[k][2] = v.z; f[k][3] = v.w;
-                }
-            }
-            if (!whole)
-#pragma unroll
-                for (int e = 0; e < VEC; ++e) f[k][e] = at + e < span ? x[at + e] : -INFINITY;
-        }
-        if (n_mine) path(1);
-        uint32_t top = 0;
-        int top_at = 0;
-#pragma unroll
-        for (int k = 0; k < kPer; ++k) {
-            const int at = (k * kThreads + tid) * VEC;
-            if (at >= span) continue;
-            const unsigned some = sh.touched[at >> 5] >> (at & 31);
-            unsigned allowed = ~0u;
-            if (a.allowed) allowed = __ldg(a.allowed + row * a.allowed_ld + ((v0 + at) >> 5)) >> (at & 31);
-#pragma unroll
-            for (int e = 0; e < VEC; ++e) {
-                if (some >> e & 1u) {
-                    const int c = sh.count[at + e];
-                    float y = f[k][e] + sh.bias[at + e];
-                    if (c > 0) {
-                        y = y > 0.0f ? __fdiv_rn(y, repeat) : y * repeat;
-                        y -= float(c) * frequency + presence;
+            for (unsigned left = some; left; left &= left - 1) {
+                const int b = __ffs(left) - 1, at = (b / VEC * kThreads + tid) * VEC + b % VEC;
+                float y = sh.x[at] + sh.bias[at];
+                int c = sh.counted(at);
+                if (n_mine && (sh.drafted[at >> 5] >> (at & 31) & 1u))
+                    for (int d = 0; d < n_mine; ++d) {
+                        const int j = sh.mine[d];
+                        if (draft[j] == v0 + at && (a.mask ? a.mask[row * words + (j >> 5)] >> (j & 31) & 1u : j <= node)) ++c;
                     }
-                    f[k][e] = y;
+                if (c > 0) {
+                    y = y > 0.0f ? __fdiv_rn(y, repeat) : y * repeat;
+                    y -= float(c) * frequency + presence;
                 }
-                if (!(allowed >> e & 1u)) f[k][e] = -INFINITY;
-                const uint32_t o = at + e < span ? ordered(f[k][e]) : 0u;
-                if (o > top) {
-                    top = o;
-                    top_at = at + e;
+                sh.x[at] = y;
+            }
+#pragma unroll
+            for (int k = 0; k < kPer; ++k) {
+                if constexpr (VEC == 4) {
+                    const float4 v = *reinterpret_cast<const float4*>(x + k * kThreads * VEC);
+                    f[k][0] = v.x; f[k][1] = v.y; f[k][2] = v.z; f[k][3] = v.w;
+                } else {
+                    f[k][0] = x[k * kThreads];
                 }
             }
-            if (a.out) {
-                float* y = a.out + row * a.out_ld + v0;
-                const bool whole = VEC == 4 && at + 3 < span;
-                if constexpr (VEC == 4) {
-                    if (whole)
-                        *reinterpret_cast<float4*>(y + at) = make_float4(f[k][0], f[k][1], f[k][2], f[k][3]);
-                }
-                if (!whole)
+        }
+        __syncwarp();
+        if (a.allowed)
+#pragma unroll
+            for (int k = 0; k < kPer; ++k) {
+                const unsigned may = __shfl_sync(0xffffffffu, allowed, k * VEC + lane * VEC / 32) >> (lane * VEC & 31);
+#pragma unroll
+                for (int e = 0; e < VEC; ++e)
+                    if (!(may >> e & 1u)) f[k][e] = -INFINITY;
+            }
+        if (a.out) {
+            float* out = a.out + row * a.out_ld + v0 + tid * VEC;
+            if (VEC == 4 && full) {
+#pragma unroll
+                for (int k = 0; k < kPer; ++k)
+                    __stcs(reinterpret_cast<float4*>(out + k * kThreads * VEC), make_float4(f[k][0], f[k][1 % VEC], f[k][2 % VEC], f[k][3 % VEC]));
+            } else {
+#pragma unroll
+                for (int k = 0; k < kPer; ++k)
 #pragma unroll
                     for (int e = 0; e < VEC; ++e)
-                        if (at + e < span) y[at + e] = f[k][e];
+                        if ((k * kThreads + tid) * VEC + e < span) out[k * kThreads * VEC + e] = f[k][e];
             }
         }
         if (a.pick) {
-            const uint32_t best = __reduce_max_sync(0xffffffffu, top);
-            const uint32_t at = __reduce_min_sync(0xffffffffu, top == best ? uint32_t(v0 + top_at) : 0xffffffffu);
-            if (lane == 0 && best) atomicMax(&sh.best[i], static_cast<unsigned long long>(best) << 32 | (0xffffffffu - at));
+            float top = f[0][0];
+#pragma unroll
+            for (int k = 0; k < kPer * VEC; ++k) top = fmaxf(top, f[k / VEC][k % VEC]);  // a NaN loses
+            const uint32_t o = ordered(top), best = __reduce_max_sync(0xffffffffu, o);
+            // the warp's largest, where the CTA has none larger so far
+            if (o == best && o && o >= uint32_t(*reinterpret_cast<volatile unsigned long long*>(&sh.best[i]) >> 32)) {
+                int at = 0;
+#pragma unroll
+                for (int k = kPer * VEC - 1; k >= 0; --k)
+                    if (f[k / VEC][k % VEC] == top) at = (k / VEC * kThreads + tid) * VEC + k % VEC;
+                atomicMax(&sh.best[i], static_cast<unsigned long long>(o) << 32 | (0xffffffffu - uint32_t(v0 + at)));
+            }
         }
-        if (n_mine) {
-            __syncthreads();
-            path(-1);
-        }
+        if (i + 1 < n_rows) load(i + 1);
     }
     if (!a.pick) return;
     __syncthreads();
@@ -220,6 +276,8 @@ int launch(LogitParams a, int n_seq, cudaStream_t s) {
     const int groups = int(std::max<long>(1, 2l * syn_num_sms() / ctas));
     a.rows_per_cta = std::min(kMaxRows, (a.n_tree + groups - 1) / groups);
     const dim3 grid{unsigned(chunks), unsigned((a.n_tree + a.rows_per_cta - 1) / a.rows_per_cta), unsigned(n_seq)};
+    const int st = syn_opt_in_smem(reinterpret_cast<const void*>(logits_kernel<CHUNK, VEC>), sizeof(Shared<CHUNK>));
+    if (st) return st;
     return syn_launch(logits_kernel<CHUNK, VEC>, grid, kThreads, sizeof(Shared<CHUNK>), s, a);
 }
 
@@ -256,7 +314,8 @@ extern "C" int syn_logits_process(const syn_logits_args* x, void* stream) {
     const uintptr_t at = reinterpret_cast<uintptr_t>(x->logits) | reinterpret_cast<uintptr_t>(x->out);
     const bool vec = (at & 15) == 0 && a.ld % 4 == 0 && (!x->out || a.out_ld % 4 == 0);
     // short chunks while the long ones would not give every SM two CTAs
-    const bool few = rows * ((size_t(x->n_vocab) + 4095) / 4096) < size_t(2) * syn_num_sms();
+    const bool few = rows * ((size_t(x->n_vocab) + 4095) / 4096) < size_t(2) * syn_num_sms() ||
+                     (x->history && size_t(x->history_ld) + x->n_tree > 0xffff);  // counts of more than 16 bits
     if (few) return vec ? launch<1024, 4>(a, x->n_seq, s) : launch<1024, 1>(a, x->n_seq, s);
     return vec ? launch<4096, 4>(a, x->n_seq, s) : launch<4096, 1>(a, x->n_seq, s);
 }

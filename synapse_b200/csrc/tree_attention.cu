@@ -25,8 +25,6 @@
 #include "tree_attention.cuh"
 
 #include <algorithm>
-#include <mutex>
-#include <vector>
 
 using namespace syn;
 
@@ -655,21 +653,6 @@ int launch_type(const TreeParams& a, cudaStream_t s) {
 }
 
 }  // namespace
-
-// The dynamic shared memory opt-in of a kernel, once per device.
-int syn_opt_in_smem(const void* kernel, size_t bytes) {
-    static std::mutex mu;
-    static std::vector<std::pair<const void*, int>> done;
-    int dev = 0;
-    int st = syn_cuda_status(cudaGetDevice(&dev));
-    if (st) return st;
-    std::lock_guard<std::mutex> lock(mu);
-    for (const auto& d : done)
-        if (d.first == kernel && d.second == dev) return SYN_OK;
-    st = syn_cuda_status(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, int(bytes)));
-    if (!st) done.push_back({kernel, dev});
-    return st;
-}
 
 extern "C" size_t syn_tree_attention_scratch_bytes(int n_seq, int n_tree, int n_head, int n_kv, int head_dim,
                                                    int max_len) {

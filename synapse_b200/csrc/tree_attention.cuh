@@ -72,4 +72,3 @@ __device__ __forceinline__ float part_weight(float m, float l, float top) {
 // heads of up to 128 dims; a.splits counts runs of 64 positions' tiles.
 constexpr int kTcRows = 128, kTcTile = 64;
 int syn_tree_attention_tc(const syn::TreeParams& a, int type, cudaStream_t s);
-int syn_opt_in_smem(const void* kernel, size_t bytes);
