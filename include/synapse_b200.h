@@ -326,8 +326,10 @@ int syn_kv_move(const syn_kv_cache* c, const int32_t* path, int path_ld, const i
  * the heads that read it.
  * len[s] is clamped to [0, max_len - n_tree]; max_len <= max_ctx bounds
  * len[s] + n_tree and sizes the split of the context over the GPU.
- * scratch: syn_tree_attention_scratch_bytes, 16-byte aligned; calls whose GPU
- * work overlaps need scratches of their own. */
+ * scratch: syn_tree_attention_scratch_bytes, 16-byte aligned, its first 4096
+ * bytes zeroed once before its first use (each call leaves them zero, ready
+ * for the next of any shape); calls whose GPU work overlaps need scratches of
+ * their own. */
 typedef struct {
     const float* q;          /* [n_seq * n_tree][n_head * head_dim], rotated */
     float* out;              /* contiguous [n_seq * n_tree][n_head * head_dim], 16-byte aligned */

@@ -544,8 +544,14 @@ def kv_move(cache, path, count, begin, stream=None):
 
 def tree_attention_scratch(cache, tree, n_head, max_len=None):
     """A scratch for tree_attention calls of this shape; it may be kept for every later call on one stream."""
-    return empty_bytes(_tree_scratch_bytes(cache.n_seq, tree, n_head, cache.n_kv, cache.head_dim,
-                                           max_len or cache.max_ctx, cache.device), cache.device)
+    return _tree_scratch(_tree_scratch_bytes(cache.n_seq, tree, n_head, cache.n_kv, cache.head_dim,
+                                             max_len or cache.max_ctx, cache.device), cache.device)
+
+
+def _tree_scratch(n, device):
+    scratch = empty_bytes(n, device)
+    scratch[:4096].zero_()
+    return scratch
 
 
 def tree_attention(cache, q, len, n_head, scale, tree=1, mask=None, max_len=None, out=None, scratch=None, layer=0,
@@ -561,7 +567,7 @@ def tree_attention(cache, q, len, n_head, scale, tree=1, mask=None, max_len=None
         out = q.new_empty((rows, cols))
     need = _tree_scratch_bytes(cache.n_seq, tree, n_head, cache.n_kv, cache.head_dim, max_len, cache.device)
     if scratch is None:
-        scratch = empty_bytes(need, q.device)
+        scratch = _tree_scratch(need, q.device)
     elif scratch.numel() * scratch.element_size() < need:
         raise ValueError(f"tree_attention: scratch of {need} bytes needed")
     a = TreeAttentionArgs(qp, _need(out, f32, rows * cols, "out"), _need(len, i32, cache.n_seq, "len"),

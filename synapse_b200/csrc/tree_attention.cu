@@ -4,16 +4,20 @@
 //
 // A KV head's work is one matrix product over the rows r = token * G + head of
 // its group (G = n_head / n_kv): M = n_tree * G rows against every position,
-// so the cache is read once for the whole tree.
+// so the cache is read once for the whole tree. With more than 16 rows (and
+// head_dim <= 128) tree_attention_tc.cu takes the call; here is the kernel for
+// few rows, where the cache's bytes are the bound.
 //
-// tree_attn_kernel: a CTA takes 16 or 32 of the M rows and a run of the
-// context. Its four warps take every fourth step of 16 positions, each with a
-// ring of its own in shared memory (16-byte asynchronous copies, no barrier
-// between the warps), and keep a running maximum, sum and output of their own
-// (one pass over K and V); the warps' results are joined at the end. With few
-// rows the context is split over CTAs so that all SMs read: each CTA leaves
-// (max, sum, output) in the scratch, and tree_join_kernel, which starts early
-// and waits for the first kernel to end, joins them in split order.
+// tree_attn_kernel: a CTA takes up to 16 of the M rows and a part of a
+// sequence's context. Its four warps take every fourth step of 16 positions,
+// each with a ring of its own in shared memory (16-byte asynchronous copies, no
+// barrier between the warps), and keep a running maximum, sum and output of
+// their own (one pass over K and V); the warps' results are joined at the end.
+// The contexts of all sequences are cut into parts of one length, as many as
+// fill the GPU whatever the sequences' own lengths; each CTA leaves (max, sum,
+// output) in the scratch, and the last of a sequence's to be done joins them,
+// in their order. (tree_attention_tc.cu leaves that to tree_join_kernel, which
+// starts early and waits for the first kernel to end: its parts are larger.)
 //
 // Precision: the products run on binary16 tensor-core instructions with float
 // accumulators. q is scaled by a power of two per row and split into two
@@ -21,7 +25,14 @@
 // stored. Quantised caches enter as integers (exact in binary16): a score is
 // the sum over blocks of scale * (q . quants); for V the block's scale is
 // m * 2^e, 2^e <= 2^9 applied to the integers (exact) and m (in [1, 2) for all
-// but extreme scales) to the float probabilities before they are split, so no value is rounded to binary16.
+// but extreme scales) to the float probabilities before they are split, so no
+// value is rounded to binary16. Each step's output is added to float registers
+// outside the tensor core, whose accumulation truncates: kept there over 64
+// steps it cost 2e-6.
+//
+// Up to 8 rows, the usual decode step, the two terms share one product of 16
+// rows: the high terms are rows 0-7, the low ones rows 8-15, and their results
+// are added.
 #include "tree_attention.cuh"
 
 #include <algorithm>
@@ -32,6 +43,7 @@ namespace {
 
 constexpr int kWarps = 4;
 constexpr int kStep = 16;            // positions per step of a warp
+constexpr size_t kCounterBytes = 4096;  // counters of parts that are done, at the start of the scratch
 __device__ __forceinline__ void ldsm4(uint32_t (&r)[4], uint32_t addr) {
     asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
                  : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
@@ -42,7 +54,13 @@ __device__ __forceinline__ void ldsm4t(uint32_t (&r)[4], uint32_t addr) {
                  : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
                  : "r"(addr));
 }
-// C += A B, m16n8k16: lane = 4 g + t holds A[g | g + 8][2t.. | 2t + 8..], B[2t.. | 2t + 8..][g], C[g | g + 8][2t..].
+// C = A B; then C += A B, m16n8k16: lane = 4 g + t holds A[g | g + 8][2t.. | 2t + 8..], B[2t.. | 2t + 8..][g], C[g | g + 8][2t..].
+__device__ __forceinline__ void mma0(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+    asm volatile(
+        "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
+        : "=f"(c[0]), "=f"(c[1]), "=f"(c[2]), "=f"(c[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(0.0f));
+}
 __device__ __forceinline__ void mma(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
     asm volatile(
         "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
@@ -64,42 +82,110 @@ struct Stage {
     static constexpr int bytes = sv_at + scales;
 };
 
-template <int TYPE, int HDP, int MT>
+template <int TYPE, int HDP, bool STACK>
 struct Plan {
     using S = Stage<TYPE, HDP>;
-    static constexpr int R = 16 * MT;                                // rows of a CTA
+    static constexpr bool quant = TYPE != SYN_F16;
+    static constexpr int R = STACK ? 8 : 16;                         // rows of a CTA
+    static constexpr int NR = R / 8;                                 // rows of a lane
     static constexpr int q_pitch = HDP * 2 + 16;
-    static constexpr int q_bytes = 2 * R * q_pitch;                  // hi and lo
-    static constexpr int stages = TYPE == SYN_F16 ? (HDP >= 256 ? 2 : 3) : 4;
-    static constexpr int ring = kWarps * stages * S::bytes;
+    static constexpr int q_bytes = 2 * R * q_pitch;                  // hi, then lo
+    static constexpr int stages = !quant && HDP >= 256 ? 2 : 3;
+    static constexpr int scale_bytes = quant ? kStep * (HDP / 32) * 10 : 0;  // a warp's scales as it uses them
+    static constexpr int warp_bytes = stages * S::bytes + scale_bytes;
+    static constexpr int ring = kWarps * warp_bytes;
     static constexpr int o_pitch = HDP + 4;                          // floats
     static constexpr int join = kWarps * R * (o_pitch + 2) * 4;      // the warps' results, over the ring
     static constexpr int smem = q_bytes + (ring > join ? ring : join) + R * 4;  // + the rows' score factors
+    static constexpr int ctas = (STACK || HDP <= 64) && 3 * (smem + 1024) <= 227 * 1024 ? 3 : 2;  // per SM
 };
 
-template <int TYPE, int HDP, int MT>
-__global__ void __launch_bounds__(kWarps * 32, 2) tree_attn_kernel(const TreeParams a) {
+// N floats (a multiple of 2) from shared memory.
+template <int N>
+__device__ __forceinline__ void load_floats(float (&x)[N], const float* p) {
+#pragma unroll
+    for (int i = 0; i < N; i += N % 4 ? 2 : 4) {
+        if constexpr (N % 4 == 0) {
+            const float4 v = *reinterpret_cast<const float4*>(p + i);
+            x[i] = v.x; x[i + 1] = v.y; x[i + 2] = v.z; x[i + 3] = v.w;
+        } else {
+            const float2 v = *reinterpret_cast<const float2*>(p + i);
+            x[i] = v.x; x[i + 1] = v.y;
+        }
+    }
+}
+
+// Joins a row's parts, in their order, by a warp: row `row` of KV head kvh of sequence seq, whose parts' rows in the
+// scratch are `first`, first + pitch, ...
+__device__ __forceinline__ void join_row(const TreeParams& a, int row, int kvh, int seq, size_t first, size_t pitch, int parts) {
+    const int lane = threadIdx.x & 31, hd = a.c.hd;
+    const float2* ml = a.part_ml + first;
+    const float* o = a.part_o + first * hd;
+    const float2 none = make_float2(-INFINITY, 0.0f);
+    float2 s = lane < parts ? __ldcg(ml + lane * pitch) : none;
+    float top = s.x;
+    for (int x = 32 + lane; x < parts; x += 32) top = fmaxf(top, __ldcg(ml + x * pitch).x);
+    top = warp_max(top);
+    const bool in = 4 * lane < hd, in2 = 128 + 4 * lane < hd;
+    float4 acc = make_float4(0, 0, 0, 0), acc2 = acc;
+    float sum = 0.0f;
+    auto add = [](float4& c, float f, const float4& v) {
+        c.x = fmaf(f, v.x, c.x); c.y = fmaf(f, v.y, c.y); c.z = fmaf(f, v.z, c.z); c.w = fmaf(f, v.w, c.w);
+    };
+    for (int x0 = 0; x0 < parts; x0 += 32) {
+        if (x0) s = x0 + lane < parts ? __ldcg(ml + (x0 + lane) * pitch) : none;
+        const float w = part_weight(s.x, s.y, top);
+        sum += warp_sum(w * s.y);
+        const int n = min(32, parts - x0);
+        auto half = [&](float4& c, int at, bool here) {  // 16 parts' loads at a time
+            for (int i0 = 0; i0 < n; i0 += 16) {
+                float4 v[16];
+#pragma unroll
+                for (int i = 0; i < 16; ++i) {
+                    v[i] = make_float4(0, 0, 0, 0);
+                    if (i0 + i < n && here) v[i] = __ldcg(reinterpret_cast<const float4*>(o + (x0 + i0 + i) * pitch * hd) + at);
+                }
+#pragma unroll
+                for (int i = 0; i < 16; ++i) {
+                    const float f = __shfl_sync(0xffffffffu, w, (i0 + i) & 31);
+                    if (i0 + i < n) add(c, f, v[i]);
+                }
+            }
+        };
+        half(acc, lane, in);
+        if (hd > 128) half(acc2, 32 + lane, in2);
+    }
+    const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
+    const int tk = row / a.group, h = kvh * a.group + row - tk * a.group;
+    float4* out = reinterpret_cast<float4*>(a.out + ((size_t(seq) * a.n_tree + tk) * a.n_head + h) * hd);
+    if (in) out[lane] = make_float4(acc.x * inv, acc.y * inv, acc.z * inv, acc.w * inv);
+    if (in2) out[32 + lane] = make_float4(acc2.x * inv, acc2.y * inv, acc2.z * inv, acc2.w * inv);
+}
+
+template <int TYPE, int HDP, bool STACK>
+__global__ void __launch_bounds__(kWarps * 32, Plan<TYPE, HDP, STACK>::ctas) tree_attn_kernel(const TreeParams a) {
     using S = Stage<TYPE, HDP>;
-    using P = Plan<TYPE, HDP, MT>;
-    constexpr int R = P::R, KS = HDP / 16, NB = HDP / 32;
-    constexpr bool kQuant = TYPE != SYN_F16;
-    constexpr bool kQReg = MT == 1 && HDP <= 128;
+    using P = Plan<TYPE, HDP, STACK>;
+    constexpr int R = P::R, NR = P::NR, KS = HDP / 16, NB = HDP / 32;
+    constexpr bool kQuant = P::quant;
+    constexpr bool kQReg = HDP <= 128;  // the q fragments stay in registers
+    constexpr int QT = STACK ? 1 : 2;   // q fragments of a k step: both terms, or one each
     extern __shared__ __align__(128) unsigned char smem[];
     unsigned char* ring = smem + P::q_bytes;
     float* row_scale = reinterpret_cast<float*>(smem + P::smem - R * 4);
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
     const int hd = a.c.hd;
-    const int kvh = blockIdx.y / a.row_blocks, rb = blockIdx.y - kvh * a.row_blocks, seq = blockIdx.z;
+    const int kvh = blockIdx.y / a.row_blocks, rb = blockIdx.y - kvh * a.row_blocks;
     const int row0 = rb * R, rows = min(R, a.rows - row0);
 
     pdl_launch_dependents();
     pdl_wait();
-    const int len = min(max(a.len[seq], 0), a.max_len - a.n_tree);
-    const int total = len + a.n_tree;
+    int seq = -1;
+    const Cutting cut = tree_cutting(a, kStep, blockIdx.x, seq);
+    if (seq < 0) return;
+    const int len = tree_len(a, seq), total = len + a.n_tree;
     const int steps = (total + kStep - 1) / kStep;
-    const int per = (steps + a.splits - 1) / a.splits;
-    const int s0 = blockIdx.x * per, s1 = min(s0 + per, steps);
-    if (s0 >= steps) return;
+    const int s0 = (int(blockIdx.x) - cut.first) * cut.per, s1 = cut.per < steps - s0 ? s0 + cut.per : steps;
 
     // --- the ring -------------------------------------------------------------
     const int nb = hd / 32;  // blocks of a row (quantised)
@@ -110,21 +196,32 @@ __global__ void __launch_bounds__(kWarps * 32, 2) tree_attn_kernel(const TreePar
     const size_t head_at = TYPE == SYN_F16 ? size_t(kvh) * hd * 2 : size_t(kvh) * a.c.max_ctx * row_bytes;
     const size_t scale_at = a.c.scale_plane + size_t(kvh) * a.c.max_ctx * nb * 2;
     const int scale_off = kQuant ? int(scale_at & 15) : 0;  // the same for every step: 16 positions are 32 nb bytes
-    unsigned char* my_ring = ring + warp * P::stages * S::bytes;
+    unsigned char* my_ring = ring + warp * P::warp_bytes;
     const uint32_t ring_s = smem_addr(my_ring);
+    const int chunks = row_bytes / 16;
+    constexpr int CP = S::row / 16;  // chunks of a full row
+    const size_t lane_at = head_at + size_t(lane / CP) * pos_pitch + (lane % CP) * 16;
+    const uint32_t lane_k = (lane / CP) * S::k_pitch + (lane % CP) * 16, lane_v = S::v_at + (lane / CP) * S::v_pitch + (lane % CP) * 16;
     auto load = [&](int step, int stage) {
         const uint32_t st = ring_s + stage * S::bytes;
         const int p0 = step * kStep;
-        const int chunks = row_bytes / 16;
-        constexpr int CP = S::row / 16;  // chunks of a full row
+        constexpr int rows_at_once = 32 / CP;
+        const char *kp = kbase + lane_at + size_t(p0) * pos_pitch, *vp = vbase + lane_at + size_t(p0) * pos_pitch;
+        if (hd == HDP && p0 + kStep <= total) {
 #pragma unroll
-        for (int i = 0; i < kStep * CP / 32; ++i) {
-            const int r = (i * 32 + lane) / CP, c = (i * 32 + lane) % CP;
-            const bool in = p0 + r < total;
-            const size_t at = head_at + size_t(in ? p0 + r : 0) * pos_pitch + c * 16;
-            if (c < chunks) {
-                cp16(st + r * S::k_pitch + c * 16, kbase + at, in);
-                cp16(st + S::v_at + r * S::v_pitch + c * 16, vbase + at, in);
+            for (int i = 0; i < kStep / rows_at_once; ++i) {
+                cp16(st + lane_k + i * rows_at_once * S::k_pitch, kp + i * rows_at_once * pos_pitch);
+                cp16(st + lane_v + i * rows_at_once * S::v_pitch, vp + i * rows_at_once * pos_pitch);
+            }
+        } else {
+#pragma unroll
+            for (int i = 0; i < kStep / rows_at_once; ++i) {
+                const bool in = p0 + i * rows_at_once + lane / CP < total;
+                const size_t at = in ? size_t(i) * rows_at_once * pos_pitch : 0;
+                if (lane % CP < chunks) {
+                    cp16(st + lane_k + i * rows_at_once * S::k_pitch, in ? kp + at : kbase, in);
+                    cp16(st + lane_v + i * rows_at_once * S::v_pitch, in ? vp + at : vbase, in);
+                }
             }
         }
         if (kQuant) {
@@ -134,11 +231,21 @@ __global__ void __launch_bounds__(kWarps * 32, 2) tree_attn_kernel(const TreePar
             const int n = (scale_off + (last - p0) * nb * 2 + 15) / 16;
             constexpr int most = S::scales / 16;
             const int which = lane / 16, c = lane % 16;
-            if (c < n) cp16(st + (which ? S::sv_at : S::sk_at) + c * 16, (which ? vbase : kbase) + at + c * 16, true);
-            if (most > 16 && c + 16 < n)
-                cp16(st + (which ? S::sv_at : S::sk_at) + (c + 16) * 16, (which ? vbase : kbase) + at + (c + 16) * 16, true);
+            const char* from = (which ? vbase : kbase) + at + c * 16;
+            const uint32_t to = st + (which ? S::sv_at : S::sk_at) + c * 16;
+            if (c < n) cp16(to, from);
+            if (most > 16 && c + 16 < n) cp16(to + 256, from + 256);
         }
     };
+    // q's rows are on their way before the tiles are
+    float qx[R / kWarps][NB];
+#pragma unroll
+    for (int i = 0; i < R / kWarps; ++i) {
+        const int r = i * kWarps + warp, row = row0 + r, qt = row / a.group, h = row - qt * a.group;
+        const float* src = a.q + (size_t(seq) * a.n_tree + qt) * a.q_stride + size_t(kvh * a.group + h) * hd + lane;
+#pragma unroll
+        for (int b = 0; b < NB; ++b) qx[i][b] = r < rows && 32 * b + lane < hd ? __ldg(src + 32 * b) : 0.0f;
+    }
     if (hd != HDP) {  // dims past the head stay zero
         for (int i = tid; i < P::ring / 16; i += kWarps * 32) reinterpret_cast<uint4*>(ring)[i] = make_uint4(0, 0, 0, 0);
         __syncthreads();
@@ -152,20 +259,15 @@ __global__ void __launch_bounds__(kWarps * 32, 2) tree_attn_kernel(const TreePar
     }
 
     // --- q: scaled to a row maximum in [2^8, 2^9), split, in the order of the K fragments -------
-    for (int r = warp; r < R; r += kWarps) {
-        const int row = row0 + r, tok = row / a.group, h = row - tok * a.group;
-        const bool in = r < rows;
-        const float* src = a.q + (size_t(seq) * a.n_tree + (in ? tok : 0)) * a.q_stride + size_t(kvh * a.group + (in ? h : 0)) * hd;
-        float x[NB], m = 0.0f;
 #pragma unroll
-        for (int b = 0; b < NB; ++b) {
-            const int d = 32 * b + lane;
-            x[b] = in && d < hd ? src[d] : 0.0f;
-            m = fmaxf(m, fabsf(x[b]));
-        }
-        m = warp_max(m);
+    for (int i = 0; i < R / kWarps; ++i) {
+        const int r = i * kWarps + warp;
+        float(&x)[NB] = qx[i];
+        float m = 0.0f;
+#pragma unroll
+        for (int b = 0; b < NB; ++b) m = fmaxf(m, fabsf(x[b]));
         float up, down;
-        q_factor(m, up, down);
+        q_factor(warp_max(m), up, down);
         if (lane == 0) row_scale[r] = a.scale_log2 * down;
 #pragma unroll
         for (int b = 0; b < NB; ++b) {
@@ -187,31 +289,27 @@ __global__ void __launch_bounds__(kWarps * 32, 2) tree_attn_kernel(const TreePar
     }
     __syncthreads();
 
+    // fragments of 16 rows: all high terms (with the low ones 16 rows on), or 8 high and 8 low
     const uint32_t q_s = smem_addr(smem) + (lane & 15) * P::q_pitch + (lane >> 4) * 16;
-    uint32_t qh[kQReg ? KS : 1][4], ql[kQReg ? KS : 1][4];
-    if (kQReg) {
+    uint32_t qf[kQReg ? KS : 1][QT][4];
+    if (kQReg)
 #pragma unroll
-        for (int k = 0; k < KS; ++k) {
-            ldsm4(qh[k], q_s + k * 32);
-            ldsm4(ql[k], q_s + R * P::q_pitch + k * 32);
-        }
+        for (int k = 0; k < KS; ++k)
+#pragma unroll
+            for (int x = 0; x < QT; ++x) ldsm4(qf[k][x], q_s + x * 16 * P::q_pitch + k * 32);
+    float rs[NR], m[NR], l[NR], o[HDP / 8][2 * NR];
+    int tok[NR];
+#pragma unroll
+    for (int u = 0; u < NR; ++u) {
+        rs[u] = row_scale[8 * u + g];
+        tok[u] = (row0 + 8 * u + g) / a.group;
+        m[u] = -INFINITY;
+        l[u] = 0.0f;
     }
-    float rs[MT][2], m[MT][2], l[MT][2], o[MT][HDP / 8][4];
-    int tok[MT][2];
 #pragma unroll
-    for (int i = 0; i < MT; ++i) {
+    for (int n = 0; n < HDP / 8; ++n)
 #pragma unroll
-        for (int u = 0; u < 2; ++u) {
-            rs[i][u] = row_scale[16 * i + 8 * u + g];
-            tok[i][u] = (row0 + 16 * i + 8 * u + g) / a.group;
-            m[i][u] = -INFINITY;
-            l[i][u] = 0.0f;
-        }
-#pragma unroll
-        for (int n = 0; n < HDP / 8; ++n)
-#pragma unroll
-            for (int e = 0; e < 4; ++e) o[i][n][e] = 0.0f;
-    }
+        for (int e = 0; e < 2 * NR; ++e) o[n][e] = 0.0f;
 
     // --- the steps of this warp ----------------------------------------------------
     int stage = 0;
@@ -229,67 +327,64 @@ __global__ void __launch_bounds__(kWarps * 32, 2) tree_attn_kernel(const TreePar
         const uint32_t st_s = ring_s + stage * S::bytes;
         const int p0 = step * kStep;
 
-        // scores of 16 positions: n-tile u holds positions p0 + 8 u + {2t, 2t + 1}
-        float s[MT][2][4];
+        // this step's scales as the lanes use them: K's, and V's as m (float) and 2^e (binary16)
+        float* kds = reinterpret_cast<float*>(my_ring + P::stages * S::bytes);  // [16][NB]
+        float* vms = kds + kStep * NB;                                          // [16][NB]
+        uint16_t* ves = reinterpret_cast<uint16_t*>(vms + kStep * NB);          // [8 pairs][NB][2]
+        if constexpr (kQuant) {
 #pragma unroll
-        for (int i = 0; i < MT; ++i)
+            for (int i = 0; i < kStep * NB / 32; ++i) {
+                const int id = i * 32 + lane, r = id / NB, b = id % NB;
+                // a position past the context has scales of 0; one whose V scale is not finite scores NaN (rows
+                // that do not see it mask that)
+                const bool ok = p0 + r < total && b < nb;
+                const uint32_t dk = ok ? reinterpret_cast<const uint16_t*>(st + S::sk_at + scale_off)[r * nb + b] : 0u;
+                const uint32_t dv = ok ? reinterpret_cast<const uint16_t*>(st + S::sv_at + scale_off)[r * nb + b] : 0u;
+                const bool finite = (dv & 0x7c00u) != 0x7c00u;
+                const uint32_t pow = finite ? min(max(dv & 0x7c00u, 0x0400u), 0x6000u) : 0x0400u;  // 2^-14 .. 2^9: 127 * 2^9 is finite
+                const float inv = __uint_as_float(0x7f000000u - __float_as_uint(f16_from_bits(uint16_t(pow))));
+                kds[id] = finite ? f16_from_bits(uint16_t(dk)) : __uint_as_float(0x7fffffffu);
+                vms[id] = finite ? f16_from_bits(uint16_t(dv)) * inv : 0.0f;
+                ves[((r >> 1) * NB + b) * 2 + (r & 1)] = uint16_t(pow);
+            }
+            __syncwarp();
+        }
+
+        // scores of 16 positions: n-tile u holds positions p0 + 8 u + {2t, 2t + 1}, for NR rows each
+        float s[2][2 * NR];
+        auto products = [&](float (&c)[2][4], int k, const uint32_t (&b)[2][2], bool first) {
+            uint32_t f[QT][4];
+            if (!kQReg)
+#pragma unroll
+                for (int x = 0; x < QT; ++x) ldsm4(f[x], q_s + x * 16 * P::q_pitch + k * 32);
+#pragma unroll
+            for (int x = 0; x < QT; ++x)
+#pragma unroll
+                for (int u = 0; u < 2; ++u) {
+                    if (first && x == 0) mma0(c[u], kQReg ? qf[kQReg ? k : 0][x] : f[x], b[u][0], b[u][1]);
+                    else mma(c[u], kQReg ? qf[kQReg ? k : 0][x] : f[x], b[u][0], b[u][1]);
+                }
+        };
+        if constexpr (!kQuant) {
+            float c[2][4];
+#pragma unroll
+            for (int k = 0; k < KS; ++k) {
+                uint32_t x[4];  // (n-tile 0: b0, b1), (n-tile 1: b0, b1)
+                ldsm4(x, st_s + ((lane & 7) + ((lane >> 4) << 3)) * S::k_pitch + k * 32 + ((lane >> 3) & 1) * 16);
+                const uint32_t b[2][2] = {{x[0], x[1]}, {x[2], x[3]}};
+                products(c, k, b, k == 0);
+            }
 #pragma unroll
             for (int u = 0; u < 2; ++u)
 #pragma unroll
-                for (int e = 0; e < 4; ++e) s[i][u][e] = 0.0f;
-        float vm[kQuant ? NB : 1][4];   // V scales' mantissas of positions 2t, 2t + 1, 2t + 8, 2t + 9
-        uint32_t ve[kQuant ? NB : 1][2];  // and their powers of two, as binary16 pairs
-        if constexpr (!kQuant) {
-#pragma unroll
-            for (int k = 0; k < KS; ++k) {
-                uint32_t b[4];  // (n-tile 0: b0, b1), (n-tile 1: b0, b1)
-                ldsm4(b, st_s + ((lane & 7) + ((lane >> 4) << 3)) * S::k_pitch + k * 32 + ((lane >> 3) & 1) * 16);
-#pragma unroll
-                for (int i = 0; i < MT; ++i) {
-                    uint32_t ah[4], al[4];
-                    if (!kQReg) {
-                        ldsm4(ah, q_s + 16 * i * P::q_pitch + k * 32);
-                        ldsm4(al, q_s + (R + 16 * i) * P::q_pitch + k * 32);
-                    }
-                    mma(s[i][0], kQReg ? qh[kQReg ? k : 0] : ah, b[0], b[1]);
-                    mma(s[i][1], kQReg ? qh[kQReg ? k : 0] : ah, b[2], b[3]);
-                    mma(s[i][0], kQReg ? ql[kQReg ? k : 0] : al, b[0], b[1]);
-                    mma(s[i][1], kQReg ? ql[kQReg ? k : 0] : al, b[2], b[3]);
-                }
-            }
+                for (int e = 0; e < 2 * NR; ++e) s[u][e] = STACK ? c[u][e] + c[u][e + 2] : c[u][e];
         } else {
-            // the scales of this lane's positions; a position past the context has scales of 0, one whose
-            // V scale is not finite scores NaN (rows that do not see it mask that)
-            float kd[NB][4];
+            float kd[4][NB];  // of positions 2t, 2t + 1, 2t + 8, 2t + 9
 #pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                const int r = 2 * t + (j & 1) + 8 * (j >> 1);
-                const bool in = p0 + r < total;
-                const uint16_t* sk = reinterpret_cast<const uint16_t*>(st + S::sk_at + scale_off) + r * nb;
-                const uint16_t* sv = reinterpret_cast<const uint16_t*>(st + S::sv_at + scale_off) + r * nb;
-#pragma unroll
-                for (int b = 0; b < NB; ++b) {
-                    const bool ok = in && b < nb;
-                    const uint32_t dk = ok ? sk[b] : 0u, dv = ok ? sv[b] : 0u;
-                    kd[b][j] = f16_from_bits(uint16_t(dk));
-                    const bool finite = (dv & 0x7c00u) != 0x7c00u;
-                    if (!finite) kd[b][j] = __uint_as_float(0x7fffffffu);
-                    const uint32_t pow = min(max(dv & 0x7c00u, 0x0400u), 0x6000u);  // 2^-14 .. 2^9: 127 * 2^9 is finite
-                    const float inv = __uint_as_float(0x7f000000u - __float_as_uint(f16_from_bits(uint16_t(pow))));
-                    vm[b][j] = finite ? f16_from_bits(uint16_t(dv)) * inv : 0.0f;
-                    const uint32_t p = finite ? pow : 0x0400u;
-                    ve[b][j >> 1] = (j & 1) ? (ve[b][j >> 1] | p << 16) : p;
-                }
-            }
+            for (int j = 0; j < 4; ++j) load_floats(kd[j], kds + (2 * t + (j & 1) + 8 * (j >> 1)) * NB);
 #pragma unroll
             for (int b = 0; b < NB; ++b) {
-                float c[MT][2][4];
-#pragma unroll
-                for (int i = 0; i < MT; ++i)
-#pragma unroll
-                    for (int u = 0; u < 2; ++u)
-#pragma unroll
-                        for (int e = 0; e < 4; ++e) c[i][u][e] = 0.0f;
+                float c[2][4];
                 uint32_t w[2][2];  // [n-tile][product of 16 dims]: four quants as bytes
 #pragma unroll
                 for (int u = 0; u < 2; ++u) {
@@ -313,26 +408,15 @@ __global__ void __launch_bounds__(kWarps * 32, 2) tree_attn_kernel(const TreePar
                         bb[u][0] = bits(__hsub2(bytes_h2(w[u][h], 0x4140), zero));
                         bb[u][1] = bits(__hsub2(bytes_h2(w[u][h], 0x4342), zero));
                     }
-#pragma unroll
-                    for (int i = 0; i < MT; ++i) {
-                        const int k = 2 * b + h;
-                        uint32_t ah[4], al[4];
-                        if (!kQReg) {
-                            ldsm4(ah, q_s + 16 * i * P::q_pitch + k * 32);
-                            ldsm4(al, q_s + (R + 16 * i) * P::q_pitch + k * 32);
-                        }
-                        mma(c[i][0], kQReg ? qh[kQReg ? k : 0] : ah, bb[0][0], bb[0][1]);
-                        mma(c[i][1], kQReg ? qh[kQReg ? k : 0] : ah, bb[1][0], bb[1][1]);
-                        mma(c[i][0], kQReg ? ql[kQReg ? k : 0] : al, bb[0][0], bb[0][1]);
-                        mma(c[i][1], kQReg ? ql[kQReg ? k : 0] : al, bb[1][0], bb[1][1]);
-                    }
+                    products(c, 2 * b + h, bb, h == 0);
                 }
 #pragma unroll
-                for (int i = 0; i < MT; ++i)
+                for (int u = 0; u < 2; ++u)
 #pragma unroll
-                    for (int u = 0; u < 2; ++u)
-#pragma unroll
-                        for (int e = 0; e < 4; ++e) s[i][u][e] = fmaf(c[i][u][e], kd[b][2 * u + (e & 1)], s[i][u][e]);
+                    for (int e = 0; e < 2 * NR; ++e) {
+                        const float x = STACK ? c[u][e] + c[u][e + 2] : c[u][e], d = kd[2 * u + (e & 1)][b];
+                        s[u][e] = b == 0 ? x * d : fmaf(x, d, s[u][e]);
+                    }
             }
         }
 
@@ -358,92 +442,95 @@ __global__ void __launch_bounds__(kWarps * 32, 2) tree_attn_kernel(const TreePar
             flags = (flags | flags >> 16) & 0xffffu;
             __syncwarp();
 #pragma unroll
-            for (int i = 0; i < MT; ++i)
+            for (int u = 0; u < 2; ++u)
 #pragma unroll
-                for (int u = 0; u < 2; ++u)
-#pragma unroll
-                    for (int e = 0; e < 4; ++e)
-                        if (flags >> (8 * u + 2 * t + (e & 1)) & 1u) s[i][u][e] = __uint_as_float(0x7fffffffu);
+                for (int e = 0; e < 2 * NR; ++e)
+                    if (flags >> (8 * u + 2 * t + (e & 1)) & 1u) s[u][e] = __uint_as_float(0x7fffffffu);
         }
 #pragma unroll
-        for (int i = 0; i < MT; ++i)
+        for (int u = 0; u < 2; ++u)
+#pragma unroll
+            for (int e = 0; e < 2 * NR; ++e) s[u][e] *= rs[e >> 1];
+        if (edge) {
 #pragma unroll
             for (int u = 0; u < 2; ++u)
 #pragma unroll
-                for (int e = 0; e < 4; ++e) s[i][u][e] *= rs[i][e >> 1];
-        if (edge) {
-#pragma unroll
-            for (int i = 0; i < MT; ++i)
-#pragma unroll
-                for (int u = 0; u < 2; ++u)
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) {
-                        const int j = p0 + 8 * u + 2 * t + (e & 1) - len;
-                        const bool sees = j < 0 || tree_sees(a, seq, tok[i][e >> 1], j);
-                        if (!sees) s[i][u][e] = -INFINITY;
-                    }
+                for (int e = 0; e < 2 * NR; ++e) {
+                    const int j = p0 + 8 * u + 2 * t + (e & 1) - len;
+                    const bool sees = j < 0 || tree_sees(a, seq, tok[e >> 1], j);
+                    if (!sees) s[u][e] = -INFINITY;
+                }
         }
 
         // running maximum, probabilities, sum
-        uint32_t ph[MT][4], pl[MT][4];
-        float p[MT][2][4];
+        float p[2][2 * NR], mn[NR];
+        bool grows = false;
 #pragma unroll
-        for (int i = 0; i < MT; ++i) {
-            bool grows = false;
-            float mn[2];
+        for (int u = 0; u < NR; ++u) {
+            float x = fmaxf(fmaxf(s[0][2 * u], s[0][2 * u + 1]), fmaxf(s[1][2 * u], s[1][2 * u + 1]));
+            x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 1));
+            x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 2));
+            mn[u] = fmaxf(m[u], x);
+            grows |= mn[u] > m[u];
+        }
+        if (__any_sync(0xffffffffu, grows)) {
+            float f[NR];
+#pragma unroll
+            for (int u = 0; u < NR; ++u) {
+                f[u] = mn[u] > m[u] ? ex2(m[u] - mn[u]) : 1.0f;  // m = -inf: 0
+                m[u] = mn[u];
+                l[u] *= f[u];
+            }
+#pragma unroll
+            for (int n = 0; n < HDP / 8; ++n)
+#pragma unroll
+                for (int e = 0; e < 2 * NR; ++e) o[n][e] *= f[e >> 1];
+        }
+#pragma unroll
+        for (int u = 0; u < 2; ++u)
+#pragma unroll
+            for (int e = 0; e < 2 * NR; ++e) {
+                const float mm = m[e >> 1];
+                p[u][e] = ex2(s[u][e] - (mm == -INFINITY ? 0.0f : mm) + kPShift);
+                l[e >> 1] += p[u][e];
+            }
+
+        // out += p V: the A fragments of the probabilities times four factors (one for each position of a lane)
+        uint32_t pf[QT][4];
+        auto split_p = [&](const float (&f)[4]) {
 #pragma unroll
             for (int u = 0; u < 2; ++u) {
-                float x = fmaxf(fmaxf(s[i][0][2 * u], s[i][0][2 * u + 1]), fmaxf(s[i][1][2 * u], s[i][1][2 * u + 1]));
-                x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 1));
-                x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 2));
-                mn[u] = fmaxf(m[i][u], x);
-                grows |= mn[u] > m[i][u];
-            }
-            if (__any_sync(0xffffffffu, grows)) {
-                float f[2];
-#pragma unroll
-                for (int u = 0; u < 2; ++u) {
-                    f[u] = mn[u] > m[i][u] ? ex2(m[i][u] - mn[u]) : 1.0f;  // m = -inf: 0
-                    m[i][u] = mn[u];
-                    l[i][u] *= f[u];
+                if (STACK) {
+                    split2(p[u][0] * f[2 * u], p[u][1] * f[2 * u + 1], pf[0][2 * u], pf[0][2 * u + 1]);
+                } else {
+                    split2(p[u][0] * f[2 * u], p[u][1] * f[2 * u + 1], pf[0][2 * u], pf[QT - 1][2 * u]);
+                    split2(p[u][2 * NR - 2] * f[2 * u], p[u][2 * NR - 1] * f[2 * u + 1], pf[0][2 * u + 1], pf[QT - 1][2 * u + 1]);
                 }
-#pragma unroll
-                for (int n = 0; n < HDP / 8; ++n)
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) o[i][n][e] *= f[e >> 1];
             }
+        };
+        auto output = [&](float (&acc)[2 * NR], uint32_t b0, uint32_t b1) {
+            float c[4];
+            mma0(c, pf[0], b0, b1);
+            if (!STACK) mma(c, pf[QT - 1], b0, b1);
 #pragma unroll
-            for (int u = 0; u < 2; ++u)
-#pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    const float mm = m[i][e >> 1];
-                    p[i][u][e] = ex2(s[i][u][e] - (mm == -INFINITY ? 0.0f : mm) + kPShift);
-                    l[i][e >> 1] += p[i][u][e];
-                }
-        }
-
-        // out += p V
+            for (int e = 0; e < 2 * NR; ++e) acc[e] += STACK ? c[e] + c[e + 2] : c[e];
+        };
         if constexpr (!kQuant) {
-#pragma unroll
-            for (int i = 0; i < MT; ++i)
-#pragma unroll
-                for (int u = 0; u < 2; ++u) {
-                    split2(p[i][u][0], p[i][u][1], ph[i][2 * u], pl[i][2 * u]);
-                    split2(p[i][u][2], p[i][u][3], ph[i][2 * u + 1], pl[i][2 * u + 1]);
-                }
+            split_p({1.0f, 1.0f, 1.0f, 1.0f});
 #pragma unroll
             for (int n = 0; n < HDP / 16; ++n) {
                 uint32_t b[4];
                 ldsm4t(b, st_s + S::v_at + ((lane & 7) + ((lane >> 3) & 1) * 8) * S::v_pitch + n * 32 + (lane >> 4) * 16);
-#pragma unroll
-                for (int i = 0; i < MT; ++i) {
-                    mma(o[i][2 * n], ph[i], b[0], b[1]);
-                    mma(o[i][2 * n + 1], ph[i], b[2], b[3]);
-                    mma(o[i][2 * n], pl[i], b[0], b[1]);
-                    mma(o[i][2 * n + 1], pl[i], b[2], b[3]);
-                }
+                output(o[2 * n], b[0], b[1]);
+                output(o[2 * n + 1], b[2], b[3]);
             }
         } else {
+            float vm[4][NB];
+#pragma unroll
+            for (int j = 0; j < 4; ++j) load_floats(vm[j], vms + (2 * t + (j & 1) + 8 * (j >> 1)) * NB);
+            float ve[2][NB];  // binary16 pairs of positions 2t, 2t + 1 | 2t + 8, 2t + 9
+#pragma unroll
+            for (int j = 0; j < 2; ++j) load_floats(ve[j], reinterpret_cast<const float*>(ves) + (t + 4 * j) * NB);
             uint32_t r4[4];  // a block's bytes of 2 positions x 2 dims: (positions 0-7, 8-15) x (dims 0-15, 16-31)
 #pragma unroll
             for (int b = 0; b < NB; ++b) {
@@ -451,15 +538,9 @@ __global__ void __launch_bounds__(kWarps * 32, 2) tree_attn_kernel(const TreePar
                     ldsm4t(r4, st_s + S::v_at + ((lane & 7) + ((lane >> 3) & 1) * 8) * S::v_pitch + b * 32 + (lane >> 4) * 16);
                 else if ((b & 1) == 0)  // two blocks of 16 bytes
                     ldsm4t(r4, st_s + S::v_at + ((lane & 7) + ((lane >> 3) & 1) * 8) * S::v_pitch + b * 16 + (lane >> 4) * 16);
-#pragma unroll
-                for (int i = 0; i < MT; ++i)
-#pragma unroll
-                    for (int u = 0; u < 2; ++u) {
-                        split2(p[i][u][0] * vm[b][2 * u], p[i][u][1] * vm[b][2 * u + 1], ph[i][2 * u], pl[i][2 * u]);
-                        split2(p[i][u][2] * vm[b][2 * u], p[i][u][3] * vm[b][2 * u + 1], ph[i][2 * u + 1], pl[i][2 * u + 1]);
-                    }
+                split_p({vm[0][b], vm[1][b], vm[2][b], vm[3][b]});
                 const __half2 zero = half2_of(TYPE == SYN_Q8_0 ? 0x64806480u : 0x64086408u);
-                const __half2 e0 = half2_of(ve[b][0]), e1 = half2_of(ve[b][1]);
+                const __half2 e0 = half2_of(__float_as_uint(ve[0][b])), e1 = half2_of(__float_as_uint(ve[1][b]));
                 // n-tile 4 b + 2 half + odd: dims 32 b + 16 half + 2 n + odd
 #pragma unroll
                 for (int half = 0; half < 2; ++half) {
@@ -474,17 +555,13 @@ __global__ void __launch_bounds__(kWarps * 32, 2) tree_attn_kernel(const TreePar
 #pragma unroll
                     for (int odd = 0; odd < 2; ++odd) {
                         const uint32_t sel = odd ? 0x4341u : 0x4240u;
-                        const uint32_t b0 = bits(__hmul2(__hsub2(bytes_h2(x0, sel), zero), e0));
-                        const uint32_t b1 = bits(__hmul2(__hsub2(bytes_h2(x1, sel), zero), e1));
-#pragma unroll
-                        for (int i = 0; i < MT; ++i) {
-                            mma(o[i][4 * b + 2 * half + odd], ph[i], b0, b1);
-                            mma(o[i][4 * b + 2 * half + odd], pl[i], b0, b1);
-                        }
+                        output(o[4 * b + 2 * half + odd], bits(__hmul2(__hsub2(bytes_h2(x0, sel), zero), e0)),
+                               bits(__hmul2(__hsub2(bytes_h2(x1, sel), zero), e1)));
                     }
                 }
             }
         }
+        __syncwarp();
         if (++stage == P::stages) stage = 0;
     }
     cp_wait<0>();
@@ -495,31 +572,29 @@ __global__ void __launch_bounds__(kWarps * 32, 2) tree_attn_kernel(const TreePar
     float* jm = jo + kWarps * R * P::o_pitch;          // [kWarps][R]
     float* jl = jm + kWarps * R;
 #pragma unroll
-    for (int i = 0; i < MT; ++i)
-#pragma unroll
-        for (int u = 0; u < 2; ++u) {
-            float sum = l[i][u];
-            sum += __shfl_xor_sync(0xffffffffu, sum, 1);
-            sum += __shfl_xor_sync(0xffffffffu, sum, 2);
-            const int r = 16 * i + 8 * u + g;
-            if (t == 0) {
-                jm[warp * R + r] = m[i][u];
-                jl[warp * R + r] = sum;
-            }
-            float* at = jo + (warp * R + r) * P::o_pitch;
-            if constexpr (!kQuant) {
-#pragma unroll
-                for (int n = 0; n < HDP / 8; ++n)
-                    *reinterpret_cast<float2*>(at + 8 * n + 2 * t) = make_float2(o[i][n][2 * u], o[i][n][2 * u + 1]);
-            } else {
-#pragma unroll
-                for (int n = 0; n < HDP / 16; ++n)  // (even, odd) n-tiles hold dims 4t, 4t + 2 and 4t + 1, 4t + 3
-                    *reinterpret_cast<float4*>(at + 16 * n + 4 * t) =
-                        make_float4(o[i][2 * n][2 * u], o[i][2 * n + 1][2 * u], o[i][2 * n][2 * u + 1], o[i][2 * n + 1][2 * u + 1]);
-            }
+    for (int u = 0; u < NR; ++u) {
+        float sum = l[u];
+        sum += __shfl_xor_sync(0xffffffffu, sum, 1);
+        sum += __shfl_xor_sync(0xffffffffu, sum, 2);
+        const int r = 8 * u + g;
+        if (t == 0) {
+            jm[warp * R + r] = m[u];
+            jl[warp * R + r] = sum;
         }
+        float* at = jo + (warp * R + r) * P::o_pitch;
+        if constexpr (!kQuant) {
+#pragma unroll
+            for (int n = 0; n < HDP / 8; ++n)
+                *reinterpret_cast<float2*>(at + 8 * n + 2 * t) = make_float2(o[n][2 * u], o[n][2 * u + 1]);
+        } else {
+#pragma unroll
+            for (int n = 0; n < HDP / 16; ++n)  // (even, odd) n-tiles hold dims 4t, 4t + 2 and 4t + 1, 4t + 3
+                *reinterpret_cast<float4*>(at + 16 * n + 4 * t) =
+                    make_float4(o[2 * n][2 * u], o[2 * n + 1][2 * u], o[2 * n][2 * u + 1], o[2 * n + 1][2 * u + 1]);
+        }
+    }
     __syncthreads();
-    const size_t part = ((size_t(seq) * gridDim.y + blockIdx.y) * a.splits + blockIdx.x) * R;
+    const size_t part = (size_t(blockIdx.x) * gridDim.y + blockIdx.y) * R;
     for (int r = warp; r < rows; r += kWarps) {
         float mx = -INFINITY;
 #pragma unroll
@@ -542,84 +617,58 @@ __global__ void __launch_bounds__(kWarps * 32, 2) tree_attn_kernel(const TreePar
         }
         if (!whole && lane == 0) a.part_ml[part + r] = make_float2(mx, sum);
     }
+    if (a.splits == 1) return;
+
+    // --- the last of the sequence's parts to be done joins them ----------------------------
+    __threadfence();
+    __syncthreads();
+    __shared__ bool last;
+    if (tid == 0) {
+        unsigned* arrived = a.arrived + size_t(seq) * gridDim.y + blockIdx.y;
+        last = atomicAdd(arrived, 1u) == unsigned(cut.parts - 1);
+        if (last) *arrived = 0;  // ready for the next call
+        __threadfence();
+    }
+    __syncthreads();
+    if (!last) return;
+    const size_t first = (size_t(cut.first) * gridDim.y + blockIdx.y) * R;
+    for (int r = warp; r < rows; r += kWarps) join_row(a, row0 + r, kvh, seq, first + r, size_t(gridDim.y) * R, cut.parts);
 }
 
-// Joins a call's splits, in their order: a warp per row (token, head).
+// Joins the sequences' parts: a warp per row (token, head).
 __global__ void __launch_bounds__(128) tree_join_kernel(const TreeParams a, int R, int step) {
     pdl_wait();
-    const int lane = threadIdx.x & 31, hd = a.c.hd;
-    const size_t id = size_t(blockIdx.x) * 4 + (threadIdx.x >> 5);  // row of all rows
-    if (id >= size_t(a.c.n_seq) * a.c.n_kv * a.rows) return;
-    const int row = int(id % a.rows), kvh = int(id / a.rows % a.c.n_kv), seq = int(id / a.rows / a.c.n_kv);
-    const int rb = row / R, r = row - rb * R;
-    // the splits that had steps
-    const int len = min(max(a.len[seq], 0), a.max_len - a.n_tree);
-    const int steps = (len + a.n_tree + step - 1) / step, per = (steps + a.splits - 1) / a.splits;
-    const int active = (steps + per - 1) / per;
-    const size_t first = (size_t(seq) * a.c.n_kv + kvh) * a.row_blocks + rb;
-    const float2* ml = a.part_ml + first * a.splits * R + r;
-    const float* o = a.part_o + (first * a.splits * R + r) * hd;
-    float top = -INFINITY;
-    for (int x = lane; x < active; x += 32) top = fmaxf(top, __ldcg(ml + size_t(x) * R).x);
-    top = warp_max(top);
-    const bool in = 4 * lane < hd, in2 = 128 + 4 * lane < hd;
-    float4 acc = make_float4(0, 0, 0, 0), acc2 = acc;
-    float sum = 0.0f;
-    auto add = [](float4& c, float f, const float4& v) {
-        c.x = fmaf(f, v.x, c.x); c.y = fmaf(f, v.y, c.y); c.z = fmaf(f, v.z, c.z); c.w = fmaf(f, v.w, c.w);
-    };
-    for (int x0 = 0; x0 < active; x0 += 32) {
-        const float2 s = x0 + lane < active ? __ldcg(ml + size_t(x0 + lane) * R) : make_float2(-INFINITY, 0.0f);
-        const float w = part_weight(s.x, s.y, top);
-        sum += warp_sum(w * s.y);
-        const int n = min(32, active - x0);
-        for (int i0 = 0; i0 < n; i0 += 8) {
-            float4 v[8], v2[8];
-#pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                const float4* p = reinterpret_cast<const float4*>(o + size_t(x0 + i0 + i) * R * hd);
-                v[i] = v2[i] = make_float4(0, 0, 0, 0);
-                if (i0 + i < n && in) v[i] = __ldcg(p + lane);
-                if (i0 + i < n && in2) v2[i] = __ldcg(p + 32 + lane);
-            }
-#pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                const float f = __shfl_sync(0xffffffffu, w, (i0 + i) & 31);
-                if (i0 + i < n) {
-                    add(acc, f, v[i]);
-                    if (hd > 128) add(acc2, f, v2[i]);
-                }
-            }
-        }
-    }
-    const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
-    const int tk = row / a.group, h = kvh * a.group + row - tk * a.group;
-    float4* out = reinterpret_cast<float4*>(a.out + ((size_t(seq) * a.n_tree + tk) * a.n_head + h) * hd);
-    if (in) out[lane] = make_float4(acc.x * inv, acc.y * inv, acc.z * inv, acc.w * inv);
-    if (in2) out[32 + lane] = make_float4(acc2.x * inv, acc2.y * inv, acc2.z * inv, acc2.w * inv);
+    const unsigned id = blockIdx.x * 4 + (threadIdx.x >> 5), per_seq = unsigned(a.c.n_kv) * a.rows;
+    if (id >= unsigned(a.c.n_seq) * per_seq) return;
+    int seq = int(id / per_seq);
+    const int row = int(id % per_seq) % a.rows, kvh = int(id % per_seq) / a.rows, rb = row / R;
+    const Cutting cut = tree_cutting(a, step, 0, seq);
+    const size_t unit = size_t(a.c.n_kv) * a.row_blocks;
+    join_row(a, row, kvh, seq, (cut.first * unit + size_t(kvh) * a.row_blocks + rb) * R + row - rb * R, unit * R, cut.parts);
 }
 
-// How a call is cut: rows of a CTA, CTAs over the rows, splits of the context.
+// How a call is cut: rows of a CTA, CTAs over the rows, splits of the context
+// (the mean number of parts of a sequence), and all parts.
 struct Cut {
     bool tc;
-    int R, row_blocks, splits;
-    size_t units;
+    int R, row_blocks, splits, parts;
+    size_t rows;  // of all parts in the scratch
 };
 Cut cut_of(int n_seq, int n_tree, int n_head, int n_kv, int head_dim, int max_len) {
     Cut c;
     const int rows = n_tree * (n_head / n_kv);
     const size_t sms = size_t(syn_num_sms());
     c.tc = rows > 16 && head_dim <= 128;
-    c.R = c.tc ? kTcRows : 16;
+    c.R = c.tc ? kTcRows : rows <= 8 ? 8 : 16;
     c.row_blocks = (rows + c.R - 1) / c.R;
-    c.units = size_t(n_seq) * n_kv * c.row_blocks;
+    const size_t units = size_t(n_seq) * n_kv * c.row_blocks;
     if (c.tc) {
         // one CTA per SM: the split of the tiles whose last wave ends first
         const int tiles = (max_len + kTcTile - 1) / kTcTile;
         size_t best = ~size_t(0);
         c.splits = 1;
         for (int n = 1; n <= std::min(tiles, 128); ++n) {
-            const size_t waves = (c.units * n + sms - 1) / sms, per = size_t(tiles + n - 1) / n;
+            const size_t waves = (units * n + sms - 1) / sms, per = size_t(tiles + n - 1) / n;
             const size_t cost = waves * (per + 8);  // a CTA's start and end take about 8 tiles
             if (cost < best) {
                 best = cost;
@@ -627,29 +676,32 @@ Cut cut_of(int n_seq, int n_tree, int n_head, int n_kv, int head_dim, int max_le
             }
         }
     } else {
-        // two CTAs per SM; a split has at least two steps of every warp
+        // three CTAs per SM; a part has at least two steps of every warp
         const int most = (max_len + 2 * kWarps * kStep - 1) / (2 * kWarps * kStep);
-        c.splits = int(std::max<size_t>(1, std::min<size_t>(2 * sms / c.units, size_t(most))));
+        c.splits = int(std::max<size_t>(1, std::min<size_t>(3 * sms / units, size_t(most))));
+        if (units * sizeof(unsigned) > kCounterBytes) c.splits = 1;
     }
+    c.parts = c.splits == 1 ? n_seq : n_seq == 1 ? c.splits : n_seq * (c.splits + 1);
+    c.rows = size_t(c.parts) * n_kv * c.row_blocks * c.R;
     return c;
 }
 
-template <int TYPE, int HDP, int MT>
-int launch(const TreeParams& a, cudaStream_t s) {
-    auto kernel = tree_attn_kernel<TYPE, HDP, MT>;
-    constexpr int smem = Plan<TYPE, HDP, MT>::smem;
+template <int TYPE, int HDP, bool STACK>
+int launch(const TreeParams& a, int parts, cudaStream_t s) {
+    auto kernel = tree_attn_kernel<TYPE, HDP, STACK>;
+    constexpr int smem = Plan<TYPE, HDP, STACK>::smem;
     static_assert(smem <= 227 * 1024, "shared memory of a CTA");
     const int st = syn_opt_in_smem(reinterpret_cast<const void*>(kernel), smem);
     if (st) return st;
-    const dim3 grid{unsigned(a.splits), unsigned(a.c.n_kv * a.row_blocks), unsigned(a.c.n_seq)};
+    const dim3 grid{unsigned(parts), unsigned(a.c.n_kv * a.row_blocks), 1};
     return syn_launch(kernel, grid, kWarps * 32, smem, s, a);
 }
 
 template <int TYPE>
-int launch_type(const TreeParams& a, cudaStream_t s) {
-    if (a.c.hd <= 64) return launch<TYPE, 64, 1>(a, s);
-    if (a.c.hd <= 128) return launch<TYPE, 128, 1>(a, s);
-    return launch<TYPE, 256, 1>(a, s);
+int launch_type(const TreeParams& a, const Cut& c, cudaStream_t s) {
+    if (a.c.hd <= 64) return c.R == 8 ? launch<TYPE, 64, true>(a, c.parts, s) : launch<TYPE, 64, false>(a, c.parts, s);
+    if (a.c.hd <= 128) return c.R == 8 ? launch<TYPE, 128, true>(a, c.parts, s) : launch<TYPE, 128, false>(a, c.parts, s);
+    return c.R == 8 ? launch<TYPE, 256, true>(a, c.parts, s) : launch<TYPE, 256, false>(a, c.parts, s);
 }
 
 }  // namespace
@@ -660,7 +712,7 @@ extern "C" size_t syn_tree_attention_scratch_bytes(int n_seq, int n_tree, int n_
         head_dim > 256 || max_len < n_tree)
         return 0;
     const Cut c = cut_of(n_seq, n_tree, n_head, n_kv, head_dim, max_len);
-    return c.splits > 1 ? align256(c.units * c.splits * c.R * 8) + align256(c.units * c.splits * c.R * size_t(head_dim) * 4) : 256;
+    return kCounterBytes + (c.splits > 1 ? align256(c.rows * 8) + align256(c.rows * head_dim * 4) : 0);
 }
 
 extern "C" int syn_tree_attention(const syn_kv_cache* c, int layer, const syn_tree_attention_args* x, void* stream) {
@@ -678,8 +730,10 @@ extern "C" int syn_tree_attention(const syn_kv_cache* c, int layer, const syn_tr
     TreeParams a{};
     a.c = kv_view(c, layer);
     a.q = x->q; a.out = x->out; a.len = x->len; a.mask = x->mask;
-    a.part_ml = static_cast<float2*>(x->scratch);
-    a.part_o = reinterpret_cast<float*>(static_cast<char*>(x->scratch) + align256(cut.units * cut.splits * cut.R * 8));
+    char* scratch = static_cast<char*>(x->scratch);
+    a.arrived = reinterpret_cast<unsigned*>(scratch);
+    a.part_ml = reinterpret_cast<float2*>(scratch + kCounterBytes);
+    a.part_o = reinterpret_cast<float*>(scratch + kCounterBytes + align256(cut.rows * 8));
     a.q_stride = x->q_stride ? x->q_stride : q_row;
     a.n_tree = x->n_tree; a.n_head = x->n_head;
     a.group = x->n_head / c->n_kv;
@@ -690,11 +744,11 @@ extern "C" int syn_tree_attention(const syn_kv_cache* c, int layer, const syn_tr
     a.splits = cut.splits;
     a.scale_log2 = x->scale * 1.4426950408889634f;
     cudaStream_t s = static_cast<cudaStream_t>(stream);
-    if (cut.tc) st = syn_tree_attention_tc(a, c->type, s);
-    else if (c->type == SYN_F16) st = launch_type<SYN_F16>(a, s);
-    else if (c->type == SYN_Q8_0) st = launch_type<SYN_Q8_0>(a, s);
-    else st = launch_type<SYN_Q4_0>(a, s);
-    if (st || cut.splits == 1) return st;
+    if (cut.tc) st = syn_tree_attention_tc(a, c->type, cut.parts, s);
+    else if (c->type == SYN_F16) st = launch_type<SYN_F16>(a, cut, s);
+    else if (c->type == SYN_Q8_0) st = launch_type<SYN_Q8_0>(a, cut, s);
+    else st = launch_type<SYN_Q4_0>(a, cut, s);
+    if (st || cut.splits == 1 || !cut.tc) return st;
     const size_t rows = size_t(c->n_seq) * c->n_kv * a.rows;
-    return syn_launch_pdl(true, tree_join_kernel, unsigned((rows + 3) / 4), 128, 0, s, a, cut.R, cut.tc ? kTcTile : kStep);
+    return syn_launch_pdl(true, tree_join_kernel, unsigned((rows + 3) / 4), 128, 0, s, a, cut.R, kTcTile);
 }

@@ -14,8 +14,9 @@ struct TreeParams {
     float* out;
     const int32_t* len;
     const uint32_t* mask;
-    float2* part_ml;     // [n_seq][n_kv * row blocks][splits][R]: a part's maximum and sum of a row
-    float* part_o;       // [n_seq][n_kv * row blocks][splits][R][hd]: its output, not divided
+    unsigned* arrived;   // [n_seq][n_kv * row blocks]: parts that are done; zero between calls
+    float2* part_ml;     // [parts][n_kv * row blocks][R]: a part's maximum and sum of a row
+    float* part_o;       // [parts][n_kv * row blocks][R][hd]: its output, not divided
     size_t q_stride;
     int n_tree, n_head, group, rows, row_blocks, max_len, mask_words, splits;
     float scale_log2;    // scale * log2(e)
@@ -23,6 +24,9 @@ struct TreeParams {
 
 __device__ __forceinline__ void cp16(uint32_t dst, const void* src, bool in) {
     asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(in ? 16 : 0) : "memory");
+}
+__device__ __forceinline__ void cp16(uint32_t dst, const void* src) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
 }
 __device__ __forceinline__ void cp_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 template <int N>
@@ -55,6 +59,59 @@ __device__ __forceinline__ void q_factor(float m, float& up, float& down) {
     up = plain ? 256.0f : __uint_as_float(uint32_t(254 + 8 - e) << 23);
     down = plain ? 1.0f / 256.0f : __uint_as_float(uint32_t(e - 8) << 23);
 }
+// How the sequences' contexts are cut into parts, equally long whatever the
+// sequences' lengths: with splits > 1, parts of `per` steps each, numbered
+// through the sequences, at most n_seq * splits + n_seq of them (n_seq = 1:
+// splits); with splits = 1 a part is a sequence.
+struct Cutting {
+    int per;    // steps of a part
+    int first;  // the sequence's first part
+    int parts;  // and its number of parts
+};
+__device__ __forceinline__ int tree_len(const TreeParams& a, int seq) {
+    return min(max(__ldg(a.len + seq), 0), a.max_len - a.n_tree);
+}
+__device__ __forceinline__ int tree_steps(const TreeParams& a, int seq, int step) {
+    return (tree_len(a, seq) + a.n_tree + step - 1) / step;
+}
+// For a warp: the cutting of sequence seq, or, with seq = -1, of the sequence
+// that holds part `part` (seq = -1 stays when there is none).
+__device__ __forceinline__ Cutting tree_cutting(const TreeParams& a, int step, int part, int& seq) {
+    const int lane = threadIdx.x & 31, n = a.c.n_seq;
+    if (a.splits == 1) {
+        if (seq < 0) seq = part;
+        return {0x7fffffff, seq, 1};
+    }
+    if (n == 1) {
+        seq = 0;
+        const int steps = tree_steps(a, 0, step), per = (steps + a.splits - 1) / a.splits, parts = (steps + per - 1) / per;
+        if (part >= parts) seq = -1;
+        return {per, 0, parts};
+    }
+    int total = 0;
+    for (int s = lane; s < n; s += 32) total += tree_steps(a, s, step);
+    total = __reduce_add_sync(0xffffffffu, total);
+    const int per = (total + n * a.splits - 1) / (n * a.splits);
+    int before = 0;
+    for (int s0 = 0; s0 < n; s0 += 32) {
+        const int mine = s0 + lane < n ? (tree_steps(a, s0 + lane, step) + per - 1) / per : 0;
+        int sum = mine;  // inclusive, over the lanes
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const int x = __shfl_up_sync(0xffffffffu, sum, o);
+            if (lane >= o) sum += x;
+        }
+        const bool here = seq >= 0 ? s0 + lane == seq : s0 + lane < n && part < before + sum;
+        const unsigned who = __ballot_sync(0xffffffffu, here);
+        if (who) {
+            const int l = __ffs(who) - 1;
+            seq = s0 + l;
+            return {per, before + __shfl_sync(0xffffffffu, sum - mine, l), __shfl_sync(0xffffffffu, mine, l)};
+        }
+        before += __shfl_sync(0xffffffffu, sum, 31);
+    }
+    return {per, 0, 0};
+}
 // Whether token tk of sequence seq sees the tree's row j >= 0.
 __device__ __forceinline__ bool tree_sees(const TreeParams& a, int seq, int tk, int j) {
     if (j >= a.n_tree || tk >= a.n_tree) return false;
@@ -69,6 +126,6 @@ __device__ __forceinline__ float part_weight(float m, float l, float top) {
 }  // namespace syn
 
 // The tcgen05 kernel (tree_attention_tc.cu): 128 rows of a KV head per CTA,
-// heads of up to 128 dims; a.splits counts runs of 64 positions' tiles.
+// heads of up to 128 dims, a step of a part being a tile of 64 positions.
 constexpr int kTcRows = 128, kTcTile = 64;
-int syn_tree_attention_tc(const syn::TreeParams& a, int type, cudaStream_t s);
+int syn_tree_attention_tc(const syn::TreeParams& a, int type, int parts, cudaStream_t s);

@@ -121,17 +121,17 @@ __global__ void __launch_bounds__(kTcThreads, 1) tree_attn_tc_kernel(const TreeP
     const uint32_t tiles_s = smem_addr(tiles);
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const int hd = a.c.hd;
-    const int kvh = blockIdx.y / a.row_blocks, rb = blockIdx.y - kvh * a.row_blocks, seq = blockIdx.z;
+    const int kvh = blockIdx.y / a.row_blocks, rb = blockIdx.y - kvh * a.row_blocks;
     const int row0 = rb * kTcRows, rows = min(kTcRows, a.rows - row0);
 
     pdl_launch_dependents();
     pdl_wait();
-    const int len = min(max(a.len[seq], 0), a.max_len - a.n_tree);
-    const int total = len + a.n_tree;
+    int seq = -1;
+    const Cutting cut = tree_cutting(a, kTcTile, blockIdx.x, seq);
+    if (seq < 0) return;
+    const int len = tree_len(a, seq), total = len + a.n_tree;
     const int n_tiles = (total + kTcTile - 1) / kTcTile;
-    const int per = (n_tiles + a.splits - 1) / a.splits;
-    const int t0 = blockIdx.x * per, n = min(per, n_tiles - t0);  // tiles t0 .. t0 + n - 1
-    if (n <= 0) return;
+    const int t0 = (int(blockIdx.x) - cut.first) * cut.per, n = min(cut.per, n_tiles - t0);  // tiles t0 .. t0 + n - 1
     const int edge0 = len / kTcTile;  // the first tile with a row of the tree
 
     if (tid == 0) {
@@ -327,7 +327,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) tree_attn_tc_kernel(const TreeP
         if (live && r < rows && !*reinterpret_cast<volatile int*>(&sh.abort)) {
             const bool whole = a.splits == 1;
             const int row = row0 + r, tok = row / a.group, h = kvh * a.group + row - tok * a.group;
-            const size_t part = ((size_t(seq) * gridDim.y + blockIdx.y) * a.splits + blockIdx.x) * kTcRows + r;
+            const size_t part = (size_t(blockIdx.x) * gridDim.y + blockIdx.y) * kTcRows + r;
             float* out = whole ? a.out + ((size_t(seq) * a.n_tree + tok) * a.n_head + h) * hd : a.part_o + part * hd;
             const float inv = !whole ? 1.0f : l == 0.0f ? 0.0f : 1.0f / l;
 #pragma unroll
@@ -591,7 +591,7 @@ int cache_map(const TreeParams& a, const char* base, CUtensorMap* m) {
 }
 
 template <int TYPE, int HDP>
-int launch(const TreeParams& a, cudaStream_t s) {
+int launch(const TreeParams& a, int parts, cudaStream_t s) {
     auto kernel = tree_attn_tc_kernel<TYPE, HDP>;
     constexpr int smem = TcPlan<TYPE, HDP>::smem;
     static_assert(smem + sizeof(TcShared) <= 227 * 1024, "shared memory of a CTA");
@@ -602,16 +602,16 @@ int launch(const TreeParams& a, cudaStream_t s) {
         if ((st = cache_map(a, a.c.k, &maps.k))) return st;
         if ((st = cache_map(a, a.c.v, &maps.v))) return st;
     }
-    const dim3 grid{unsigned(a.splits), unsigned(a.c.n_kv * a.row_blocks), unsigned(a.c.n_seq)};
+    const dim3 grid{unsigned(parts), unsigned(a.c.n_kv * a.row_blocks), 1};
     return syn_launch(kernel, grid, kTcThreads, smem, s, a, maps);
 }
 
 }  // namespace
 
-int syn_tree_attention_tc(const TreeParams& a, int type, cudaStream_t s) {
+int syn_tree_attention_tc(const TreeParams& a, int type, int parts, cudaStream_t s) {
     if (a.c.hd <= 64)
-        return type == SYN_F16 ? launch<SYN_F16, 64>(a, s) : type == SYN_Q8_0 ? launch<SYN_Q8_0, 64>(a, s) : launch<SYN_Q4_0, 64>(a, s);
-    return type == SYN_F16 ? launch<SYN_F16, 128>(a, s) : type == SYN_Q8_0 ? launch<SYN_Q8_0, 128>(a, s) : launch<SYN_Q4_0, 128>(a, s);
+        return type == SYN_F16 ? launch<SYN_F16, 64>(a, parts, s) : type == SYN_Q8_0 ? launch<SYN_Q8_0, 64>(a, parts, s) : launch<SYN_Q4_0, 64>(a, parts, s);
+    return type == SYN_F16 ? launch<SYN_F16, 128>(a, parts, s) : type == SYN_Q8_0 ? launch<SYN_Q8_0, 128>(a, parts, s) : launch<SYN_Q4_0, 128>(a, parts, s);
 }
 
 // Bounded waits of the kernel that gave up on the current device (-1: unreadable).
