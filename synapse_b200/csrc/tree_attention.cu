@@ -24,8 +24,8 @@
 // binary16 terms (22 bits), and so are the probabilities; K and V enter as
 // stored. Quantised caches enter as integers (exact in binary16): a score is
 // the sum over blocks of scale * (q . quants); for V the block's scale is
-// m * 2^e, 2^e <= 2^9 applied to the integers (exact) and m (in [1, 2) for all
-// but extreme scales) to the float probabilities before they are split, so no
+// m * 2^e, 2^e <= 2^5 applied to the integers (exact) and m (in [1, 2) unless
+// the scale is beyond 2^6) to the float probabilities before they are split, so no
 // value is rounded to binary16. Each step's output is added to float registers
 // outside the tensor core, whose accumulation truncates: kept there over 64
 // steps it cost 2e-6.
@@ -341,7 +341,7 @@ __global__ void __launch_bounds__(kWarps * 32, Plan<TYPE, HDP, STACK>::ctas) tre
                 const uint32_t dk = ok ? reinterpret_cast<const uint16_t*>(st + S::sk_at + scale_off)[r * nb + b] : 0u;
                 const uint32_t dv = ok ? reinterpret_cast<const uint16_t*>(st + S::sv_at + scale_off)[r * nb + b] : 0u;
                 const bool finite = (dv & 0x7c00u) != 0x7c00u;
-                const uint32_t pow = finite ? min(max(dv & 0x7c00u, 0x0400u), 0x6000u) : 0x0400u;  // 2^-14 .. 2^9: 127 * 2^9 is finite
+                const uint32_t pow = finite ? min(max(dv & 0x7c00u, 0x0400u), 0x5000u) : 0x0400u;  // 2^-14 .. 2^5: 1152 * 2^5 is finite
                 const float inv = __uint_as_float(0x7f000000u - __float_as_uint(f16_from_bits(uint16_t(pow))));
                 kds[id] = finite ? f16_from_bits(uint16_t(dk)) : __uint_as_float(0x7fffffffu);
                 vms[id] = finite ? f16_from_bits(uint16_t(dv)) * inv : 0.0f;
@@ -512,8 +512,9 @@ __global__ void __launch_bounds__(kWarps * 32, Plan<TYPE, HDP, STACK>::ctas) tre
             float c[4];
             mma0(c, pf[0], b0, b1);
             if (!STACK) mma(c, pf[QT - 1], b0, b1);
-#pragma unroll
-            for (int e = 0; e < 2 * NR; ++e) acc[e] += STACK ? c[e] + c[e + 2] : c[e];
+            if (STACK) add2(c[0], c[1], c[2], c[3]);
+            add2(acc[0], acc[1], c[0], c[1]);
+            if (!STACK) add2(acc[2 * NR - 2], acc[2 * NR - 1], c[2], c[3]);
         };
         if constexpr (!kQuant) {
             split_p({1.0f, 1.0f, 1.0f, 1.0f});
@@ -539,8 +540,9 @@ __global__ void __launch_bounds__(kWarps * 32, Plan<TYPE, HDP, STACK>::ctas) tre
                 else if ((b & 1) == 0)  // two blocks of 16 bytes
                     ldsm4t(r4, st_s + S::v_at + ((lane & 7) + ((lane >> 3) & 1) * 8) * S::v_pitch + b * 16 + (lane >> 4) * 16);
                 split_p({vm[0][b], vm[1][b], vm[2][b], vm[3][b]});
-                const __half2 zero = half2_of(TYPE == SYN_Q8_0 ? 0x64806480u : 0x64086408u);
+                const __half2 zero = half2_of(TYPE == SYN_Q8_0 ? 0xe480e480u : 0xe408e408u);
                 const __half2 e0 = half2_of(__float_as_uint(ve[0][b])), e1 = half2_of(__float_as_uint(ve[1][b]));
+                const __half2 z0 = __hmul2(zero, e0), z1 = __hmul2(zero, e1);  // -1152 * 2^e | -1032 * 2^e
                 // n-tile 4 b + 2 half + odd: dims 32 b + 16 half + 2 n + odd
 #pragma unroll
                 for (int half = 0; half < 2; ++half) {
@@ -555,8 +557,8 @@ __global__ void __launch_bounds__(kWarps * 32, Plan<TYPE, HDP, STACK>::ctas) tre
 #pragma unroll
                     for (int odd = 0; odd < 2; ++odd) {
                         const uint32_t sel = odd ? 0x4341u : 0x4240u;
-                        output(o[4 * b + 2 * half + odd], bits(__hmul2(__hsub2(bytes_h2(x0, sel), zero), e0)),
-                               bits(__hmul2(__hsub2(bytes_h2(x1, sel), zero), e1)));
+                        output(o[4 * b + 2 * half + odd], bits(__hfma2(bytes_h2(x0, sel), e0, z0)),
+                               bits(__hfma2(bytes_h2(x1, sel), e1, z1)));
                     }
                 }
             }
@@ -606,7 +608,7 @@ __global__ void __launch_bounds__(kWarps * 32, Plan<TYPE, HDP, STACK>::ctas) tre
             sum += f[w] * jl[w * R + r];
         }
         const int row = row0 + r, tk = row / a.group, h = kvh * a.group + row - tk * a.group;
-        const bool whole = a.splits == 1;
+        const bool whole = a.parts == 0;
         float* out = whole ? a.out + ((size_t(seq) * a.n_tree + tk) * a.n_head + h) * hd : a.part_o + (part + r) * hd;
         const float inv = !whole ? 1.0f : sum == 0.0f ? 0.0f : 1.0f / sum;
         for (int d = lane; d < hd; d += 32) {
@@ -617,7 +619,7 @@ __global__ void __launch_bounds__(kWarps * 32, Plan<TYPE, HDP, STACK>::ctas) tre
         }
         if (!whole && lane == 0) a.part_ml[part + r] = make_float2(mx, sum);
     }
-    if (a.splits == 1) return;
+    if (a.parts == 0) return;
 
     // --- the last of the sequence's parts to be done joins them ----------------------------
     __threadfence();
@@ -647,11 +649,11 @@ __global__ void __launch_bounds__(128) tree_join_kernel(const TreeParams a, int 
     join_row(a, row, kvh, seq, (cut.first * unit + size_t(kvh) * a.row_blocks + rb) * R + row - rb * R, unit * R, cut.parts);
 }
 
-// How a call is cut: rows of a CTA, CTAs over the rows, splits of the context
-// (the mean number of parts of a sequence), and all parts.
+// How a call is cut: rows of a CTA, CTAs over the rows, parts of the contexts
+// (0: a part is a sequence).
 struct Cut {
     bool tc;
-    int R, row_blocks, splits, parts;
+    int R, row_blocks, parts;
     size_t rows;  // of all parts in the scratch
 };
 Cut cut_of(int n_seq, int n_tree, int n_head, int n_kv, int head_dim, int max_len) {
@@ -661,47 +663,48 @@ Cut cut_of(int n_seq, int n_tree, int n_head, int n_kv, int head_dim, int max_le
     c.tc = rows > 16 && head_dim <= 128;
     c.R = c.tc ? kTcRows : rows <= 8 ? 8 : 16;
     c.row_blocks = (rows + c.R - 1) / c.R;
-    const size_t units = size_t(n_seq) * n_kv * c.row_blocks;
+    const size_t units = size_t(n_kv) * c.row_blocks;  // CTAs of a part
     if (c.tc) {
-        // one CTA per SM: the split of the tiles whose last wave ends first
-        const int tiles = (max_len + kTcTile - 1) / kTcTile;
+        // one CTA per SM: the parts whose last wave ends first
+        const size_t tiles = size_t(max_len + kTcTile - 1) / kTcTile * n_seq;
         size_t best = ~size_t(0);
-        c.splits = 1;
-        for (int n = 1; n <= std::min(tiles, 128); ++n) {
-            const size_t waves = (units * n + sms - 1) / sms, per = size_t(tiles + n - 1) / n;
+        c.parts = 0;
+        for (size_t n = n_seq; n <= std::min(tiles, size_t(n_seq) * 128); ++n) {
+            const size_t waves = (units * n + sms - 1) / sms, per = (tiles + n - 1) / n;
             const size_t cost = waves * (per + 8);  // a CTA's start and end take about 8 tiles
+            if (waves > 4 && n > size_t(n_seq)) break;
             if (cost < best) {
                 best = cost;
-                c.splits = n;
+                c.parts = int(n);
             }
         }
     } else {
         // three CTAs per SM; a part has at least two steps of every warp
-        const int most = (max_len + 2 * kWarps * kStep - 1) / (2 * kWarps * kStep);
-        c.splits = int(std::max<size_t>(1, std::min<size_t>(3 * sms / units, size_t(most))));
-        if (units * sizeof(unsigned) > kCounterBytes) c.splits = 1;
+        const size_t most = size_t(max_len + 2 * kWarps * kStep - 1) / (2 * kWarps * kStep) * n_seq;
+        c.parts = int(std::min(3 * sms / units, most));
     }
-    c.parts = c.splits == 1 ? n_seq : n_seq == 1 ? c.splits : n_seq * (c.splits + 1);
-    c.rows = size_t(c.parts) * n_kv * c.row_blocks * c.R;
+    if (c.parts <= n_seq && !(n_seq == 1 && c.parts > 1)) c.parts = 0;
+    if (!c.tc && units * n_seq * sizeof(unsigned) > kCounterBytes) c.parts = 0;
+    c.rows = size_t(c.parts) * units * c.R;
     return c;
 }
 
 template <int TYPE, int HDP, bool STACK>
-int launch(const TreeParams& a, int parts, cudaStream_t s) {
+int launch(const TreeParams& a, cudaStream_t s) {
     auto kernel = tree_attn_kernel<TYPE, HDP, STACK>;
     constexpr int smem = Plan<TYPE, HDP, STACK>::smem;
     static_assert(smem <= 227 * 1024, "shared memory of a CTA");
     const int st = syn_opt_in_smem(reinterpret_cast<const void*>(kernel), smem);
     if (st) return st;
-    const dim3 grid{unsigned(parts), unsigned(a.c.n_kv * a.row_blocks), 1};
+    const dim3 grid{unsigned(a.parts ? a.parts : a.c.n_seq), unsigned(a.c.n_kv * a.row_blocks), 1};
     return syn_launch(kernel, grid, kWarps * 32, smem, s, a);
 }
 
 template <int TYPE>
 int launch_type(const TreeParams& a, const Cut& c, cudaStream_t s) {
-    if (a.c.hd <= 64) return c.R == 8 ? launch<TYPE, 64, true>(a, c.parts, s) : launch<TYPE, 64, false>(a, c.parts, s);
-    if (a.c.hd <= 128) return c.R == 8 ? launch<TYPE, 128, true>(a, c.parts, s) : launch<TYPE, 128, false>(a, c.parts, s);
-    return c.R == 8 ? launch<TYPE, 256, true>(a, c.parts, s) : launch<TYPE, 256, false>(a, c.parts, s);
+    if (a.c.hd <= 64) return c.R == 8 ? launch<TYPE, 64, true>(a, s) : launch<TYPE, 64, false>(a, s);
+    if (a.c.hd <= 128) return c.R == 8 ? launch<TYPE, 128, true>(a, s) : launch<TYPE, 128, false>(a, s);
+    return c.R == 8 ? launch<TYPE, 256, true>(a, s) : launch<TYPE, 256, false>(a, s);
 }
 
 }  // namespace
@@ -712,7 +715,7 @@ extern "C" size_t syn_tree_attention_scratch_bytes(int n_seq, int n_tree, int n_
         head_dim > 256 || max_len < n_tree)
         return 0;
     const Cut c = cut_of(n_seq, n_tree, n_head, n_kv, head_dim, max_len);
-    return kCounterBytes + (c.splits > 1 ? align256(c.rows * 8) + align256(c.rows * head_dim * 4) : 0);
+    return kCounterBytes + (c.parts ? align256(c.rows * 8) + align256(c.rows * head_dim * 4) : 0);
 }
 
 extern "C" int syn_tree_attention(const syn_kv_cache* c, int layer, const syn_tree_attention_args* x, void* stream) {
@@ -741,14 +744,14 @@ extern "C" int syn_tree_attention(const syn_kv_cache* c, int layer, const syn_tr
     a.row_blocks = cut.row_blocks;
     a.max_len = x->max_len;
     a.mask_words = (x->n_tree + 31) / 32;
-    a.splits = cut.splits;
+    a.parts = cut.parts;
     a.scale_log2 = x->scale * 1.4426950408889634f;
     cudaStream_t s = static_cast<cudaStream_t>(stream);
-    if (cut.tc) st = syn_tree_attention_tc(a, c->type, cut.parts, s);
+    if (cut.tc) st = syn_tree_attention_tc(a, c->type, s);
     else if (c->type == SYN_F16) st = launch_type<SYN_F16>(a, cut, s);
     else if (c->type == SYN_Q8_0) st = launch_type<SYN_Q8_0>(a, cut, s);
     else st = launch_type<SYN_Q4_0>(a, cut, s);
-    if (st || cut.splits == 1 || !cut.tc) return st;
+    if (st || !cut.parts || !cut.tc) return st;
     const size_t rows = size_t(c->n_seq) * c->n_kv * a.rows;
     return syn_launch_pdl(true, tree_join_kernel, unsigned((rows + 3) / 4), 128, 0, s, a, cut.R, kTcTile);
 }

@@ -18,7 +18,8 @@ struct TreeParams {
     float2* part_ml;     // [parts][n_kv * row blocks][R]: a part's maximum and sum of a row
     float* part_o;       // [parts][n_kv * row blocks][R][hd]: its output, not divided
     size_t q_stride;
-    int n_tree, n_head, group, rows, row_blocks, max_len, mask_words, splits;
+    int n_tree, n_head, group, rows, row_blocks, max_len, mask_words;
+    int parts;           // that the contexts may be cut into, more than n_seq (n_seq = 1: or 1); 0: not cut
     float scale_log2;    // scale * log2(e)
 };
 
@@ -47,6 +48,12 @@ __device__ __forceinline__ void split2(float x, float y, uint32_t& hi, uint32_t&
     hi = bits(h);
     lo = bits(__floats2half2_rn(x - f.x, y - f.y));
 }
+// a += b of two floats each.
+__device__ __forceinline__ void add2(float& a0, float& a1, float b0, float b1) {
+    asm("{\n .reg .b64 a, b;\n mov.b64 a, {%0, %1};\n mov.b64 b, {%2, %3};\n add.rn.f32x2 a, a, b;\n mov.b64 {%0, %1}, a;\n}\n"
+        : "+f"(a0), "+f"(a1)
+        : "f"(b0), "f"(b1));
+}
 // Bytes i and j of x as binary16 integers 1024 + byte.
 __device__ __forceinline__ __half2 bytes_h2(uint32_t x, uint32_t sel) { return half2_of(__byte_perm(x, 0x64646464u, sel)); }
 
@@ -59,10 +66,9 @@ __device__ __forceinline__ void q_factor(float m, float& up, float& down) {
     up = plain ? 256.0f : __uint_as_float(uint32_t(254 + 8 - e) << 23);
     down = plain ? 1.0f / 256.0f : __uint_as_float(uint32_t(e - 8) << 23);
 }
-// How the sequences' contexts are cut into parts, equally long whatever the
-// sequences' lengths: with splits > 1, parts of `per` steps each, numbered
-// through the sequences, at most n_seq * splits + n_seq of them (n_seq = 1:
-// splits); with splits = 1 a part is a sequence.
+// How the sequences' contexts are cut into parts: of one length, `per` steps,
+// whatever the sequences' lengths, numbered through the sequences, and the
+// shortest of which there are at most a.parts (0: a part is a sequence).
 struct Cutting {
     int per;    // steps of a part
     int first;  // the sequence's first part
@@ -78,20 +84,30 @@ __device__ __forceinline__ int tree_steps(const TreeParams& a, int seq, int step
 // that holds part `part` (seq = -1 stays when there is none).
 __device__ __forceinline__ Cutting tree_cutting(const TreeParams& a, int step, int part, int& seq) {
     const int lane = threadIdx.x & 31, n = a.c.n_seq;
-    if (a.splits == 1) {
+    if (a.parts == 0) {
         if (seq < 0) seq = part;
-        return {0x7fffffff, seq, 1};
+        return {0x3fffffff, seq, 1};
     }
     if (n == 1) {
         seq = 0;
-        const int steps = tree_steps(a, 0, step), per = (steps + a.splits - 1) / a.splits, parts = (steps + per - 1) / per;
+        const int steps = tree_steps(a, 0, step), per = (steps + a.parts - 1) / a.parts, parts = (steps + per - 1) / per;
         if (part >= parts) seq = -1;
         return {per, 0, parts};
     }
-    int total = 0;
-    for (int s = lane; s < n; s += 32) total += tree_steps(a, s, step);
+    const int own = lane < n ? tree_steps(a, lane, step) : 0;
+    int total = own;
+    for (int s = 32 + lane; s < n; s += 32) total += tree_steps(a, s, step);
     total = __reduce_add_sync(0xffffffffu, total);
-    const int per = (total + n * a.splits - 1) / (n * a.splits);
+    // total / per + n parts are enough, so there are at most a.parts of the second length
+    int per = (total + a.parts - 1) / a.parts, most = (total + a.parts - n - 1) / (a.parts - n);
+    while (per < most) {
+        const int mid = (per + most) / 2;
+        int parts = (own + mid - 1) / mid;
+        for (int s = 32 + lane; s < n; s += 32) parts += (tree_steps(a, s, step) + mid - 1) / mid;
+        parts = __reduce_add_sync(0xffffffffu, parts);
+        if (parts <= a.parts) most = mid;
+        else per = mid + 1;
+    }
     int before = 0;
     for (int s0 = 0; s0 < n; s0 += 32) {
         const int mine = s0 + lane < n ? (tree_steps(a, s0 + lane, step) + per - 1) / per : 0;
@@ -128,4 +144,4 @@ __device__ __forceinline__ float part_weight(float m, float l, float top) {
 // The tcgen05 kernel (tree_attention_tc.cu): 128 rows of a KV head per CTA,
 // heads of up to 128 dims, a step of a part being a tile of 64 positions.
 constexpr int kTcRows = 128, kTcTile = 64;
-int syn_tree_attention_tc(const syn::TreeParams& a, int type, int parts, cudaStream_t s);
+int syn_tree_attention_tc(const syn::TreeParams& a, int type, cudaStream_t s);

@@ -325,7 +325,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) tree_attn_tc_kernel(const TreeP
         asm volatile("bar.sync 2, 384;" ::: "memory");  // the softmax warps' m and l
         const float l = sh.l[r];
         if (live && r < rows && !*reinterpret_cast<volatile int*>(&sh.abort)) {
-            const bool whole = a.splits == 1;
+            const bool whole = a.parts == 0;
             const int row = row0 + r, tok = row / a.group, h = kvh * a.group + row - tok * a.group;
             const size_t part = (size_t(blockIdx.x) * gridDim.y + blockIdx.y) * kTcRows + r;
             float* out = whole ? a.out + ((size_t(seq) * a.n_tree + tok) * a.n_head + h) * hd : a.part_o + part * hd;
@@ -591,7 +591,7 @@ int cache_map(const TreeParams& a, const char* base, CUtensorMap* m) {
 }
 
 template <int TYPE, int HDP>
-int launch(const TreeParams& a, int parts, cudaStream_t s) {
+int launch(const TreeParams& a, cudaStream_t s) {
     auto kernel = tree_attn_tc_kernel<TYPE, HDP>;
     constexpr int smem = TcPlan<TYPE, HDP>::smem;
     static_assert(smem + sizeof(TcShared) <= 227 * 1024, "shared memory of a CTA");
@@ -602,16 +602,16 @@ int launch(const TreeParams& a, int parts, cudaStream_t s) {
         if ((st = cache_map(a, a.c.k, &maps.k))) return st;
         if ((st = cache_map(a, a.c.v, &maps.v))) return st;
     }
-    const dim3 grid{unsigned(parts), unsigned(a.c.n_kv * a.row_blocks), 1};
+    const dim3 grid{unsigned(a.parts ? a.parts : a.c.n_seq), unsigned(a.c.n_kv * a.row_blocks), 1};
     return syn_launch(kernel, grid, kTcThreads, smem, s, a, maps);
 }
 
 }  // namespace
 
-int syn_tree_attention_tc(const TreeParams& a, int type, int parts, cudaStream_t s) {
+int syn_tree_attention_tc(const TreeParams& a, int type, cudaStream_t s) {
     if (a.c.hd <= 64)
-        return type == SYN_F16 ? launch<SYN_F16, 64>(a, parts, s) : type == SYN_Q8_0 ? launch<SYN_Q8_0, 64>(a, parts, s) : launch<SYN_Q4_0, 64>(a, parts, s);
-    return type == SYN_F16 ? launch<SYN_F16, 128>(a, parts, s) : type == SYN_Q8_0 ? launch<SYN_Q8_0, 128>(a, parts, s) : launch<SYN_Q4_0, 128>(a, parts, s);
+        return type == SYN_F16 ? launch<SYN_F16, 64>(a, s) : type == SYN_Q8_0 ? launch<SYN_Q8_0, 64>(a, s) : launch<SYN_Q4_0, 64>(a, s);
+    return type == SYN_F16 ? launch<SYN_F16, 128>(a, s) : type == SYN_Q8_0 ? launch<SYN_Q8_0, 128>(a, s) : launch<SYN_Q4_0, 128>(a, s);
 }
 
 // Bounded waits of the kernel that gave up on the current device (-1: unreadable).
