@@ -48,11 +48,29 @@ __device__ __forceinline__ void split2(float x, float y, uint32_t& hi, uint32_t&
     hi = bits(h);
     lo = bits(__floats2half2_rn(x - f.x, y - f.y));
 }
-// a += b of two floats each.
+// a += b, of two floats each.
 __device__ __forceinline__ void add2(float& a0, float& a1, float b0, float b1) {
     asm("{\n .reg .b64 a, b;\n mov.b64 a, {%0, %1};\n mov.b64 b, {%2, %3};\n add.rn.f32x2 a, a, b;\n mov.b64 {%0, %1}, a;\n}\n"
         : "+f"(a0), "+f"(a1)
         : "f"(b0), "f"(b1));
+}
+// a *= b; a = a f + b; a += b c, of two floats each.
+__device__ __forceinline__ void mul2(float& a0, float& a1, float b0, float b1) {
+    asm("{\n .reg .b64 a, b;\n mov.b64 a, {%0, %1};\n mov.b64 b, {%2, %3};\n mul.rn.f32x2 a, a, b;\n mov.b64 {%0, %1}, a;\n}\n"
+        : "+f"(a0), "+f"(a1)
+        : "f"(b0), "f"(b1));
+}
+__device__ __forceinline__ void fma2(float& a0, float& a1, float f0, float f1, float b0, float b1) {
+    asm("{\n .reg .b64 a, f, b;\n mov.b64 a, {%0, %1};\n mov.b64 f, {%2, %3};\n mov.b64 b, {%4, %5};\n"
+        " fma.rn.f32x2 a, a, f, b;\n mov.b64 {%0, %1}, a;\n}\n"
+        : "+f"(a0), "+f"(a1)
+        : "f"(f0), "f"(f1), "f"(b0), "f"(b1));
+}
+__device__ __forceinline__ void fma2_to(float& a0, float& a1, float b0, float b1, float c0, float c1) {
+    asm("{\n .reg .b64 a, b, c;\n mov.b64 a, {%0, %1};\n mov.b64 b, {%2, %3};\n mov.b64 c, {%4, %5};\n"
+        " fma.rn.f32x2 a, b, c, a;\n mov.b64 {%0, %1}, a;\n}\n"
+        : "+f"(a0), "+f"(a1)
+        : "f"(b0), "f"(b1), "f"(c0), "f"(c1));
 }
 // Bytes i and j of x as binary16 integers 1024 + byte.
 __device__ __forceinline__ __half2 bytes_h2(uint32_t x, uint32_t sel) { return half2_of(__byte_perm(x, 0x64646464u, sel)); }

@@ -5,15 +5,18 @@
 // with the A operand in tensor memory (Q for the whole call; P where S was)
 // and the tile in shared memory. As in the other kernel q and the
 // probabilities are two binary16 terms each, so S takes two products and O
-// two; a quantised tile is also two terms (its scale, brought to a common
-// power of two per tile, times its integers: 18 bits), so S and O take three
-// (the product of the two low terms is under 2^-22). A tile's O is read from
-// tensor memory and added to float registers, because sums in the tensor
-// core's accumulators lose a little with every product.
+// two; a quantised tile is also two terms (its scales times its integers: 18
+// bits), so S and O take three (the product of the two low terms is under
+// 2^-22). For that a position's row of K (V) is stored over the power of two
+// of its largest scale; a score takes K's power back, and the probabilities
+// take V's, their running maximum being that of probability times power, so
+// that neither V nor the probabilities leave binary16's range. A tile's O is
+// read from tensor memory and added to float registers, because sums in the
+// tensor core's accumulators lose a little with every product.
 //
 // Warps: 0-3 softmax (a thread owns a row: no exchange between lanes), 4-7
-// and 8-11 the two halves of O, 12-17 fill the tiles (F16: tensor copies;
-// quantised: integers to binary16), 18 issues the products. Tensor
+// and 8-11 the two halves of O, 12-18 fill the tiles (F16: tensor copies;
+// quantised: integers to binary16), 19 issues the products. Tensor
 // memory: Q high | Q low | two S (then P) | two O.
 //
 // Bound: the products take 16 (F16) or 24 cycles per position and KV head
@@ -26,7 +29,7 @@ using namespace syn;
 
 namespace {
 
-constexpr int kFillWarps = 6, kMmaWarp = 12 + kFillWarps, kTcThreads = (kMmaWarp + 1) * 32;
+constexpr int kFillWarps = 7, kMmaWarp = 12 + kFillWarps, kTcThreads = (kMmaWarp + 1) * 32;
 constexpr int kFill = 32 * kFillWarps;  // threads that fill tiles
 constexpr uint64_t kTcWaitNs = 2000000000ull;  // a wait gives up after 2 s
 constexpr int kEdgeTiles = kMaxTree / kTcTile + 2;  // tiles that hold rows of the tree
@@ -62,11 +65,11 @@ struct TcShared {
     uint64_t q_full, kv_full[5], kv_empty[5], s_full[2], p_full[4], o_full[2], o_empty[2], done;
     unsigned long long bad[kEdgeTiles];  // positions of a tree tile that hold values that are not finite
     float corr[4][kTcRows];              // a tile's factor of the rows' sums so far
-    float v_factor[4];                   // and of its O
-    float k_scale[8], v_scale[8];        // powers of two of a tile's terms
+    float k_pow[5][kTcTile];             // the powers of two of a stage's positions: K's,
+    float v_log[5][kTcTile];             // V's logarithm,
+    float v_inv[5][kTcTile];             // and V's inverse
     float m[kTcRows], l[kTcRows];
     float q_scale[kTcRows];              // the rows' factor of a product's scores
-    unsigned top[2][kFillWarps];                  // the fill warps' largest scales, of K and of V
     uint32_t tmem;
     int abort;
 };
@@ -234,56 +237,69 @@ __global__ void __launch_bounds__(kTcThreads, 1) tree_attn_tc_kernel(const TreeP
             if (!ok) break;
             if (live) {
                 tc_fence_after();
-                uint32_t s[2][32];
+                float s[2][32];
                 tmem_ld32(s[0], lanes + P::s + (j & 1) * kTcTile);
                 tmem_ld32(s[1], lanes + P::s + (j & 1) * kTcTile + 32);
-                const float cc = P::quant ? c * sh.k_scale[j & 7] : c;
                 tmem_wait_ld();
-                float x = -INFINITY;
-                if (!edge) {
+                // the scores, plus the logarithm of V's power
+                auto each4 = [&](auto f) {
 #pragma unroll
-                    for (int u = 0; u < 2; ++u)
-#pragma unroll
-                        for (int e = 0; e < 32; ++e) {
-                            const float v = __uint_as_float(s[u][e]) * cc;
-                            s[u][e] = __float_as_uint(v);
-                            x = fmaxf(x, v);
-                        }
-                } else {
+                    for (int e = 0; e < kTcTile; e += 4) f(reinterpret_cast<float(&)[4]>(s[e >> 5][e & 31]), e);
+                };
+                each4([&](float(&v)[4], int e) {
+                    if (P::quant) {
+                        const float4 kp = *reinterpret_cast<const float4*>(sh.k_pow[st] + e), vl = *reinterpret_cast<const float4*>(sh.v_log[st] + e);
+                        mul2(v[0], v[1], kp.x, kp.y);
+                        mul2(v[2], v[3], kp.z, kp.w);
+                        fma2(v[0], v[1], c, c, vl.x, vl.y);
+                        fma2(v[2], v[3], c, c, vl.z, vl.w);
+                    } else {
+                        mul2(v[0], v[1], c, c);
+                        mul2(v[2], v[3], c, c);
+                    }
+                });
+                if (edge) {
                     const unsigned long long bad = sh.bad[t - edge0], sees = tile_sees(a, seq, tok, t * kTcTile - len);
+                    each4([&](float(&v)[4], int e) {
 #pragma unroll
-                    for (int u = 0; u < 2; ++u)
-#pragma unroll
-                        for (int e = 0; e < 32; ++e) {
-                            const int p = 32 * u + e;
-                            float v = __uint_as_float(s[u][e]) * cc;
-                            if (bad >> p & 1ull) v = __uint_as_float(0x7fffffffu);
-                            if (!(sees >> p & 1ull)) v = -INFINITY;
-                            s[u][e] = __float_as_uint(v);
-                            x = fmaxf(x, v);
+                        for (int i = 0; i < 4; ++i) {
+                            if (bad >> (e + i) & 1ull) v[i] = __uint_as_float(0x7fffffffu);
+                            if (!(sees >> (e + i) & 1ull)) v[i] = -INFINITY;
                         }
+                    });
                 }
-                const float mn = fmaxf(m, x);
-                sh.corr[j & 3][r] = mn > m ? ex2(m - mn) : 1.0f;  // m = -inf: 0
-                l *= mn > m ? ex2(m - mn) : 1.0f;
+                float x = -INFINITY;
+                each4([&](float(&v)[4], int) { x = fmaxf(fmaxf(fmaxf(x, v[0]), fmaxf(v[1], v[2])), v[3]); });
+                const float mn = fmaxf(m, x), corr = mn > m ? ex2(m - mn) : 1.0f;  // m = -inf: 0
+                sh.corr[j & 3][r] = corr;
                 m = mn;
-                const float base = (m == -INFINITY ? 0.0f : m) - kPShift;
-                float sum[4] = {};
+                const float base = kPShift - (m == -INFINITY ? 0.0f : m);
+                float sum[4] = {l * corr, 0.0f, 0.0f, 0.0f};
 #pragma unroll
                 for (int u = 0; u < 4; ++u) {
                     uint32_t hi[8], lo[8];
 #pragma unroll
-                    for (int e = 0; e < 8; ++e) {
-                        const int at = 16 * (u & 1) + 2 * e;
-                        const float p0 = ex2(__uint_as_float(s[u >> 1][at]) - base), p1 = ex2(__uint_as_float(s[u >> 1][at + 1]) - base);
-                        sum[e & 3] += p0 + p1;
-                        split2(p0, p1, hi[e], lo[e]);
+                    for (int e = 0; e < 8; e += 2) {
+                        float(&v)[4] = reinterpret_cast<float(&)[4]>(s[u >> 1][16 * (u & 1) + 2 * e]);
+                        add2(v[0], v[1], base, base);
+                        add2(v[2], v[3], base, base);
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) v[i] = ex2(v[i]);
+                        if (P::quant) {  // the sum is the probabilities' own
+                            const float4 vi = *reinterpret_cast<const float4*>(sh.v_inv[st] + 16 * u + 2 * e);
+                            fma2_to(sum[0], sum[1], v[0], v[1], vi.x, vi.y);
+                            fma2_to(sum[2], sum[3], v[2], v[3], vi.z, vi.w);
+                        } else {
+                            add2(sum[0], sum[1], v[0], v[1]);
+                            add2(sum[2], sum[3], v[2], v[3]);
+                        }
+                        split2(v[0], v[1], hi[e], lo[e]);
+                        split2(v[2], v[3], hi[e + 1], lo[e + 1]);
                     }
                     tmem_st8(lanes + P::s + (j & 1) * kTcTile + 8 * u, hi);
                     tmem_st8(lanes + P::s + (j & 1) * kTcTile + 32 + 8 * u, lo);
                 }
-                l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
-                if (P::quant && tid == 0) sh.v_factor[j & 3] = sh.v_scale[j & 7];
+                l = (sum[0] + sum[1]) + (sum[2] + sum[3]);
                 tmem_wait_st();
             }
             tc_fence_before();
@@ -306,17 +322,15 @@ __global__ void __launch_bounds__(kTcThreads, 1) tree_attn_tc_kernel(const TreeP
             if (!ok) break;
             if (live) {
                 tc_fence_after();
-                const float f = sh.corr[j & 3][r], vf = P::quant ? sh.v_factor[j & 3] : 1.0f;
+                const float f = sh.corr[j & 3][r];
 #pragma unroll
                 for (int b = 0; b < W / 16; ++b) {
-                    uint32_t o[16];
+                    float o[16];
                     tmem_ld16(o, from + (j & 1) * HDP + 16 * b);
                     tmem_wait_ld();
 #pragma unroll
-                    for (int e = 0; e < 16; ++e) {
-                        const float v = __uint_as_float(o[e]);
-                        acc[16 * b + e] = fmaf(acc[16 * b + e], f, P::quant ? v * vf : v);
-                    }
+                    for (int e = 0; e < 16; e += 2)
+                        fma2(acc[16 * b + e], acc[16 * b + e + 1], f, f, o[e], o[e + 1]);
                 }
             }
             tc_fence_before();
@@ -403,110 +417,98 @@ __global__ void __launch_bounds__(kTcThreads, 1) tree_attn_tc_kernel(const TreeP
                     mbar_wait_bounded(&sh.kv_full[k % P::stages], uint32_t(k / P::stages) & 1, kTcWaitNs);
         } else {
             constexpr int VPC = TYPE == SYN_Q8_0 ? 16 : 32;          // values of 16 bytes of quants
-            constexpr int CP = HDP / VPC, NC = kTcTile * CP, N = (NC + kFill - 1) / kFill;  // chunks of a row, of a tile, of a thread
+            constexpr int CP = HDP / VPC, NI = kTcTile * CP / 32, N = (2 * NI + kFillWarps - 1) / kFillWarps;  // chunks of a row; sets of K; of a warp
             const int nb = hd / 32, chunks = hd / VPC;
             const size_t head = size_t(kvh) * a.c.max_ctx;
             const uint16_t *ks = reinterpret_cast<const uint16_t*>(kb + a.c.scale_plane), *vs = reinterpret_cast<const uint16_t*>(vb + a.c.scale_plane);
-            // a thread's chunks of K and of V: V's load while K is converted, the next K's while V is
-            struct Half {
-                uint4 q[N];
-                uint32_t d[N];  // scale bits
-            } kh, vh;
-            auto fetch = [&](Half& h, const char* base, const uint16_t* scales, int t) {
-#pragma unroll
-                for (int i = 0; i < N; ++i) {
-                    const int p = (i * kFill + ft) / CP, ch = (i * kFill + ft) % CP, pos = t * kTcTile + p;
-                    h.d[i] = 0;
-                    h.q[i] = make_uint4(0, 0, 0, 0);
-                    if (ch < chunks && pos < total && i * kFill + ft < NC) {
-                        const size_t rowi = head + pos;
-                        h.q[i] = __ldg(reinterpret_cast<const uint4*>(base + (rowi * chunks + ch) * 16));
-                        h.d[i] = __ldg(scales + rowi * nb + ch * VPC / 32);
-                    }
+            // A warp's share of a tile: sets of 32 chunks (16 bytes of quants) of K, then of V, every kFillWarps-th.
+            // A set of the next tile is requested as soon as this tile's is in hand.
+            uint4 q[N];
+            uint32_t d[N];  // scale bits
+            auto fetch = [&](int k, int t) {
+                const int i = k * kFillWarps + warp - 12;
+                if (i >= 2 * NI) return;
+                const bool v = i >= NI;
+                const int id = (v ? i - NI : i) * 32 + lane, p = id / CP, ch = id % CP, pos = t * kTcTile + p;
+                q[k] = make_uint4(0, 0, 0, 0);
+                d[k] = 0;
+                if (ch < chunks && pos < total) {
+                    const size_t rowi = head + pos;
+                    q[k] = __ldg(reinterpret_cast<const uint4*>((v ? vb : kb) + (rowi * chunks + ch) * 16));
+                    d[k] = __ldg((v ? vs : ks) + rowi * nb + ch * VPC / 32);
                 }
             };
-            // Converts a half of tile t into its two terms at `to`; the scale of the tile's integers goes to *scale.
-            // False when a wait has given up (in any of the warps).
-            auto convert = [&](Half& h, int which, bool ok, int j, unsigned char* to, float* scale) {
-                const int t = t0 + j;
-                uint32_t top = 0;
-#pragma unroll
-                for (int i = 0; i < N; ++i) {
-                    // a scale that is not finite: a tree row's position is bad (NaN for who sees it), others are NaN
-                    const int p = (i * kFill + ft) / CP;
-                    const bool finite = (h.d[i] & 0x7c00u) != 0x7c00u;
-                    if (!finite && t * kTcTile + p >= len) {
-                        h.d[i] = 0;
-                        atomicOr(&sh.bad[t - edge0], 1ull << p);
-                    }
-                    if (finite) top = max(top, h.d[i] & 0x7fffu);
+            auto convert = [&](int k, int j) {
+                const int i = k * kFillWarps + warp - 12, t = t0 + j, st = j % P::stages;
+                if (i >= 2 * NI) return;
+                const bool v = i >= NI;
+                const int id = (v ? i - NI : i) * 32 + lane, p = id / CP, ch = id % CP;  // past the head: scales of 0
+                const bool finite = (d[k] & 0x7c00u) != 0x7c00u;
+                if (!finite && t * kTcTile + p >= len) {  // a tree row's position is bad: NaN for who sees it
+                    d[k] = 0;
+                    atomicOr(&sh.bad[t - edge0], 1ull << p);
                 }
-                top = __reduce_max_sync(0xffffffffu, top);
-                if (lane == 0) sh.top[which][warp - 12] = ok ? top : ~0u;
-                asm volatile("bar.sync 1, %0;" ::"n"(kFill) : "memory");
+                // the position's largest scale to [2^8, 2^9): 127 of it is finite, and the low term reaches 2^-33 of it
+                uint32_t top = finite ? d[k] & 0x7fffu : 0u;
 #pragma unroll
-                for (int w = 0; w < kFillWarps; ++w) top = max(top, sh.top[which][w]);
-                if (top == ~0u) return false;
-                // the largest scale to [2^8, 2^9): 127 of it is finite, and the low term reaches 2^-33 of it
+                for (int o = 1; o < CP; o <<= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
                 const int e = 23 - int(max(top >> 10, 1u));
-                const float up = __uint_as_float(uint32_t(127 + e) << 23);
-                if (ft == 0) *scale = __uint_as_float(uint32_t(127 - e) << 23);
-                const __half2 zero = half2_of(TYPE == SYN_Q8_0 ? 0x64806480u : 0x64086408u);
-#pragma unroll
-                for (int i = 0; i < N; ++i) {
-                    const int p = (i * kFill + ft) / CP, ch = (i * kFill + ft) % CP;  // past the head: scales of 0
-                    if (NC % kFill && i * kFill + ft >= NC) break;
-                    const __half2 d = __float2half2_rn(f16_from_bits(uint16_t(h.d[i])) * up);
-                    // neighbouring threads store different 16-byte columns of the swizzled rows at a time: those of
-                    // the second 64 dims take the block's chunks in another order
-                    const int c0 = ch * (VPC / 8), turn = (c0 >> 3) * (VPC / 16);
-                    unsigned char* rowp = to + (c0 >> 3) * P::atom + p * 128;
-                    const int col = (((c0 ^ p) & 7) ^ turn) << 4;
-                    uint32_t w[4] = {h.q[i].x, h.q[i].y, h.q[i].z, h.q[i].w};
-                    if (TYPE == SYN_Q8_0) {
-#pragma unroll
-                        for (int e = 0; e < 4; ++e) w[e] ^= 0x80808080u;
-                        if (turn) {
-                            const uint32_t x = w[0], y = w[1];
-                            w[0] = w[2]; w[1] = w[3]; w[2] = x; w[3] = y;
-                        }
-                    } else if (turn) {
-#pragma unroll
-                        for (int e = 0; e < 4; ++e) w[e] = w[e] >> 4 | w[e] << 28;  // the high nibbles first
-                    }
-#pragma unroll
-                    for (int k = 0; k < VPC / 8; ++k) {  // 8 dims: one chunk of each term
-                        uint32_t hi[4], lo[4];
-#pragma unroll
-                        for (int e2 = 0; e2 < 2; ++e2) {
-                            uint32_t x = w[2 * (k & 1) + e2];
-                            if (TYPE == SYN_Q4_0) x = (k >> 1 ? (turn ? x << 4 | x >> 28 : x >> 4) : x) & 0x0f0f0f0fu;
-#pragma unroll
-                            for (int o = 0; o < 2; ++o) {
-                                const __half2 v = __hsub2(bytes_h2(x, o ? 0x4342u : 0x4140u), zero);
-                                const __half2 y = __hmul2(v, d);
-                                hi[2 * e2 + o] = bits(y);
-                                lo[2 * e2 + o] = bits(__hfma2(v, d, __hneg2(y)));
-                            }
-                        }
-                        unsigned char* at = rowp + (col ^ (k << 4));
-                        *reinterpret_cast<uint4*>(at) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
-                        *reinterpret_cast<uint4*>(at + P::tile) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
+                const float up = __uint_as_float(uint32_t(127 + e) << 23), down = __uint_as_float(uint32_t(127 - e) << 23);
+                if (ch == 0) {
+                    if (!v) {
+                        sh.k_pow[st][p] = down;
+                    } else {
+                        sh.v_log[st][p] = float(-e);
+                        sh.v_inv[st][p] = up;
                     }
                 }
-                return true;
+                const __half2 zero = half2_of(TYPE == SYN_Q8_0 ? 0x64806480u : 0x64086408u);
+                const __half2 scale = __float2half2_rn(f16_from_bits(uint16_t(d[k])) * up);
+                // neighbouring threads store different 16-byte columns of the swizzled rows at a time: those of the
+                // second 64 dims take the chunk's eights in another order
+                const int c0 = ch * (VPC / 8), turn = (c0 >> 3) * (VPC / 16);
+                unsigned char* rowp = tiles + st * P::stage + (v ? P::v_hi : 0) + (c0 >> 3) * P::atom + p * 128;
+                const int col = (((c0 ^ p) & 7) ^ turn) << 4;
+                uint32_t w[4] = {q[k].x, q[k].y, q[k].z, q[k].w};
+                if (TYPE == SYN_Q8_0) {
+#pragma unroll
+                    for (int x = 0; x < 4; ++x) w[x] ^= 0x80808080u;
+                    if (turn) {
+                        const uint32_t x = w[0], y = w[1];
+                        w[0] = w[2]; w[1] = w[3]; w[2] = x; w[3] = y;
+                    }
+                }
+                const int sh0 = TYPE == SYN_Q4_0 && turn ? 4 : 0;  // Q4_0: the high nibbles first
+#pragma unroll
+                for (int g = 0; g < VPC / 8; ++g) {  // 8 dims: one 16-byte column of each term
+                    uint32_t hi[4], lo[4];
+#pragma unroll
+                    for (int x2 = 0; x2 < 2; ++x2) {
+                        uint32_t x = w[2 * (g & 1) + x2];
+                        if (TYPE == SYN_Q4_0) x = x >> (g >> 1 ? 4 - sh0 : sh0) & 0x0f0f0f0fu;
+#pragma unroll
+                        for (int o = 0; o < 2; ++o) {
+                            const __half2 n = __hsub2(bytes_h2(x, o ? 0x4342u : 0x4140u), zero);
+                            const __half2 y = __hmul2(n, scale);
+                            hi[2 * x2 + o] = bits(y);
+                            lo[2 * x2 + o] = bits(__hfma2(n, scale, __hneg2(y)));
+                        }
+                    }
+                    unsigned char* at = rowp + (col ^ (g << 4));
+                    *reinterpret_cast<uint4*>(at) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
+                    *reinterpret_cast<uint4*>(at + P::tile) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
+                }
             };
-            fetch(kh, kb, ks, t0);
-            fetch(vh, vb, vs, t0);
+#pragma unroll
+            for (int k = 0; k < N; ++k) fetch(k, t0);
             for (int j = 0; j < n; ++j) {
-                const int st = j % P::stages, t = t0 + j;
-                bool ok = j != 1 || warp_wait(&sh.q_full, 0, sh);
-                if (j >= P::stages) ok = ok && warp_wait(&sh.kv_empty[st], uint32_t(j / P::stages - 1) & 1, sh);
-                unsigned char* to = tiles + st * P::stage;
-                if (!convert(kh, 0, ok, j, to, &sh.k_scale[j & 7])) break;
-                if (j + 1 < n) fetch(kh, kb, ks, t + 1);
-                convert(vh, 1, true, j, to + P::v_hi, &sh.v_scale[j & 7]);
-                if (j + 1 < n) fetch(vh, vb, vs, t + 1);
+                if (j == 1 && !warp_wait(&sh.q_full, 0, sh)) break;
+                if (j >= P::stages && !warp_wait(&sh.kv_empty[j % P::stages], uint32_t(j / P::stages - 1) & 1, sh)) break;
+#pragma unroll
+                for (int k = 0; k < N; ++k) {
+                    convert(k, j);
+                    if (j + 1 < n) fetch(k, t0 + j + 1);
+                }
                 full(j);
             }
         }
