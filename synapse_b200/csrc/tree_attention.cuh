@@ -41,13 +41,6 @@ __device__ __forceinline__ float ex2(float x) {
 }
 __device__ __forceinline__ uint32_t bits(__half2 h) { return *reinterpret_cast<uint32_t*>(&h); }
 __device__ __forceinline__ __half2 half2_of(uint32_t u) { return *reinterpret_cast<__half2*>(&u); }
-// (x, y) as binary16 pairs hi + lo.
-__device__ __forceinline__ void split2(float x, float y, uint32_t& hi, uint32_t& lo) {
-    const __half2 h = __floats2half2_rn(x, y);
-    const float2 f = __half22float2(h);
-    hi = bits(h);
-    lo = bits(__floats2half2_rn(x - f.x, y - f.y));
-}
 // a += b, of two floats each.
 __device__ __forceinline__ void add2(float& a0, float& a1, float b0, float b1) {
     asm("{\n .reg .b64 a, b;\n mov.b64 a, {%0, %1};\n mov.b64 b, {%2, %3};\n add.rn.f32x2 a, a, b;\n mov.b64 {%0, %1}, a;\n}\n"
@@ -71,6 +64,14 @@ __device__ __forceinline__ void fma2_to(float& a0, float& a1, float b0, float b1
         " fma.rn.f32x2 a, b, c, a;\n mov.b64 {%0, %1}, a;\n}\n"
         : "+f"(a0), "+f"(a1)
         : "f"(b0), "f"(b1), "f"(c0), "f"(c1));
+}
+// (x, y) as binary16 pairs hi + lo.
+__device__ __forceinline__ void split2(float x, float y, uint32_t& hi, uint32_t& lo) {
+    const __half2 h = __floats2half2_rn(x, y);
+    float2 f = __half22float2(h);
+    fma2(f.x, f.y, -1.0f, -1.0f, x, y);
+    hi = bits(h);
+    lo = bits(__floats2half2_rn(f.x, f.y));
 }
 // Bytes i and j of x as binary16 integers 1024 + byte.
 __device__ __forceinline__ __half2 bytes_h2(uint32_t x, uint32_t sel) { return half2_of(__byte_perm(x, 0x64646464u, sel)); }

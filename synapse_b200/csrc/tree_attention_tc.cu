@@ -14,11 +14,9 @@
 // read from tensor memory and added to float registers, because sums in the
 // tensor core's accumulators lose a little with every product.
 //
-// Warps: 0-3 and 4-7 softmax (a thread owns a row's half of the tile: two
-// threads exchange their maxima, no lanes; one thread for the whole row left
-// the products waiting, 2200 cycles a tile against 1024), 8-11 and 12-15 the
-// two halves of O, 16-22 fill the tiles (F16: tensor copies; quantised:
-// integers to binary16), 23 issues the products. Tensor
+// Warps: 0-3 softmax (a thread owns a row: no exchange between lanes), 4-7
+// and 8-11 the two halves of O, 12-18 fill the tiles (F16: tensor copies;
+// quantised: integers to binary16), 19 issues the products. Tensor
 // memory: Q high | Q low | two S (then P) | two O.
 //
 // Bound: the products take 16 (F16) or 24 cycles per position and KV head
@@ -31,7 +29,7 @@ using namespace syn;
 
 namespace {
 
-constexpr int kFillWarps = 7, kFillWarp0 = 16, kMmaWarp = kFillWarp0 + kFillWarps, kTcThreads = (kMmaWarp + 1) * 32;
+constexpr int kFillWarps = 7, kFillWarp0 = 12, kMmaWarp = kFillWarp0 + kFillWarps, kTcThreads = (kMmaWarp + 1) * 32;
 constexpr int kFill = 32 * kFillWarps;  // threads that fill tiles
 constexpr uint64_t kTcWaitNs = 2000000000ull;  // a wait gives up after 2 s
 constexpr uint32_t kTcNapNs = 1000000;         // and sleeps in the barrier meanwhile: polling takes issue slots
@@ -71,17 +69,15 @@ struct TcShared {
     float k_pow[5][kTcTile];             // the powers of two of a stage's positions: K's,
     float v_log[5][kTcTile];             // V's logarithm,
     float v_inv[5][kTcTile];             // and V's inverse
-    float m[kTcRows], l[2][kTcRows];
-    float top[2][2][kTcRows];            // the halves' maxima of a row
-    int failed[2];                       // a wait of the softmax warps gave up
+    float m[kTcRows], l[kTcRows];
     float q_scale[kTcRows];              // the rows' factor of a product's scores
     uint32_t tmem;
     int abort;
 };
 
-// Waits for phase `parity`; false when it gave up, here or in another thread of the CTA.
-__device__ __forceinline__ bool tc_wait(uint64_t* bar, uint32_t parity, TcShared& sh) {
-    if (mbar_try_wait_sleep(bar, parity, kTcNapNs)) return true;
+// Waits for phase `parity`; false when it gave up, here or in another thread of the CTA. The way of a barrier that is
+// not ready yet is a call: the loops stay small enough for the instruction cache that the roles share.
+__device__ __noinline__ bool tc_wait_on(uint64_t* bar, uint32_t parity, TcShared& sh) {
     const uint64_t t0 = global_ns();
     for (;;) {
         if (mbar_try_wait_sleep(bar, parity, kTcNapNs)) return true;
@@ -94,7 +90,9 @@ __device__ __forceinline__ bool tc_wait(uint64_t* bar, uint32_t parity, TcShared
     }
 }
 __device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity, TcShared& sh) {
-    return __all_sync(0xffffffffu, tc_wait(bar, parity, sh));
+    bool ok = mbar_try_wait(bar, parity);
+    if (!ok) ok = tc_wait_on(bar, parity, sh);
+    return __all_sync(0xffffffffu, ok);
 }
 
 // Byte offset of 16-byte chunk c (8 dims) of position p in a swizzled tile.
@@ -143,7 +141,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) tree_attn_tc_kernel(const TreeP
     const int edge0 = len / kTcTile;  // the first tile with a row of the tree
 
     if (tid == 0) {
-        mbar_init(&sh.q_full, 256);
+        mbar_init(&sh.q_full, 128);
         for (int i = 0; i < P::stages; ++i) {
             mbar_init(&sh.kv_full[i], kFillWarps);
             mbar_init(&sh.kv_empty[i], 1);
@@ -153,10 +151,10 @@ __global__ void __launch_bounds__(kTcThreads, 1) tree_attn_tc_kernel(const TreeP
             mbar_init(&sh.o_full[i], 1);
             mbar_init(&sh.o_empty[i], 256);
         }
-        for (int i = 0; i < 4; ++i) mbar_init(&sh.p_full[i], 256);
+        for (int i = 0; i < 4; ++i) mbar_init(&sh.p_full[i], 128);
         mbar_init(&sh.done, 1);
         mbar_init_fence();
-        sh.abort = sh.failed[0] = sh.failed[1] = 0;
+        sh.abort = 0;
     }
     if (tid < kEdgeTiles) sh.bad[tid] = 0;
     if (warp == kMmaWarp) tmem_alloc_all(&sh.tmem);
@@ -193,7 +191,8 @@ __global__ void __launch_bounds__(kTcThreads, 1) tree_attn_tc_kernel(const TreeP
             for (int e = 0; e < V; ++e) top = max(top, __float_as_uint(fabsf(x[i][e])));
             float up, down;
             q_factor(__uint_as_float(__reduce_max_sync(0xffffffffu, top)), up, down);
-            if (lane == 0) sh.q_scale[r] = a.scale_log2 * down;
+            if (lane == 0) sh.q_scale[r] = fabsf(a.scale_log2) * down;
+            if (a.scale_log2 < 0.0f) up = -up;  // the scores' factor is positive: maxima may be taken before it
             unsigned char* at = q_stage + r * 2 * kQPitch + lane * V * 2;
 #pragma unroll
             for (int e = 0; e < V; e += 2) {
@@ -209,24 +208,24 @@ __global__ void __launch_bounds__(kTcThreads, 1) tree_attn_tc_kernel(const TreeP
     tc_fence_after();
     const uint32_t tm = sh.tmem;
 
-    if (warp < 8) {
-        // ---- softmax: thread = row and half of the tile ---------------------------------
+    if (warp < 4) {
+        // ---- softmax: thread = row -------------------------------------------------
         const bool live = 32 * (warp & 3) < rows;  // the warp has rows
-        const int r = tid & 127, half = warp >> 2, tok = (row0 + r) / a.group;
+        const int r = tid & 127, row = row0 + r;
+        const int tok = row / a.group;
         const uint32_t lanes = tm + (uint32_t(32 * (warp & 3)) << 16);
         const float c = sh.q_scale[r];
         if (live) {
-            // the high terms by one half's warps, the low ones by the other's
-            const uint32_t to = lanes + (half ? P::q_lo : P::q_hi);
 #pragma unroll
-            for (int b = 0; b < HDP / 32; ++b) {
+            for (int b = 0; b < HDP / 16; ++b) {  // 16 columns: 32 dims of the high, then of the low term
+                const int term = b / (HDP / 32), at = b % (HDP / 32);
                 uint32_t w[16];
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
-                    const uint4 x = *reinterpret_cast<const uint4*>(q_stage + (r * 2 + half) * kQPitch + b * 64 + e * 16);
+                    const uint4 x = *reinterpret_cast<const uint4*>(q_stage + (r * 2 + term) * kQPitch + at * 64 + e * 16);
                     w[4 * e] = x.x; w[4 * e + 1] = x.y; w[4 * e + 2] = x.z; w[4 * e + 3] = x.w;
                 }
-                tmem_st16(to + 16 * b, w);
+                tmem_st16(lanes + (term ? P::q_lo : P::q_hi) + 16 * at, w);
             }
             tmem_wait_st();
         }
@@ -239,63 +238,65 @@ __global__ void __launch_bounds__(kTcThreads, 1) tree_attn_tc_kernel(const TreeP
             const bool edge = t >= edge0;
             bool ok = warp_wait(&sh.s_full[j & 1], uint32_t(j >> 1) & 1, sh);
             if (ok && (P::quant || edge)) ok = warp_wait(&sh.kv_full[st], uint32_t(j / P::stages) & 1, sh);
-            if (!ok) sh.failed[j & 1] = 1;
-            const uint32_t buf = lanes + P::s + (j & 1) * kTcTile;
-            float s[32], x = -INFINITY;
-            auto each4 = [&](auto f) {
-#pragma unroll
-                for (int e = 0; e < 32; e += 4) f(reinterpret_cast<float(&)[4]>(s[e]), 32 * half + e, e);
-            };
-            if (live && ok) {
+            if (!ok) break;
+            if (live) {
                 tc_fence_after();
-                tmem_ld32(s, buf + 32 * half);
+                float s[2][32];
+                tmem_ld32(s[0], lanes + P::s + (j & 1) * kTcTile);
+                tmem_ld32(s[1], lanes + P::s + (j & 1) * kTcTile + 32);
                 tmem_wait_ld();
-                // the scores, plus the logarithm of V's power
-                each4([&](float(&v)[4], int at, int) {
-                    if (P::quant) {
-                        const float4 kp = *reinterpret_cast<const float4*>(sh.k_pow[st] + at), vl = *reinterpret_cast<const float4*>(sh.v_log[st] + at);
+                // F16: raw scores, times c > 0 in the exponent; quantised: times K's power and c, plus the logarithm of V's
+                auto each4 = [&](auto f) {
+#pragma unroll
+                    for (int e = 0; e < kTcTile; e += 4) f(reinterpret_cast<float(&)[4]>(s[e >> 5][e & 31]), e);
+                };
+                if (P::quant)
+                    each4([&](float(&v)[4], int e) {
+                        const float4 kp = *reinterpret_cast<const float4*>(sh.k_pow[st] + e), vl = *reinterpret_cast<const float4*>(sh.v_log[st] + e);
                         mul2(v[0], v[1], kp.x, kp.y);
                         mul2(v[2], v[3], kp.z, kp.w);
                         fma2(v[0], v[1], c, c, vl.x, vl.y);
                         fma2(v[2], v[3], c, c, vl.z, vl.w);
-                    } else {
-                        mul2(v[0], v[1], c, c);
-                        mul2(v[2], v[3], c, c);
-                    }
-                });
+                    });
                 if (edge) {
                     const unsigned long long bad = sh.bad[t - edge0], sees = tile_sees(a, seq, tok, t * kTcTile - len);
-                    each4([&](float(&v)[4], int at, int) {
+                    const uint32_t bw[2] = {uint32_t(bad), uint32_t(bad >> 32)}, sw[2] = {uint32_t(sees), uint32_t(sees >> 32)};
 #pragma unroll
-                        for (int i = 0; i < 4; ++i) {
-                            if (bad >> (at + i) & 1ull) v[i] = __uint_as_float(0x7fffffffu);
-                            if (!(sees >> (at + i) & 1ull)) v[i] = -INFINITY;
-                        }
-                    });
+                    for (int u = 0; u < 2; ++u)
+#pragma unroll
+                        for (int e = 0; e < 32; ++e)
+                            if (!(sw[u] >> e & 1u)) s[u][e] = -INFINITY;
+                            else if (bw[u] >> e & 1u) s[u][e] = __uint_as_float(0x7fffffffu);
                 }
-                each4([&](float(&v)[4], int, int) { x = fmaxf(fmaxf(fmaxf(x, v[0]), fmaxf(v[1], v[2])), v[3]); });
-                sh.top[j & 1][half][r] = x;
-            }
-            asm volatile("bar.sync 1, 256;" ::: "memory");  // both halves have read their scores, too
-            if (*reinterpret_cast<volatile int*>(&sh.failed[j & 1])) break;
-            if (live) {
-                const float mn = fmaxf(m, fmaxf(x, sh.top[j & 1][half ^ 1][r])), corr = mn > m ? ex2(m - mn) : 1.0f;  // m = -inf: 0
-                if (half == 0) sh.corr[j & 3][r] = corr;
+                float x[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+                each4([&](float(&v)[4], int e) {
+                    float& y = x[(e >> 2) & 3];
+                    y = fmaxf(fmaxf(fmaxf(y, v[0]), fmaxf(v[1], v[2])), v[3]);
+                });
+                const float most = fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3]));
+                const float mn = fmaxf(m, P::quant || most == -INFINITY ? most : most * c);
+                const float corr = mn > m ? ex2(m - mn) : 1.0f;  // m = -inf: 0
+                sh.corr[j & 3][r] = corr;
                 m = mn;
                 const float base = kPShift - (m == -INFINITY ? 0.0f : m);
                 float sum[4] = {l * corr, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-                for (int u = 0; u < 2; ++u) {
+                for (int u = 0; u < 4; ++u) {
                     uint32_t hi[8], lo[8];
 #pragma unroll
                     for (int e = 0; e < 8; e += 2) {
-                        float(&v)[4] = reinterpret_cast<float(&)[4]>(s[16 * u + 2 * e]);
-                        add2(v[0], v[1], base, base);
-                        add2(v[2], v[3], base, base);
+                        float(&v)[4] = reinterpret_cast<float(&)[4]>(s[u >> 1][16 * (u & 1) + 2 * e]);
+                        if (P::quant) {
+                            add2(v[0], v[1], base, base);
+                            add2(v[2], v[3], base, base);
+                        } else {
+                            fma2(v[0], v[1], c, c, base, base);
+                            fma2(v[2], v[3], c, c, base, base);
+                        }
 #pragma unroll
                         for (int i = 0; i < 4; ++i) v[i] = ex2(v[i]);
                         if (P::quant) {  // the sum is the probabilities' own
-                            const float4 vi = *reinterpret_cast<const float4*>(sh.v_inv[st] + 32 * half + 16 * u + 2 * e);
+                            const float4 vi = *reinterpret_cast<const float4*>(sh.v_inv[st] + 16 * u + 2 * e);
                             fma2_to(sum[0], sum[1], v[0], v[1], vi.x, vi.y);
                             fma2_to(sum[2], sum[3], v[2], v[3], vi.z, vi.w);
                         } else {
@@ -305,8 +306,8 @@ __global__ void __launch_bounds__(kTcThreads, 1) tree_attn_tc_kernel(const TreeP
                         split2(v[0], v[1], hi[e], lo[e]);
                         split2(v[2], v[3], hi[e + 1], lo[e + 1]);
                     }
-                    tmem_st8(buf + 16 * half + 8 * u, hi);
-                    tmem_st8(buf + 32 + 16 * half + 8 * u, lo);
+                    tmem_st8(lanes + P::s + (j & 1) * kTcTile + 8 * u, hi);
+                    tmem_st8(lanes + P::s + (j & 1) * kTcTile + 32 + 8 * u, lo);
                 }
                 l = (sum[0] + sum[1]) + (sum[2] + sum[3]);
                 tmem_wait_st();
@@ -314,12 +315,12 @@ __global__ void __launch_bounds__(kTcThreads, 1) tree_attn_tc_kernel(const TreeP
             tc_fence_before();
             mbar_arrive(&sh.p_full[j & 3]);
         }
-        if (half == 0) sh.m[r] = m;
-        sh.l[half][r] = l;
-    } else if (warp < 16) {
+        sh.m[r] = m;
+        sh.l[r] = l;
+    } else if (warp < 12) {
         // ---- O: thread = row, half of the dims -----------------------------------------
         constexpr int W = HDP / 2;
-        const int half = (warp - 8) >> 2, r = tid & 127;
+        const int half = (warp - 4) >> 2, r = tid & 127;
         const bool live = 32 * (warp & 3) < rows;
         const uint32_t from = tm + (uint32_t(32 * (warp & 3)) << 16) + P::o + half * W;
         float acc[W];
@@ -333,20 +334,20 @@ __global__ void __launch_bounds__(kTcThreads, 1) tree_attn_tc_kernel(const TreeP
                 tc_fence_after();
                 const float f = sh.corr[j & 3][r];
 #pragma unroll
-                for (int b = 0; b < W / 8; ++b) {
-                    float o[8];
-                    tmem_ld8(o, from + (j & 1) * HDP + 8 * b);
+                for (int b = 0; b < W / 16; ++b) {
+                    float o[16];
+                    tmem_ld16(o, from + (j & 1) * HDP + 16 * b);
                     tmem_wait_ld();
 #pragma unroll
-                    for (int e = 0; e < 8; e += 2)
-                        fma2(acc[8 * b + e], acc[8 * b + e + 1], f, f, o[e], o[e + 1]);
+                    for (int e = 0; e < 16; e += 2)
+                        fma2(acc[16 * b + e], acc[16 * b + e + 1], f, f, o[e], o[e + 1]);
                 }
             }
             tc_fence_before();
             mbar_arrive(&sh.o_empty[j & 1]);
         }
-        asm volatile("bar.sync 2, 512;" ::: "memory");  // the softmax warps' m and l
-        const float l = sh.l[0][r] + sh.l[1][r];
+        asm volatile("bar.sync 2, 384;" ::: "memory");  // the softmax warps' m and l
+        const float l = sh.l[r];
         if (live && r < rows && !*reinterpret_cast<volatile int*>(&sh.abort)) {
             const bool whole = a.parts == 0;
             const int row = row0 + r, tok = row / a.group, h = kvh * a.group + row - tok * a.group;
@@ -362,7 +363,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) tree_attn_tc_kernel(const TreeP
         }
     } else if (warp < kMmaWarp) {
         // ---- tiles ------------------------------------------------------------------------
-        const int ft = tid - 32 * kFillWarp0;
+        const int fw = warp - kFillWarp0, ft = fw * 32 + lane;
         const char *kb = a.c.k + size_t(seq) * a.c.seq_stride, *vb = a.c.v + size_t(seq) * a.c.seq_stride;
         auto full = [&](int j) {
             fence_async_shared();
@@ -380,7 +381,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) tree_attn_tc_kernel(const TreeP
                 if (j >= P::stages && !warp_wait(&sh.kv_empty[st], uint32_t(j / P::stages - 1) & 1, sh)) break;
                 if (t < edge0 && hd % 64 == 0) {
                     if (lane == 0) {
-                        if (warp == kFillWarp0) {
+                        if (fw == 0) {
                             const uint32_t to = tiles_s + st * P::stage;
                             fence_async_shared();  // q was staged here
                             mbar_expect_tx(&sh.kv_full[st], 2 * uint32_t(hd) * kTcTile * 2);
@@ -435,7 +436,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) tree_attn_tc_kernel(const TreeP
             uint4 q[N];
             uint32_t d[N];  // scale bits
             auto fetch = [&](int k, int t) {
-                const int i = k * kFillWarps + warp - kFillWarp0;
+                const int i = k * kFillWarps + fw;
                 if (i >= 2 * NI) return;
                 const bool v = i >= NI;
                 const int id = (v ? i - NI : i) * 32 + lane, p = id / CP, ch = id % CP, pos = t * kTcTile + p;
@@ -448,7 +449,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) tree_attn_tc_kernel(const TreeP
                 }
             };
             auto convert = [&](int k, int j) {
-                const int i = k * kFillWarps + warp - kFillWarp0, t = t0 + j, st = j % P::stages;
+                const int i = k * kFillWarps + fw, t = t0 + j, st = j % P::stages;
                 if (i >= 2 * NI) return;
                 const bool v = i >= NI;
                 const int id = (v ? i - NI : i) * 32 + lane, p = id / CP, ch = id % CP;  // past the head: scales of 0
@@ -574,7 +575,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) tree_attn_tc_kernel(const TreeP
         mbar_wait_bounded(&sh.done, 0, kTcWaitNs);
     }
     __syncwarp();
-    if (warp < 8) asm volatile("bar.sync 2, 512;" ::: "memory");
+    if (warp < 4) asm volatile("bar.sync 2, 384;" ::: "memory");
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
