@@ -158,55 +158,66 @@ __global__ void __launch_bounds__(kTcThreads, 1) tree_attn_tc_kernel(const TreeP
     }
     if (tid < kEdgeTiles) sh.bad[tid] = 0;
     if (warp == kMmaWarp) tmem_alloc_all(&sh.tmem);
-    // q: a warp takes 8 rows (lane = dims), split into the tile memory that the fill warps leave free until q_full
-    constexpr int kQPitch = HDP * 2 + 16;
-    unsigned char* q_stage = tiles + P::stage;  // [row][high | low]
-    if (warp < kTcRows / 8) {
-        constexpr int V = HDP / 32;
-        const bool vec = V == 4 && ((reinterpret_cast<uintptr_t>(a.q) & 15) | (a.q_stride & 3)) == 0;
-        float x[8][V];
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-            const int r = 8 * warp + i, row = row0 + r, tok = row / a.group, h = row - tok * a.group;
-            const float* q = a.q + (size_t(seq) * a.n_tree + tok) * a.q_stride + size_t(kvh * a.group + h) * hd + lane * V;
-#pragma unroll
-            for (int e = 0; e < V; ++e) x[i][e] = 0.0f;
-            if (r < rows && lane * V < hd) {
-                if constexpr (V == 4) {
-                    if (vec) {
-                        const float4 f = __ldg(reinterpret_cast<const float4*>(q));
-                        x[i][0] = f.x; x[i][1] = f.y; x[i][2] = f.z; x[i][3] = f.w;
-                    }
-                }
-                if (!vec)
-#pragma unroll
-                    for (int e = 0; e < V; ++e) x[i][e] = __ldg(q + e);
-            }
-        }
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-            const int r = 8 * warp + i;
-            uint32_t top = 0;
-#pragma unroll
-            for (int e = 0; e < V; ++e) top = max(top, __float_as_uint(fabsf(x[i][e])));
-            float up, down;
-            q_factor(__uint_as_float(__reduce_max_sync(0xffffffffu, top)), up, down);
-            if (lane == 0) sh.q_scale[r] = fabsf(a.scale_log2) * down;
-            if (a.scale_log2 < 0.0f) up = -up;  // the scores' factor is positive: maxima may be taken before it
-            unsigned char* at = q_stage + r * 2 * kQPitch + lane * V * 2;
-#pragma unroll
-            for (int e = 0; e < V; e += 2) {
-                uint32_t hi, lo;
-                split2(x[i][e] * up, x[i][e + 1] * up, hi, lo);
-                *reinterpret_cast<uint32_t*>(at + 2 * e) = hi;
-                *reinterpret_cast<uint32_t*>(at + kQPitch + 2 * e) = lo;
-            }
-        }
-    }
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
     const uint32_t tm = sh.tmem;
+
+    // q, by all but the fill warps, which start on the tiles: a row at a time (lane = dims), as it is and then split in
+    // place, in the tile memory that they leave free until q_full. Rows past the last stay what they are; they reach no other row's output.
+    constexpr int kQPitch = HDP * 2 + 16;
+    unsigned char* q_stage = tiles + P::stage;  // [row][high | low]
+    if (warp < kFillWarp0) {
+        constexpr int V = HDP / 32;
+        const bool vec = ((reinterpret_cast<uintptr_t>(a.q) & 15) | (a.q_stride & 3)) == 0;
+        const float* q = a.q + size_t(seq) * a.n_tree * a.q_stride + size_t(kvh) * a.group * hd;
+        int tok = (row0 + warp) / a.group, h = row0 + warp - tok * a.group;
+#pragma unroll 1
+        for (int r = warp; r < rows; r += kFillWarp0) {
+            const float* src = q + size_t(tok) * a.q_stride + h * hd;
+            unsigned char* to = q_stage + r * 2 * kQPitch;
+            if (vec) {
+                if (4 * lane < HDP) cp16(smem_addr(to) + 16 * lane, 4 * lane < hd ? src + 4 * lane : src, 4 * lane < hd);
+            } else {
+#pragma unroll 1
+                for (int d = lane; d < HDP; d += 32) reinterpret_cast<float*>(to)[d] = d < hd ? __ldg(src + d) : 0.0f;
+            }
+            for (h += kFillWarp0; h >= a.group; h -= a.group) ++tok;
+        }
+        cp_commit();
+        cp_wait<0>();
+        __syncwarp();
+#pragma unroll 1
+        for (int r = warp; r < rows; r += kFillWarp0) {
+            unsigned char* row = q_stage + r * 2 * kQPitch;
+            float x[V];
+            uint32_t top = 0;
+            if constexpr (V == 4) {
+                const float4 f = reinterpret_cast<const float4*>(row)[lane];
+                x[0] = f.x; x[1] = f.y; x[2] = f.z; x[3] = f.w;
+            } else {
+                const float2 f = reinterpret_cast<const float2*>(row)[lane];
+                x[0] = f.x; x[1] = f.y;
+            }
+#pragma unroll
+            for (int e = 0; e < V; ++e) top = max(top, __float_as_uint(fabsf(x[e])));
+            float up, down;
+            q_factor(__uint_as_float(__reduce_max_sync(0xffffffffu, top)), up, down);
+            if (lane == 0) sh.q_scale[r] = fabsf(a.scale_log2) * down;
+            if (a.scale_log2 < 0.0f) up = -up;  // the scores' factor is positive: maxima may be taken before it
+            uint32_t hi[V / 2], lo[V / 2];
+#pragma unroll
+            for (int e = 0; e < V; e += 2) split2(x[e] * up, x[e + 1] * up, hi[e / 2], lo[e / 2]);
+            if constexpr (V == 4) {
+                reinterpret_cast<uint2*>(row)[lane] = make_uint2(hi[0], hi[1]);
+                reinterpret_cast<uint2*>(row + kQPitch)[lane] = make_uint2(lo[0], lo[1]);
+            } else {
+                reinterpret_cast<uint32_t*>(row)[lane] = hi[0];
+                reinterpret_cast<uint32_t*>(row + kQPitch)[lane] = lo[0];
+            }
+        }
+        asm volatile("bar.sync 2, 384;" ::: "memory");
+    }
 
     if (warp < 4) {
         // ---- softmax: thread = row -------------------------------------------------
@@ -348,18 +359,35 @@ __global__ void __launch_bounds__(kTcThreads, 1) tree_attn_tc_kernel(const TreeP
         }
         asm volatile("bar.sync 2, 384;" ::: "memory");  // the softmax warps' m and l
         const float l = sh.l[r];
-        if (live && r < rows && !*reinterpret_cast<volatile int*>(&sh.abort)) {
-            const bool whole = a.parts == 0;
-            const int row = row0 + r, tok = row / a.group, h = kvh * a.group + row - tok * a.group;
-            const size_t part = (size_t(blockIdx.x) * gridDim.y + blockIdx.y) * kTcRows + r;
-            float* out = whole ? a.out + ((size_t(seq) * a.n_tree + tok) * a.n_head + h) * hd : a.part_o + part * hd;
-            const float inv = !whole ? 1.0f : l == 0.0f ? 0.0f : 1.0f / l;
+        // through the tile memory (every product has read it: the last O was waited for), for whole-line stores
+        constexpr int pitch = HDP + 4;
+        float* stage = reinterpret_cast<float*>(tiles);
+        const bool whole = a.parts == 0;
+        const float inv = !whole ? 1.0f : l == 0.0f ? 0.0f : 1.0f / l;
+        const size_t part = (size_t(blockIdx.x) * gridDim.y + blockIdx.y) * kTcRows;
+        if (live) {
 #pragma unroll
             for (int d = 0; d < W; d += 4)
-                if (half * W + d < hd)
-                    *reinterpret_cast<float4*>(out + half * W + d) =
-                        make_float4(acc[d] * inv, acc[d + 1] * inv, acc[d + 2] * inv, acc[d + 3] * inv);
-            if (!whole && half == 0) a.part_ml[part] = make_float2(sh.m[r], l);
+                *reinterpret_cast<float4*>(stage + r * pitch + half * W + d) =
+                    make_float4(acc[d] * inv, acc[d + 1] * inv, acc[d + 2] * inv, acc[d + 3] * inv);
+            if (!whole && half == 0 && r < rows) a.part_ml[part + r] = make_float2(sh.m[r], l);
+        }
+        asm volatile("bar.sync 3, 256;" ::: "memory");
+        if (4 * lane < hd) {
+            const float* from = stage + 4 * lane;
+            if (!whole) {
+                float* out = a.part_o + part * hd + 4 * lane;
+#pragma unroll 2
+                for (int x = warp - 4; x < rows; x += 8)
+                    *reinterpret_cast<float4*>(out + x * hd) = *reinterpret_cast<const float4*>(from + x * pitch);
+            } else {
+#pragma unroll 1
+                for (int x = warp - 4; x < rows; x += 8) {
+                    const int row = row0 + x, tok = row / a.group, h = kvh * a.group + row - tok * a.group;
+                    *reinterpret_cast<float4*>(a.out + ((size_t(seq) * a.n_tree + tok) * a.n_head + h) * hd + 4 * lane) =
+                        *reinterpret_cast<const float4*>(from + x * pitch);
+                }
+            }
         }
     } else if (warp < kMmaWarp) {
         // ---- tiles ------------------------------------------------------------------------
