@@ -656,7 +656,15 @@ struct Cut {
     int R, row_blocks, parts;
     size_t rows;  // of all parts in the scratch
 };
-Cut cut_of(int n_seq, int n_tree, int n_head, int n_kv, int head_dim, int max_len) {
+// CTAs of the few-row kernel on an SM.
+template <int TYPE>
+constexpr int slots(int hd, bool stack) {
+    return hd <= 64    ? (stack ? Plan<TYPE, 64, true>::ctas : Plan<TYPE, 64, false>::ctas)
+           : hd <= 128 ? (stack ? Plan<TYPE, 128, true>::ctas : Plan<TYPE, 128, false>::ctas)
+                       : (stack ? Plan<TYPE, 256, true>::ctas : Plan<TYPE, 256, false>::ctas);
+}
+// type -1: the most parts of any type, for the scratch's size.
+Cut cut_of(int type, int n_seq, int n_tree, int n_head, int n_kv, int head_dim, int max_len) {
     Cut c;
     const int rows = n_tree * (n_head / n_kv);
     const size_t sms = size_t(syn_num_sms());
@@ -679,9 +687,14 @@ Cut cut_of(int n_seq, int n_tree, int n_head, int n_kv, int head_dim, int max_le
             }
         }
     } else {
-        // three CTAs per SM; a part has at least two steps of every warp
+        // one wave of CTAs; a part has at least two steps of every warp
+        const bool stack = c.R == 8;
+        const int per_sm = type == SYN_F16    ? slots<SYN_F16>(head_dim, stack)
+                           : type == SYN_Q8_0 ? slots<SYN_Q8_0>(head_dim, stack)
+                           : type == SYN_Q4_0 ? slots<SYN_Q4_0>(head_dim, stack)
+                                              : 3;
         const size_t most = size_t(max_len + 2 * kWarps * kStep - 1) / (2 * kWarps * kStep) * n_seq;
-        c.parts = int(std::min(3 * sms / units, most));
+        c.parts = int(std::min(per_sm * sms / units, most));
     }
     if (c.parts <= n_seq && !(n_seq == 1 && c.parts > 1)) c.parts = 0;
     if (!c.tc && units * n_seq * sizeof(unsigned) > kCounterBytes) c.parts = 0;
@@ -714,7 +727,7 @@ extern "C" size_t syn_tree_attention_scratch_bytes(int n_seq, int n_tree, int n_
     if (n_seq <= 0 || n_tree <= 0 || n_tree > kMaxTree || n_kv <= 0 || n_head <= 0 || n_head % n_kv || head_dim <= 0 ||
         head_dim > 256 || max_len < n_tree)
         return 0;
-    const Cut c = cut_of(n_seq, n_tree, n_head, n_kv, head_dim, max_len);
+    const Cut c = cut_of(-1, n_seq, n_tree, n_head, n_kv, head_dim, max_len);
     return kCounterBytes + (c.parts ? align256(c.rows * 8) + align256(c.rows * head_dim * 4) : 0);
 }
 
@@ -728,7 +741,7 @@ extern "C" int syn_tree_attention(const syn_kv_cache* c, int layer, const syn_tr
     const size_t q_row = size_t(x->n_head) * c->head_dim;
     if (x->q_stride && x->q_stride < q_row) return SYN_ERR_INVALID;
     if ((reinterpret_cast<uintptr_t>(x->scratch) | reinterpret_cast<uintptr_t>(x->out)) & 15) return SYN_ERR_INVALID;
-    const Cut cut = cut_of(c->n_seq, x->n_tree, x->n_head, c->n_kv, c->head_dim, x->max_len);
+    const Cut cut = cut_of(c->type, c->n_seq, x->n_tree, x->n_head, c->n_kv, c->head_dim, x->max_len);
     if (size_t(c->n_kv) * cut.row_blocks > 65535) return SYN_ERR_UNSUPPORTED;
     TreeParams a{};
     a.c = kv_view(c, layer);
