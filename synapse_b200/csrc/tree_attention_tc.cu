@@ -561,12 +561,12 @@ __global__ void __launch_bounds__(kTcThreads, 1) tree_attn_tc_kernel(const TreeP
             const uint64_t k = smem_desc(tiles_s + st * P::stage, 16, 1024);
             if (elect_one()) {
 #pragma unroll
-                for (int term = 0; term < (P::quant ? 3 : 2); ++term) {  // hi hi, lo hi, hi lo
+                for (int term = P::quant ? 2 : 1; term >= 0; --term) {  // hi lo, lo hi, hi hi: the small first, for sums truncate
                     const uint32_t qa = tm + (term == 1 ? P::q_lo : P::q_hi);
 #pragma unroll
                     for (int i = 0; i < HDP / 16; ++i)
                         mma_ts(d, qa + 8 * i, k + (((term == 2 ? P::k_lo : 0) + (i >> 2) * P::atom + (i & 3) * 32) >> 4), ds,
-                               term > 0 || i > 0);
+                               term < (P::quant ? 2 : 1) || i > 0);
                 }
                 mma_commit(&sh.s_full[j & 1]);
             }
@@ -586,11 +586,11 @@ __global__ void __launch_bounds__(kTcThreads, 1) tree_attn_tc_kernel(const TreeP
             const uint64_t v = smem_desc(tiles_s + st * P::stage + P::v_hi, P::atom, 1024);
             if (elect_one()) {
 #pragma unroll
-                for (int term = 0; term < (P::quant ? 3 : 2); ++term) {
+                for (int term = P::quant ? 2 : 1; term >= 0; --term) {
 #pragma unroll
                     for (int i = 0; i < kTcTile / 16; ++i)
                         mma_ts(d, pa + (term == 1 ? 32 : 0) + 8 * i, v + (((term == 2 ? P::tile : 0) + i * 2048) >> 4), dv,
-                               term > 0 || i > 0);
+                               term < (P::quant ? 2 : 1) || i > 0);
                 }
                 mma_commit(&sh.o_full[j & 1]);
                 mma_commit(&sh.kv_empty[st]);
