@@ -456,56 +456,67 @@ __global__ void __launch_bounds__(kTcThreads, 1) tree_attn_tc_kernel(const TreeP
         } else {
             constexpr int VPC = TYPE == SYN_Q8_0 ? 16 : 32;          // values of 16 bytes of quants
             constexpr int CP = HDP / VPC, NI = kTcTile * CP / 32, N = (2 * NI + kFillWarps - 1) / kFillWarps;  // chunks of a row; sets of K; of a warp
+            constexpr int PS = 32 / CP;  // positions of a set
             const int nb = hd / 32, chunks = hd / VPC;
-            const size_t head = size_t(kvh) * a.c.max_ctx;
-            const uint16_t *ks = reinterpret_cast<const uint16_t*>(kb + a.c.scale_plane), *vs = reinterpret_cast<const uint16_t*>(vb + a.c.scale_plane);
-            // A warp's share of a tile: sets of 32 chunks (16 bytes of quants) of K, then of V, every kFillWarps-th.
-            // A set of the next tile is requested as soon as this tile's is in hand.
+            // A warp's share of a tile: sets of 32 chunks (16 bytes of quants) of K, then of V, every kFillWarps-th. A lane
+            // has the same chunk `ch` of a row in all of them. A set of the next tile is requested as soon as this
+            // tile's is in hand.
+            const int ch = lane % CP, lp = lane / CP;
+            const size_t row_at = size_t(kvh) * a.c.max_ctx + size_t(t0) * kTcTile + lp;
+            const char *kq = kb + (row_at * chunks + ch) * 16, *ks = kb + a.c.scale_plane + (row_at * nb + ch * VPC / 32) * 2;
+            const ptrdiff_t to_v = vb - kb;
+            const uint32_t set_q = PS * chunks * 16, set_s = PS * nb * 2;
             uint4 q[N];
             uint32_t d[N];  // scale bits
-            auto fetch = [&](int k, int t) {
+            auto fetch = [&](int k, int j) {
                 const int i = k * kFillWarps + fw;
                 if (i >= 2 * NI) return;
                 const bool v = i >= NI;
-                const int id = (v ? i - NI : i) * 32 + lane, p = id / CP, ch = id % CP, pos = t * kTcTile + p;
+                const int ii = v ? i - NI : i;
                 q[k] = make_uint4(0, 0, 0, 0);
                 d[k] = 0;
-                if (ch < chunks && pos < total) {
-                    const size_t rowi = head + pos;
-                    q[k] = __ldg(reinterpret_cast<const uint4*>((v ? vb : kb) + (rowi * chunks + ch) * 16));
-                    d[k] = __ldg((v ? vs : ks) + rowi * nb + ch * VPC / 32);
+                if (ch < chunks && (t0 + j) * kTcTile + ii * PS + lp < total) {
+                    const char *qp = kq + (v ? to_v : 0), *sp = ks + (v ? to_v : 0);
+                    q[k] = __ldg(reinterpret_cast<const uint4*>(qp + ii * set_q + size_t(j) * (kTcTile / PS) * set_q));
+                    d[k] = __ldg(reinterpret_cast<const uint16_t*>(sp + ii * set_s + size_t(j) * (kTcTile / PS) * set_s));
                 }
             };
-            auto convert = [&](int k, int j) {
-                const int i = k * kFillWarps + fw, t = t0 + j, st = j % P::stages;
+            // a lane's place in a swizzled row: neighbouring lanes store different 16-byte columns at a time, those of the
+            // second 64 dims take the chunk's eights in another order
+            const int c0 = ch * (VPC / 8), turn = (c0 >> 3) * (VPC / 16);
+            const uint32_t lane_at = (c0 >> 3) * P::atom + lp * 128;
+            const __half2 zero = half2_of(TYPE == SYN_Q8_0 ? 0x64806480u : 0x64086408u);
+            auto convert = [&](int k, int j, int st) {
+                const int i = k * kFillWarps + fw;
                 if (i >= 2 * NI) return;
                 const bool v = i >= NI;
-                const int id = (v ? i - NI : i) * 32 + lane, p = id / CP, ch = id % CP;  // past the head: scales of 0
-                const bool finite = (d[k] & 0x7c00u) != 0x7c00u;
-                if (!finite && t * kTcTile + p >= len) {  // a tree row's position is bad: NaN for who sees it
-                    d[k] = 0;
-                    atomicOr(&sh.bad[t - edge0], 1ull << p);
+                const int ii = v ? i - NI : i, p = ii * PS + lp;
+                uint32_t top = d[k] & 0x7fffu;
+                if (__any_sync(0xffffffffu, top >= 0x7c00u)) {  // not finite: a tree row's position is bad, NaN for who sees it
+                    const int t = t0 + j;
+                    if (top >= 0x7c00u) {
+                        if (t * kTcTile + p >= len) {
+                            d[k] = 0;
+                            atomicOr(&sh.bad[t - edge0], 1ull << p);
+                        }
+                        top = 0;
+                    }
                 }
                 // the position's largest scale to [2^8, 2^9): 127 of it is finite, and the low term reaches 2^-33 of it
-                uint32_t top = finite ? d[k] & 0x7fffu : 0u;
 #pragma unroll
-                for (int o = 1; o < CP; o <<= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
-                const int e = 23 - int(max(top >> 10, 1u));
-                const float up = __uint_as_float(uint32_t(127 + e) << 23), down = __uint_as_float(uint32_t(127 - e) << 23);
+                for (int o = TYPE == SYN_Q8_0 ? 2 : 1; o < CP; o <<= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
+                const uint32_t e = max(top >> 10, 1u);
+                const float up = __uint_as_float((150u - e) << 23), down = __uint_as_float((104u + e) << 23);  // 2^(23 - e), 2^(e - 23)
                 if (ch == 0) {
                     if (!v) {
                         sh.k_pow[st][p] = down;
                     } else {
-                        sh.v_log[st][p] = float(-e);
+                        sh.v_log[st][p] = float(int(e) - 23);
                         sh.v_inv[st][p] = up;
                     }
                 }
-                const __half2 zero = half2_of(TYPE == SYN_Q8_0 ? 0x64806480u : 0x64086408u);
                 const __half2 scale = __float2half2_rn(f16_from_bits(uint16_t(d[k])) * up);
-                // neighbouring threads store different 16-byte columns of the swizzled rows at a time: those of the
-                // second 64 dims take the chunk's eights in another order
-                const int c0 = ch * (VPC / 8), turn = (c0 >> 3) * (VPC / 16);
-                unsigned char* rowp = tiles + st * P::stage + (v ? P::v_hi : 0) + (c0 >> 3) * P::atom + p * 128;
+                unsigned char* rowp = tiles + st * P::stage + (v ? P::v_hi : 0) + lane_at + ii * (PS * 128);
                 const int col = (((c0 ^ p) & 7) ^ turn) << 4;
                 uint32_t w[4] = {q[k].x, q[k].y, q[k].z, q[k].w};
                 if (TYPE == SYN_Q8_0) {
@@ -538,16 +549,19 @@ __global__ void __launch_bounds__(kTcThreads, 1) tree_attn_tc_kernel(const TreeP
                 }
             };
 #pragma unroll
-            for (int k = 0; k < N; ++k) fetch(k, t0);
+            for (int k = 0; k < N; ++k) fetch(k, 0);
+            int st = 0;
+#pragma unroll 1
             for (int j = 0; j < n; ++j) {
                 if (j == 1 && !warp_wait(&sh.q_full, 0, sh)) break;
-                if (j >= P::stages && !warp_wait(&sh.kv_empty[j % P::stages], uint32_t(j / P::stages - 1) & 1, sh)) break;
+                if (j >= P::stages && !warp_wait(&sh.kv_empty[st], uint32_t(j / P::stages - 1) & 1, sh)) break;
 #pragma unroll
                 for (int k = 0; k < N; ++k) {
-                    convert(k, j);
-                    if (j + 1 < n) fetch(k, t0 + j + 1);
+                    convert(k, j, st);
+                    if (j + 1 < n) fetch(k, j + 1);
                 }
                 full(j);
+                if (++st == P::stages) st = 0;
             }
         }
     } else {
