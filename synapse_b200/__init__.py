@@ -480,11 +480,20 @@ def _rows(t, f32, cols, n, where):
     return t.data_ptr(), ld
 
 
-def _on(stream, device):
-    """The handle of a stream (None: the device's current one)."""
-    if stream is not None:
-        return stream.cuda_stream
+def _current(device):
+    """The handle of a device's current stream."""
     return _torch()._C._cuda_getCurrentRawStream(device.index)
+
+
+def _streamed(f):
+    """Adds a `stream` argument: the call, what it allocates included, runs with that stream as the current one."""
+    @functools.wraps(f)
+    def call(*args, stream=None, **kw):
+        if stream is None:
+            return f(*args, **kw)
+        with _torch().cuda.stream(stream):
+            return f(*args, **kw)
+    return call
 
 
 @functools.lru_cache(maxsize=256)
@@ -493,7 +502,8 @@ def _tree_scratch_bytes(n_seq, tree, n_head, n_kv, head_dim, max_len, device):
         return lib().syn_tree_attention_scratch_bytes(n_seq, tree, n_head, n_kv, head_dim, max_len)
 
 
-def kv_append(cache, k, v, slot, pos=None, rope_table=None, rope_mode=0, q=None, layer=0, stream=None):
+@_streamed
+def kv_append(cache, k, v, slot, pos=None, rope_table=None, rope_mode=0, q=None, layer=0):
     """Append tokens' K and V rows [n_seq * n][n_kv * head_dim] at slots (int32, n_seq * n), K rotated when a
     rope_table ([len][head_dim / 2][2]) is given; q [n_seq * n][n_head * head_dim], if given, is rotated too and
     returned."""
@@ -515,11 +525,12 @@ def kv_append(cache, k, v, slot, pos=None, rope_table=None, rope_mode=0, q=None,
     a = KVAppendArgs(kp, vp, qp, op, _need(slot, i32, tokens, "slot"), _need(pos, i32, tokens, "pos"),
                      _need(rope_table, f32, table_len * hd, "rope_table"), ks, qs, tokens // cache.n_seq, n_head,
                      table_len, rope_mode)
-    check(lib().syn_kv_append(cache.ref, layer, ctypes.byref(a), _on(stream, cache.device)), "syn_kv_append")
+    check(lib().syn_kv_append(cache.ref, layer, ctypes.byref(a), _current(cache.device)), "syn_kv_append")
     return out
 
 
-def kv_read(cache, n, rows=None, first=0, dtype=None, layer=0, stream=None):
+@_streamed
+def kv_read(cache, n, rows=None, first=0, dtype=None, layer=0):
     """n rows of every sequence as values, (k, v) [n_seq][n][n_kv][head_dim]: the cache rows named by `rows` (int32,
     n_seq * n), or first, first + 1, ...; dtype torch.float32 (default) or torch.float16."""
     torch = _torch()
@@ -530,16 +541,17 @@ def kv_read(cache, n, rows=None, first=0, dtype=None, layer=0, stream=None):
     k, v = cache.k.new_empty(shape, dtype=dtype), cache.k.new_empty(shape, dtype=dtype)
     check(lib().syn_kv_read(cache.ref, layer, _need(rows, torch.int32, cache.n_seq * n, "rows"), first, n,
                             F16 if dtype == torch.float16 else F32, k.data_ptr(), v.data_ptr(),
-                            _on(stream, cache.device)), "syn_kv_read")
+                            _current(cache.device)), "syn_kv_read")
     return k, v
 
 
-def kv_move(cache, path, count, begin, stream=None):
+@_streamed
+def kv_move(cache, path, count, begin):
     """Rows path[s][i] (int32, ascending, >= begin[s] + i) of sequence s become rows begin[s] + i, i < count[s], in
     every layer."""
     i32, n, ld = _torch().int32, cache.n_seq, path.shape[-1]
     check(lib().syn_kv_move(cache.ref, _need(path, i32, n * ld, "path"), ld, _need(count, i32, n, "count"),
-                            _need(begin, i32, n, "begin"), _on(stream, cache.device)), "syn_kv_move")
+                            _need(begin, i32, n, "begin"), _current(cache.device)), "syn_kv_move")
 
 
 def tree_attention_scratch(cache, tree, n_head, max_len=None):
@@ -554,8 +566,8 @@ def _tree_scratch(n, device):
     return scratch
 
 
-def tree_attention(cache, q, len, n_head, scale, tree=1, mask=None, max_len=None, out=None, scratch=None, layer=0,
-                   stream=None):
+@_streamed
+def tree_attention(cache, q, len, n_head, scale, tree=1, mask=None, max_len=None, out=None, scratch=None, layer=0):
     """Attention of `tree` tokens of every sequence over rows 0 .. len[s] - 1 and the tree's own rows after them that
     their mask bits name (None: a causal chunk); q [n_seq * tree][n_head * head_dim], rotated. See syn_tree_attention."""
     torch = _torch()
@@ -573,7 +585,7 @@ def tree_attention(cache, q, len, n_head, scale, tree=1, mask=None, max_len=None
     a = TreeAttentionArgs(qp, _need(out, f32, rows * cols, "out"), _need(len, i32, cache.n_seq, "len"),
                           _need(mask, i32, rows * ((tree + 31) // 32), "mask"), scratch.data_ptr(), qs, tree, n_head,
                           max_len, scale)
-    check(lib().syn_tree_attention(cache.ref, layer, ctypes.byref(a), _on(stream, cache.device)),
+    check(lib().syn_tree_attention(cache.ref, layer, ctypes.byref(a), _current(cache.device)),
           "syn_tree_attention")
     return out
 
@@ -583,8 +595,9 @@ def logits_scratch(n_rows, device="cuda"):
     return _torch().zeros(max(lib().syn_logits_scratch_bytes(n_rows), 1), dtype=_torch().uint8, device=device)
 
 
+@_streamed
 def logits_process(logits, n_seq, penalties=None, history=None, history_len=None, draft=None, mask=None, bias=None,
-                   allowed=None, out=None, pick=True, scratch=None, stream=None):
+                   allowed=None, out=None, pick=True, scratch=None):
     """Biases, penalties and a grammar mask on logits [n_seq * tree][n_vocab], and the pick of every row: (out, pick).
     penalties [n_seq][3] (repeat, presence, frequency), history [n_seq][ld] with history_len [n_seq], the tree's
     tokens draft [n_seq][tree] with mask words, bias (begin [n_seq + 1], tokens, values), allowed [rows][words]. out
@@ -621,7 +634,7 @@ def logits_process(logits, n_seq, penalties=None, history=None, history_len=None
                    _need(begin, i32, n_seq + 1, "bias begin"), _need(tokens, i32, n, "bias tokens"),
                    _need(values, f32, n, "bias values"), _need(allowed, i32, rows * words, "allowed"), words, sp,
                    n_seq, tree, vocab, history_ld)
-    check(lib().syn_logits_process(ctypes.byref(a), _on(stream, logits.device)), "syn_logits_process")
+    check(lib().syn_logits_process(ctypes.byref(a), _current(logits.device)), "syn_logits_process")
     return out, picks
 
 

@@ -375,9 +375,11 @@ __global__ void __launch_bounds__(kWarps * 32, Plan<TYPE, HDP, STACK>::ctas) tre
                 products(c, k, b, k == 0);
             }
 #pragma unroll
-            for (int u = 0; u < 2; ++u)
+            for (int u = 0; u < 2; ++u) {
+                if (STACK) add2(c[u][0], c[u][1], c[u][2], c[u][3]);
 #pragma unroll
-                for (int e = 0; e < 2 * NR; ++e) s[u][e] = STACK ? c[u][e] + c[u][e + 2] : c[u][e];
+                for (int e = 0; e < 2 * NR; ++e) s[u][e] = c[u][e];
+            }
         } else {
             float kd[4][NB];  // of positions 2t, 2t + 1, 2t + 8, 2t + 9
 #pragma unroll
@@ -411,12 +413,19 @@ __global__ void __launch_bounds__(kWarps * 32, Plan<TYPE, HDP, STACK>::ctas) tre
                     products(c, 2 * b + h, bb, h == 0);
                 }
 #pragma unroll
-                for (int u = 0; u < 2; ++u)
+                for (int u = 0; u < 2; ++u) {
+                    const float d0 = kd[2 * u][b], d1 = kd[2 * u + 1][b];
+                    if (STACK) add2(c[u][0], c[u][1], c[u][2], c[u][3]);
 #pragma unroll
-                    for (int e = 0; e < 2 * NR; ++e) {
-                        const float x = STACK ? c[u][e] + c[u][e + 2] : c[u][e], d = kd[2 * u + (e & 1)][b];
-                        s[u][e] = b == 0 ? x * d : fmaf(x, d, s[u][e]);
+                    for (int e = 0; e < 2 * NR; e += 2) {
+                        if (b == 0) {
+                            s[u][e] = c[u][e] * d0;
+                            s[u][e + 1] = c[u][e + 1] * d1;
+                        } else {
+                            fma2_to(s[u][e], s[u][e + 1], c[u][e], c[u][e + 1], d0, d1);
+                        }
                     }
+                }
             }
         }
 
@@ -499,14 +508,14 @@ __global__ void __launch_bounds__(kWarps * 32, Plan<TYPE, HDP, STACK>::ctas) tre
         uint32_t pf[QT][4];
         auto split_p = [&](const float (&f)[4]) {
 #pragma unroll
-            for (int u = 0; u < 2; ++u) {
-                if (STACK) {
-                    split2(p[u][0] * f[2 * u], p[u][1] * f[2 * u + 1], pf[0][2 * u], pf[0][2 * u + 1]);
-                } else {
-                    split2(p[u][0] * f[2 * u], p[u][1] * f[2 * u + 1], pf[0][2 * u], pf[QT - 1][2 * u]);
-                    split2(p[u][2 * NR - 2] * f[2 * u], p[u][2 * NR - 1] * f[2 * u + 1], pf[0][2 * u + 1], pf[QT - 1][2 * u + 1]);
+            for (int u = 0; u < 2; ++u)
+#pragma unroll
+                for (int e = 0; e < 2 * NR; e += 2) {
+                    float x = p[u][e], y = p[u][e + 1];
+                    mul2(x, y, f[2 * u], f[2 * u + 1]);
+                    if (STACK) split2(x, y, pf[0][2 * u], pf[0][2 * u + 1]);
+                    else split2(x, y, pf[0][2 * u + e / 2], pf[QT - 1][2 * u + e / 2]);
                 }
-            }
         };
         auto output = [&](float (&acc)[2 * NR], uint32_t b0, uint32_t b1) {
             float c[4];

@@ -427,6 +427,62 @@ def test_tree_attention_strided_queries_layers_and_streams():
     assert not torch.equal(syn.tree_attention(cache, q, lens, n_head, 0.2, tree=tree, layer=1), want)
 
 
+@pytest.mark.parametrize("type_", TYPES)
+@pytest.mark.parametrize("tree", [1, 9])
+def test_unaligned_rows_and_a_stream_argument(type_, tree):
+    """Rows of q, k and v that start and follow at no 16-byte boundary, and the calls' stream argument."""
+    rng = np.random.default_rng(13)
+    n_head, n_kv, hd, L = 8, 2, 128, 300
+    wide = gpu(rng.standard_normal((tree, (n_head + 2 * n_kv) * hd + 3), dtype=np.float32))
+    q, k, v = wide[:, 1:1 + n_head * hd], wide[:, 1 + n_head * hd:1 + (n_head + n_kv) * hd], wide[:, 1 + (n_head + n_kv) * hd:-2]
+    table = syn.rope_table(L + tree, hd, 0.9)
+    slot = gpu(np.arange(L, L + tree, dtype=np.int32))
+    lens = gpu(np.array([L], np.int32))
+    a, b = new_cache(type_, 1, n_kv, hd, L + tree), new_cache(type_, 1, n_kv, hd, L + tree)
+    for c in (a, b):
+        fill(c, np.random.default_rng(0), L)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    for mode in (0, 1):
+        qa = syn.kv_append(a, k, v, slot, rope_table=table, rope_mode=mode, q=q, stream=side)
+        oa = syn.tree_attention(a, qa, lens, n_head, 0.1, tree=tree, stream=side)
+        ua = syn.tree_attention(a, q, lens, n_head, 0.1, tree=tree, stream=side)
+        _, pa = syn.logits_process(ua, 1, stream=side)
+        ka, va = syn.kv_read(a, L + tree, stream=side)
+        side.synchronize()
+        qb = syn.kv_append(b, k.contiguous(), v.contiguous(), slot, rope_table=table, rope_mode=mode, q=q.contiguous())
+        ob = syn.tree_attention(b, qb, lens, n_head, 0.1, tree=tree)
+        ub = syn.tree_attention(b, q.contiguous(), lens, n_head, 0.1, tree=tree)
+        kb, vb = syn.kv_read(b, L + tree)
+        for x, y in ((qa, qb), (oa, ob), (ua, ub), (ka, kb), (va, vb)):
+            assert torch.equal(x, y)
+        assert torch.equal(pa, syn.logits_process(ub, 1)[1])
+
+
+@pytest.mark.parametrize("type_", TYPES)
+def test_wide_trees(type_):
+    check_attention(type_, 2, 1, 64, [130, 5], 300, seed=21)
+    check_attention(type_, 1, 1, 32, [40], 1024, seed=22)
+
+
+@pytest.mark.parametrize("type_", TYPES)
+def test_lengths_outside_the_bound_are_clamped(type_):
+    rng = np.random.default_rng(14)
+    for n_head, tree in ((2, 2), (24, 3)):
+        cache = new_cache(type_, 3, 2, 64, 64)
+        fill(cache, rng, 64)
+        q = gpu(rng.standard_normal((3 * tree, n_head * 64), dtype=np.float32))
+        got = syn.tree_attention(cache, q, gpu(np.array([-5, 1000, 2**31 - 1], np.int32)), n_head, 0.1, tree=tree, max_len=60)
+        want = syn.tree_attention(cache, q, gpu(np.array([0, 60 - tree, 60 - tree], np.int32)), n_head, 0.1, tree=tree, max_len=60)
+        assert torch.equal(got, want)
+
+
+@pytest.mark.parametrize("type_", TYPES)
+def test_negative_scale(type_):
+    check_attention(type_, 4, 2, 64, [70], 3, seed=31, scale=-0.125)
+    check_attention(type_, 24, 2, 64, [70], 3, seed=32, scale=-0.125)
+
+
 def test_offsets_past_32_bits():
     """Rows past 2^32 bytes: written, read, moved and attended to; the scores of all but three rows are zero."""
     n_kv, hd = 8, 128
