@@ -4,7 +4,7 @@
 //
 // A KV head's work is one matrix product over the rows r = token * G + head of
 // its group (G = n_head / n_kv): M = n_tree * G rows against every position,
-// so the cache is read once for the whole tree. With more than 16 rows (and
+// so the cache is read once for the whole tree. With many rows (cut_of, and
 // head_dim <= 128) tree_attention_tc.cu takes the call; here is the kernel for
 // few rows, where the cache's bytes are the bound.
 //
@@ -628,7 +628,7 @@ __global__ void __launch_bounds__(kWarps * 32, Plan<TYPE, HDP, STACK>::ctas) tre
         }
         if (!whole && lane == 0) a.part_ml[part + r] = make_float2(mx, sum);
     }
-    if (a.parts == 0) return;
+    if (!a.arrived) return;
 
     // --- the last of the sequence's parts to be done joins them ----------------------------
     __threadfence();
@@ -661,7 +661,7 @@ __global__ void __launch_bounds__(128) tree_join_kernel(const TreeParams a, int 
 // How a call is cut: rows of a CTA, CTAs over the rows, parts of the contexts
 // (0: a part is a sequence).
 struct Cut {
-    bool tc;
+    bool tc, join;  // on tcgen05; parts joined by tree_join_kernel
     int R, row_blocks, parts;
     size_t rows;  // of all parts in the scratch
 };
@@ -672,12 +672,15 @@ constexpr int slots(int hd, bool stack) {
            : hd <= 128 ? (stack ? Plan<TYPE, 128, true>::ctas : Plan<TYPE, 128, false>::ctas)
                        : (stack ? Plan<TYPE, 256, true>::ctas : Plan<TYPE, 256, false>::ctas);
 }
-// type -1: the most parts of any type, for the scratch's size.
+// More than 16 rows (32 of a quantised cache, whose tiles the tcgen05 kernel has to convert) go to tree_attention_tc.cu.
+// Measured for 16 sequences of 8192 positions and 8 KV heads of 128, this kernel / that one, us: F16 16 rows 97 / 136, 20
+// rows 145 / 136, 64 rows 247 / 149; Q8_0 32 rows 201 / 254, 48 rows 317 / 265; Q4_0 202 / 230, 311 / 236. For one
+// sequence of 32768: F16 20 rows 45 / 42; Q8_0 32 rows 57 / 69, 48 rows 77 / 70.
 Cut cut_of(int type, int n_seq, int n_tree, int n_head, int n_kv, int head_dim, int max_len) {
     Cut c;
     const int rows = n_tree * (n_head / n_kv);
     const size_t sms = size_t(syn_num_sms());
-    c.tc = rows > 16 && head_dim <= 128;
+    c.tc = rows > (type == SYN_F16 ? 16 : 32) && head_dim <= 128;
     c.R = c.tc ? kTcRows : rows <= 8 ? 8 : 16;
     c.row_blocks = (rows + c.R - 1) / c.R;
     const size_t units = size_t(n_kv) * c.row_blocks;  // CTAs of a part
@@ -700,13 +703,14 @@ Cut cut_of(int type, int n_seq, int n_tree, int n_head, int n_kv, int head_dim, 
         const bool stack = c.R == 8;
         const int per_sm = type == SYN_F16    ? slots<SYN_F16>(head_dim, stack)
                            : type == SYN_Q8_0 ? slots<SYN_Q8_0>(head_dim, stack)
-                           : type == SYN_Q4_0 ? slots<SYN_Q4_0>(head_dim, stack)
-                                              : 3;
+                                              : slots<SYN_Q4_0>(head_dim, stack);
         const size_t most = size_t(max_len + 2 * kWarps * kStep - 1) / (2 * kWarps * kStep) * n_seq;
         c.parts = int(std::min(per_sm * sms / units, most));
     }
     if (c.parts <= n_seq && !(n_seq == 1 && c.parts > 1)) c.parts = 0;
-    if (!c.tc && units * n_seq * sizeof(unsigned) > kCounterBytes) c.parts = 0;
+    // The last CTA has a row a warp to join, or two of a few parts, in less time than a launch; with more it has them
+    // one after another.
+    c.join = c.parts && (c.tc || rows > 8 || (rows > 4 && c.parts > 16 * n_seq) || units * n_seq * sizeof(unsigned) > kCounterBytes);
     c.rows = size_t(c.parts) * units * c.R;
     return c;
 }
@@ -736,8 +740,10 @@ extern "C" size_t syn_tree_attention_scratch_bytes(int n_seq, int n_tree, int n_
     if (n_seq <= 0 || n_tree <= 0 || n_tree > kMaxTree || n_kv <= 0 || n_head <= 0 || n_head % n_kv || head_dim <= 0 ||
         head_dim > 256 || max_len < n_tree)
         return 0;
-    const Cut c = cut_of(-1, n_seq, n_tree, n_head, n_kv, head_dim, max_len);
-    return kCounterBytes + (c.parts ? align256(c.rows * 8) + align256(c.rows * head_dim * 4) : 0);
+    size_t rows = 0;  // the most of any type
+    for (int type : {SYN_F16, SYN_Q8_0, SYN_Q4_0})
+        rows = std::max(rows, cut_of(type, n_seq, n_tree, n_head, n_kv, head_dim, max_len).rows);
+    return kCounterBytes + align256(rows * 8) + align256(rows * head_dim * 4);
 }
 
 extern "C" int syn_tree_attention(const syn_kv_cache* c, int layer, const syn_tree_attention_args* x, void* stream) {
@@ -756,7 +762,7 @@ extern "C" int syn_tree_attention(const syn_kv_cache* c, int layer, const syn_tr
     a.c = kv_view(c, layer);
     a.q = x->q; a.out = x->out; a.len = x->len; a.mask = x->mask;
     char* scratch = static_cast<char*>(x->scratch);
-    a.arrived = reinterpret_cast<unsigned*>(scratch);
+    a.arrived = cut.parts && !cut.join ? reinterpret_cast<unsigned*>(scratch) : nullptr;
     a.part_ml = reinterpret_cast<float2*>(scratch + kCounterBytes);
     a.part_o = reinterpret_cast<float*>(scratch + kCounterBytes + align256(cut.rows * 8));
     a.q_stride = x->q_stride ? x->q_stride : q_row;
@@ -773,7 +779,7 @@ extern "C" int syn_tree_attention(const syn_kv_cache* c, int layer, const syn_tr
     else if (c->type == SYN_F16) st = launch_type<SYN_F16>(a, cut, s);
     else if (c->type == SYN_Q8_0) st = launch_type<SYN_Q8_0>(a, cut, s);
     else st = launch_type<SYN_Q4_0>(a, cut, s);
-    if (st || !cut.parts || !cut.tc) return st;
+    if (st || !cut.join) return st;
     const size_t rows = size_t(c->n_seq) * c->n_kv * a.rows;
-    return syn_launch_pdl(true, tree_join_kernel, unsigned((rows + 3) / 4), 128, 0, s, a, cut.R, kTcTile);
+    return syn_launch_pdl(true, tree_join_kernel, unsigned((rows + 3) / 4), 128, 0, s, a, cut.R, cut.tc ? kTcTile : kStep);
 }
