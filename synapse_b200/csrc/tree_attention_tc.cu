@@ -24,7 +24,7 @@
 // (Q4_0) for the cache's bytes at head_dim 128. Measured: 64 tokens of 64 heads
 // over 32768 F16 positions 141 us, the tensor cores busy 45 % of it: a tile
 // takes some 2000 cycles of 1024, and leaving out the exponentials, the splitting
-// or the reading of O changes that by 3 to 9 % each: the roles wait for one
+// or the reading of O changes that by 4 to 9 %: the roles wait for one
 // another's latency. Before its first tile a CTA needs 9000 cycles (its 64 KB
 // of q to tensor memory, the first tile), after the last 5000 (64 KB of O), which
 // is most of a short context's time (32 rows of 8192 positions: 20 us).

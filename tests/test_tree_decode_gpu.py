@@ -318,6 +318,13 @@ def test_tree_attention_long(type_, lens, tree):
 
 
 @pytest.mark.parametrize("type_", TYPES)
+@pytest.mark.parametrize("tree", [2, 3, 4, 5, 8, 9])
+@pytest.mark.parametrize("lens", [[2500], [900, 3, 31]])
+def test_attention_where_the_kernels_change(type_, tree, lens):
+    check_attention(type_, 8, 2, 128, lens, tree)
+
+
+@pytest.mark.parametrize("type_", TYPES)
 @pytest.mark.parametrize("lens,tree", [([0], 70), ([100, 37], 9)])
 def test_causal_chunk(type_, lens, tree):
     check_attention(type_, 6, 2, 64, lens, tree, seed=3, mask=None)
