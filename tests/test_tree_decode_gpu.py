@@ -321,7 +321,7 @@ def test_tree_attention_long(type_, lens, tree):
 @pytest.mark.parametrize("tree", [2, 3, 4, 5, 8, 9])
 @pytest.mark.parametrize("lens", [[2500], [900, 3, 31]])
 def test_attention_where_the_kernels_change(type_, tree, lens):
-    check_attention(type_, 8, 2, 128, lens, tree)
+    check_attention(type_, 8, 2, 128, lens, tree, seed=tree)
 
 
 @pytest.mark.parametrize("type_", TYPES)
