@@ -325,6 +325,15 @@ def test_attention_where_the_kernels_change(type_, tree, lens):
 
 
 @pytest.mark.parametrize("type_", TYPES)
+@pytest.mark.parametrize("tree", [1, 3, 6])
+def test_attention_of_many_ragged_sequences(type_, tree):
+    """Far more sequences than the GPU has room for at a time, of lengths from none to several parts."""
+    lens = [int(x) for x in np.random.default_rng(9).integers(0, 60, 400)]
+    lens[3], lens[200], lens[399] = 1500, 700, 0
+    check_attention(type_, 4, 2, 64, lens, tree, seed=tree)
+
+
+@pytest.mark.parametrize("type_", TYPES)
 @pytest.mark.parametrize("lens,tree", [([0], 70), ([100, 37], 9)])
 def test_causal_chunk(type_, lens, tree):
     check_attention(type_, 6, 2, 64, lens, tree, seed=3, mask=None)
