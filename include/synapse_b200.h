@@ -355,7 +355,7 @@ int syn_tree_attention(const syn_kv_cache* c, int layer, const syn_tree_attentio
  *             (NaN is never picked).
  * Everything but logits, out or pick, and the sizes may be NULL. Tokens
  * outside the vocabulary count nowhere. A token that a sequence's bias list
- * names twice gets both. Calls that overlap on the GPU need scratches of
+ * names several times gets their sum, added in the list's order. Calls that overlap on the GPU need scratches of
  * their own. */
 typedef struct {
     const float* logits;

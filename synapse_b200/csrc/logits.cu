@@ -57,12 +57,12 @@ struct Shared {
     static constexpr bool wide = CHUNK <= 1024;
     unsigned count[wide ? CHUNK : CHUNK / 2];
     float bias[CHUNK];
-    float x[CHUNK];                   // a thread's own vectors, where it indexes them
+    float x[CHUNK];                   // a thread's own vectors, where it indexes them; before the rows, how often a bias names a token
     unsigned touched[CHUNK / 32];     // the tokens that may have a count or a bias
     unsigned drafted[CHUNK / 32];     // those some node of the tree has
     unsigned long long best[kMaxRows];
     unsigned short mine[kMaxTree];    // the nodes whose tokens are in this chunk
-    int n_mine;
+    int n_mine, thrice;
     __device__ __forceinline__ void add(int at) {
         if (wide) atomicAdd(&count[at], 1u);
         else atomicAdd(&count[at >> 1], 1u << (16 * (at & 1)));
@@ -95,11 +95,11 @@ __global__ void __launch_bounds__(kThreads, 4) logits_kernel(const LogitParams a
     const int i0 = blockIdx.y * a.rows_per_cta, n_rows = min(a.rows_per_cta, a.n_tree - i0);
     for (int i = tid; i < CHUNK; i += kThreads) {
         if (i < int(sizeof(sh.count) / 4)) sh.count[i] = 0;
-        sh.bias[i] = 0.0f;
+        sh.bias[i] = sh.x[i] = 0.0f;
         if (i < CHUNK / 32) sh.touched[i] = sh.drafted[i] = 0;
     }
     for (int i = tid; i < n_rows; i += kThreads) sh.best[i] = 0;
-    if (tid == 0) sh.n_mine = 0;
+    if (tid == 0) sh.n_mine = sh.thrice = 0;
     __syncthreads();
     pdl_launch_dependents();
     pdl_wait();
@@ -156,6 +156,7 @@ __global__ void __launch_bounds__(kThreads, 4) logits_kernel(const LogitParams a
             const int tok = a.bias_token[i];
             if (tok >= v0 && tok - v0 < span) {
                 atomicAdd(&sh.bias[tok - v0], a.bias_value[i]);
+                if (atomicAdd(reinterpret_cast<unsigned*>(sh.x) + tok - v0, 1u) == 2) sh.thrice = 1;
                 touch(tok - v0);
             }
         }
@@ -171,6 +172,16 @@ __global__ void __launch_bounds__(kThreads, 4) logits_kernel(const LogitParams a
             }
         }
     __syncthreads();
+    if (sh.thrice) {  // a sum of two is the same in either order; those of more are made again, in the list's order
+        for (int at = tid; at < CHUNK; at += kThreads)
+            if (__float_as_uint(sh.x[at]) > 2) {
+                float sum = 0.0f;
+                for (int i = a.bias_begin[seq]; i < a.bias_begin[seq + 1]; ++i)
+                    if (a.bias_token[i] == v0 + at) sum += a.bias_value[i];
+                sh.bias[at] = sum;
+            }
+        __syncthreads();
+    }
     const int n_mine = sh.n_mine;
     const float repeat = a.penalties ? a.penalties[3 * seq] : 1.0f;
     const float presence = a.penalties ? a.penalties[3 * seq + 1] : 0.0f;

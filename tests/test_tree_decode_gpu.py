@@ -630,6 +630,27 @@ def test_logits_in_place_strided_ties_and_values_that_are_not_finite():
     assert syn.logits_process(x, 3, pick=False)[1] is None
 
 
+@pytest.mark.parametrize("vocab", [1500, 64000])
+def test_logits_biases_of_a_token_add_in_the_lists_order(vocab):
+    """Sums whose value depends on the order, their entries far apart among others; long and short chunks."""
+    rng = np.random.default_rng(5)
+    rows = 1 if vocab < 4096 else 64
+    tokens = rng.integers(0, vocab, 1200).astype(np.int32)
+    values = rng.standard_normal(1200).astype(np.float32)
+    for t in (7, vocab - 1):
+        at = rng.choice(1200, 40, replace=False)
+        tokens[at] = t
+        values[at] = (rng.standard_normal(40) * 10.0 ** rng.integers(-3, 8, 40)).astype(np.float32)
+    want = np.zeros(vocab, np.float32)
+    for t, v in zip(tokens, values):
+        want[t] = want[t] + v
+    x = gpu(np.zeros((rows, vocab), np.float32))
+    bias = (gpu(np.array([0, 1200], np.int32)), gpu(tokens), gpu(values))
+    for _ in range(3):
+        out, _ = syn.logits_process(x, 1, bias=bias)
+        assert np.array_equal(out.cpu().numpy(), np.broadcast_to(want, (rows, vocab)))
+
+
 def test_logits_bias_named_twice_counts_twice_and_draft_without_mask_is_a_chain():
     x = torch.zeros(3, 100, device="cuda")
     bias = (gpu(np.array([0, 2], np.int32)), gpu(np.array([5, 5], np.int32)), gpu(np.array([1.5, 2.0], np.float32)))
