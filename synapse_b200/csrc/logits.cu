@@ -15,8 +15,8 @@
 // every value tested where it is held, 107 us (nearly every warp meets a marked
 // token and takes the long way for each of a vector's values); marked tokens
 // done afterwards in global memory, 111 us; marked tokens handed to a thread
-// each through shared memory, 74 us (two barriers a row); as it is, 63 us, of
-// which the bytes are 41 at the copy rate, and with 1024 of history 56. The
+// each through shared memory, 74 us (two barriers a row); as it is, 62 us, of
+// which the bytes are 41 at the copy rate, and with 500 of history 55. The
 // rest is the counting before the first row, one CTA of history per chunk. One
 // row of 128256 takes 5.5 us, launch and counting. The picks are joined
 // by a 64-bit maximum of (ordered value, lowest index), which does not depend on
@@ -31,7 +31,9 @@ namespace {
 
 constexpr int kThreads = 256;
 constexpr int kMaxTree = 1024;
-constexpr int kMaxRows = 8;  // rows (nodes) of one CTA: few enough that the CTAs' number evens out over the SMs
+// Rows (nodes) of one CTA: few enough that the CTAs even out over the SMs, enough to pay for the counts. Measured with 8 /
+// 4 / 2, us: 256 rows of 128256 62.3 / 61.6 / 69.3, 192 rows 48.7 / 44.4 / 47.8, 256 rows of 32000 28.2 / 20.2 / 21.7.
+constexpr int kMaxRows = 4;
 
 struct LogitParams {
     const float* x;

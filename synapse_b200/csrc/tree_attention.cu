@@ -717,13 +717,15 @@ Cut cut_of(int type, int n_seq, int n_tree, int n_head, int n_kv, int head_dim, 
             }
         }
     } else {
-        // one wave of CTAs (two to four waves of shorter parts took 4 to 10 % more); a part has at least two steps of
-        // every warp
+        // one wave of CTAs (two to four waves of shorter parts took 4 to 10 % more).
+        // A part has two steps of every warp, or one while there are no more than the 16 parts that a join loads at a
+        // time (one sequence of 1000: 7.9 -> 7.2 us; of 2000, with 32 parts, 8.0 -> 8.9).
         const bool stack = c.R == 8;
         const int per_sm = type == SYN_F16    ? slots<SYN_F16>(head_dim, stack)
                            : type == SYN_Q8_0 ? slots<SYN_Q8_0>(head_dim, stack)
                                               : slots<SYN_Q4_0>(head_dim, stack);
-        const size_t most = size_t(max_len + 2 * kWarps * kStep - 1) / (2 * kWarps * kStep) * n_seq;
+        const size_t turns = size_t(max_len + kWarps * kStep - 1) / (kWarps * kStep);  // steps of each warp
+        const size_t most = std::max((turns + 1) / 2, std::min<size_t>(turns, 16)) * n_seq;
         c.parts = int(std::min(per_sm * sms / units, most));
     }
     if (c.parts <= n_seq && !(n_seq == 1 && c.parts > 1)) c.parts = 0;
