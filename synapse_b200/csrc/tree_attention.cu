@@ -126,7 +126,8 @@ __device__ __forceinline__ void load_floats(float (&x)[N], const float* p) {
 }
 
 // Joins a row's parts, in their order, by a warp: row `row` of KV head kvh of sequence seq, whose parts' rows in the
-// scratch are `first`, first + pitch, ...
+// scratch are `first`, first + pitch, ...; B parts' loads at a time.
+template <int B>
 __device__ __forceinline__ void join_row(const TreeParams& a, int row, int kvh, int seq, size_t first, size_t pitch, int parts) {
     const int lane = threadIdx.x & 31, hd = a.c.hd;
     const float2* ml = a.part_ml + first;
@@ -147,16 +148,16 @@ __device__ __forceinline__ void join_row(const TreeParams& a, int row, int kvh, 
         const float w = part_weight(s.x, s.y, top);
         sum += warp_sum(w * s.y);
         const int n = min(32, parts - x0);
-        auto half = [&](float4& c, int at, bool here) {  // 16 parts' loads at a time
-            for (int i0 = 0; i0 < n; i0 += 16) {
-                float4 v[16];
+        auto half = [&](float4& c, int at, bool here) {
+            for (int i0 = 0; i0 < n; i0 += B) {
+                float4 v[B];
 #pragma unroll
-                for (int i = 0; i < 16; ++i) {
+                for (int i = 0; i < B; ++i) {
                     v[i] = make_float4(0, 0, 0, 0);
                     if (i0 + i < n && here) v[i] = __ldcg(reinterpret_cast<const float4*>(o + (x0 + i0 + i) * pitch * hd) + at);
                 }
 #pragma unroll
-                for (int i = 0; i < 16; ++i) {
+                for (int i = 0; i < B; ++i) {
                     const float f = __shfl_sync(0xffffffffu, w, (i0 + i) & 31);
                     if (i0 + i < n) add(c, f, v[i]);
                 }
@@ -661,7 +662,7 @@ __global__ void __launch_bounds__(kWarps * 32, Plan<TYPE, HDP, STACK>::ctas) tre
     __syncthreads();
     if (!last) return;
     const size_t first = (size_t(cut.first) * gridDim.y + blockIdx.y) * R;
-    for (int r = warp; r < rows; r += kWarps) join_row(a, row0 + r, kvh, seq, first + r, size_t(gridDim.y) * R, cut.parts);
+    for (int r = warp; r < rows; r += kWarps) join_row<16>(a, row0 + r, kvh, seq, first + r, size_t(gridDim.y) * R, cut.parts);
 }
 
 // Joins the sequences' parts: a warp per row (token, head).
@@ -673,7 +674,7 @@ __global__ void __launch_bounds__(128) tree_join_kernel(const TreeParams a, int 
     const int row = int(id % per_seq) % a.rows, kvh = int(id % per_seq) / a.rows, rb = row / R;
     const Cutting cut = tree_cutting(a, step, 0, seq);
     const size_t unit = size_t(a.c.n_kv) * a.row_blocks;
-    join_row(a, row, kvh, seq, (cut.first * unit + size_t(kvh) * a.row_blocks + rb) * R + row - rb * R, unit * R, cut.parts);
+    join_row<32>(a, row, kvh, seq, (cut.first * unit + size_t(kvh) * a.row_blocks + rb) * R + row - rb * R, unit * R, cut.parts);
 }
 
 // How a call is cut: rows of a CTA, CTAs over the rows, parts of the contexts
