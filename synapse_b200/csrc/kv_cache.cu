@@ -3,7 +3,7 @@
 // been verified. All three move each byte once; they are bound by memory for
 // long inputs and by the launch for a decode step's few rows.
 // Measured with 32 query and 8 KV heads of 128, against the copy rate of 6.5
-// TB/s: 8192 tokens appended to an F16 cache in 66 us (86 %), to Q8_0 in 81 (67
+// TB/s: 8192 tokens appended to an F16 cache in 66 us (86 %), to Q8_0 in 73 (74
 // %: the divisions and roundings of a block are the rest), one token in 1.9 us;
 // 32768 rows read as binary16 in 42 us from Q8_0 (75 %) and in 45 from F16 (92
 // %), as floats from Q8_0 in 71 (73 %). Of append, a load of the next quad ahead
@@ -29,8 +29,8 @@ struct AppendParams {
 // A thread takes 4 dims of a token's rows: n_head heads of q, then n_kv of K,
 // then n_kv of V; 8 neighbouring lanes hold a block of 32. VEC: rows and
 // strides allow 16-byte loads.
-template <int TYPE, bool VEC>
-__global__ void __launch_bounds__(256) kv_append_kernel(AppendParams a) {
+template <int TYPE, bool VEC, int THREADS = 256>
+__global__ void __launch_bounds__(THREADS) kv_append_kernel(AppendParams a) {
     pdl_launch_dependents();
     pdl_wait();
     const int hd = a.c.hd, quads = hd / 4, half = hd / 2;
@@ -315,6 +315,10 @@ extern "C" int syn_kv_append(const syn_kv_cache* c, int layer, const syn_kv_appe
     cudaStream_t s = static_cast<cudaStream_t>(stream);
     if (c->type == SYN_F16)
         return vec ? syn_launch(kv_append_kernel<SYN_F16, true>, grid, 256, 0, s, a) : syn_launch(kv_append_kernel<SYN_F16, false>, grid, 256, 0, s, a);
+    // Q8_0's CTAs of 128 threads pay once there are more than an SM has room for at a time. Measured, 256 / 128 threads, us:
+    // 512 tokens 7.5 / 9.3, 2048 23.6 / 22.0, 8192 81.5 / 73.1 (F16 65.9 / 65.1, Q4_0 75.9 / 80.5).
+    if (c->type == SYN_Q8_0 && tokens > size_t(8) * syn_num_sms())
+        return vec ? syn_launch(kv_append_kernel<SYN_Q8_0, true, 128>, grid, 128, 0, s, a) : syn_launch(kv_append_kernel<SYN_Q8_0, false, 128>, grid, 128, 0, s, a);
     if (c->type == SYN_Q8_0)
         return vec ? syn_launch(kv_append_kernel<SYN_Q8_0, true>, grid, 256, 0, s, a) : syn_launch(kv_append_kernel<SYN_Q8_0, false>, grid, 256, 0, s, a);
     return vec ? syn_launch(kv_append_kernel<SYN_Q4_0, true>, grid, 256, 0, s, a) : syn_launch(kv_append_kernel<SYN_Q4_0, false>, grid, 256, 0, s, a);

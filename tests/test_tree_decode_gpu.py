@@ -133,6 +133,24 @@ def test_append_f16_is_the_sessions_cache():
     assert torch.equal(cache.k.view(torch.int16).flatten(), kc) and torch.equal(cache.v.view(torch.int16).flatten(), vc)
 
 
+@pytest.mark.parametrize("type_", TYPES)
+@pytest.mark.parametrize("n_head,n_kv,hd", [(8, 2, 128), (5, 1, 96)])
+def test_append_of_many_tokens_is_that_of_few(type_, n_head, n_kv, hd):
+    """One call for 1500 tokens and calls of 100: the same bytes and the same rotated queries."""
+    rng = np.random.default_rng(2)
+    n = 1500
+    q, k, v = (gpu(rng.standard_normal((n, h * hd), dtype=np.float32)) for h in (n_head, n_kv, n_kv))
+    slot = gpu(rng.permutation(n).astype(np.int32))
+    table = syn.rope_table(n, hd, 10000.0 ** (-2 / hd))
+    one, many = new_cache(type_, 1, n_kv, hd, n), new_cache(type_, 1, n_kv, hd, n)
+    whole = syn.kv_append(one, k, v, slot, rope_table=table, q=q)
+    for i in range(0, n, 100):
+        part = slice(i, i + 100)
+        got = syn.kv_append(many, k[part], v[part], slot[part], rope_table=table, q=q[part])
+        assert torch.equal(got, whole[part])
+    assert torch.equal(one.k, many.k) and torch.equal(one.v, many.v)
+
+
 @pytest.mark.parametrize("type_", [syn.Q8_0, syn.Q4_0])
 def test_append_stores_finite_values_and_skips_bad_rows(type_):
     hd, ctx = 64, 8
