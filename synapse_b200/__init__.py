@@ -459,19 +459,30 @@ class KVCache:
         self.ref = ctypes.byref(self.desc)
 
 
-def _need(t, dtype, n, where):
-    """The address of a contiguous CUDA tensor of dtype with n elements (None for None)."""
+def _here():
+    """The current device's index: the library launches there."""
+    return _torch()._C._cuda_getDevice()
+
+
+def _need(t, dev, dtype, n, where):
+    """The address of a contiguous tensor of dtype with n elements on device dev, the current one (None for None)."""
     if t is None:
         return None
-    if t.dtype != dtype or not t.is_cuda or t.numel() != n or not t.is_contiguous():
-        raise ValueError(f"{where}: needs a contiguous {dtype} CUDA tensor of {n} elements")
+    if t.dtype != dtype or t.get_device() != dev or t.numel() != n or not t.is_contiguous():
+        raise ValueError(f"{where}: needs a contiguous {dtype} tensor of {n} elements on the current CUDA device")
     return t.data_ptr()
 
 
-def _rows(t, f32, cols, n, where):
+def _room(scratch, dev, n, where):
+    """Refuses a scratch that is not n contiguous bytes on the current device."""
+    if scratch.numel() * scratch.element_size() < n or scratch.get_device() != dev or not scratch.is_contiguous():
+        raise ValueError(f"{where}: needs a contiguous scratch of {n} bytes on the current CUDA device")
+
+
+def _rows(t, dev, f32, cols, n, where):
     """Rows of cols floats whose rows may be strided: (address, floats between rows)."""
-    if t.dtype != f32 or not t.is_cuda or t.shape != (n, cols):
-        raise ValueError(f"{where}: needs {n} float rows of {cols} on the GPU")
+    if t.dtype != f32 or t.get_device() != dev or t.shape != (n, cols):
+        raise ValueError(f"{where}: needs {n} float rows of {cols} on the current CUDA device")
     if t.is_contiguous():
         return t.data_ptr(), cols
     ld = t.stride(0) if n > 1 else cols
@@ -480,9 +491,11 @@ def _rows(t, f32, cols, n, where):
     return t.data_ptr(), ld
 
 
-def _current(device):
-    """The handle of a device's current stream."""
-    return _torch()._C._cuda_getCurrentRawStream(device.index)
+def _current(device, dev):
+    """The handle of the current stream of a device, which has to be dev, the current one."""
+    if device.index != dev:
+        raise ValueError(f"{device} is not the current device")
+    return _torch()._C._cuda_getCurrentRawStream(dev)
 
 
 def _streamed(f):
@@ -507,25 +520,25 @@ def kv_append(cache, k, v, slot, pos=None, rope_table=None, rope_mode=0, q=None,
     """Append tokens' K and V rows [n_seq * n][n_kv * head_dim] at slots (int32, n_seq * n), K rotated when a
     rope_table ([len][head_dim / 2][2]) is given; q [n_seq * n][n_head * head_dim], if given, is rotated too and
     returned."""
-    torch = _torch()
+    torch, dev = _torch(), _here()
     f32, i32 = torch.float32, torch.int32
     tokens, hd = slot.numel(), cache.head_dim
-    kp, ks = _rows(k, f32, cache.n_kv * hd, tokens, "kv_append k")
-    vp, vs = _rows(v, f32, cache.n_kv * hd, tokens, "kv_append v")
+    kp, ks = _rows(k, dev, f32, cache.n_kv * hd, tokens, "kv_append k")
+    vp, vs = _rows(v, dev, f32, cache.n_kv * hd, tokens, "kv_append v")
     if ks != vs or tokens % cache.n_seq:
         raise ValueError("kv_append: k and v must be strided alike, with the same tokens for every sequence")
     qp = op = out = None
     n_head = qs = 0
     if q is not None:
         n_head = q.shape[1] // hd
-        qp, qs = _rows(q, f32, n_head * hd, tokens, "kv_append q")
+        qp, qs = _rows(q, dev, f32, n_head * hd, tokens, "kv_append q")
         out = q.new_empty((tokens, n_head * hd))
         op = out.data_ptr()
     table_len = rope_table.numel() // hd if rope_table is not None else 0
-    a = KVAppendArgs(kp, vp, qp, op, _need(slot, i32, tokens, "slot"), _need(pos, i32, tokens, "pos"),
-                     _need(rope_table, f32, table_len * hd, "rope_table"), ks, qs, tokens // cache.n_seq, n_head,
+    a = KVAppendArgs(kp, vp, qp, op, _need(slot, dev, i32, tokens, "slot"), _need(pos, dev, i32, tokens, "pos"),
+                     _need(rope_table, dev, f32, table_len * hd, "rope_table"), ks, qs, tokens // cache.n_seq, n_head,
                      table_len, rope_mode)
-    check(lib().syn_kv_append(cache.ref, layer, ctypes.byref(a), _current(cache.device)), "syn_kv_append")
+    check(lib().syn_kv_append(cache.ref, layer, ctypes.byref(a), _current(cache.device, dev)), "syn_kv_append")
     return out
 
 
@@ -533,15 +546,15 @@ def kv_append(cache, k, v, slot, pos=None, rope_table=None, rope_mode=0, q=None,
 def kv_read(cache, n, rows=None, first=0, dtype=None, layer=0):
     """n rows of every sequence as values, (k, v) [n_seq][n][n_kv][head_dim]: the cache rows named by `rows` (int32,
     n_seq * n), or first, first + 1, ...; dtype torch.float32 (default) or torch.float16."""
-    torch = _torch()
+    torch, dev = _torch(), _here()
     dtype = dtype or torch.float32
     if dtype not in (torch.float32, torch.float16):
         raise ValueError("kv_read: dtype is torch.float32 or torch.float16")
     shape = (cache.n_seq, n, cache.n_kv, cache.head_dim)
     k, v = cache.k.new_empty(shape, dtype=dtype), cache.k.new_empty(shape, dtype=dtype)
-    check(lib().syn_kv_read(cache.ref, layer, _need(rows, torch.int32, cache.n_seq * n, "rows"), first, n,
+    check(lib().syn_kv_read(cache.ref, layer, _need(rows, dev, torch.int32, cache.n_seq * n, "rows"), first, n,
                             F16 if dtype == torch.float16 else F32, k.data_ptr(), v.data_ptr(),
-                            _current(cache.device)), "syn_kv_read")
+                            _current(cache.device, dev)), "syn_kv_read")
     return k, v
 
 
@@ -549,9 +562,9 @@ def kv_read(cache, n, rows=None, first=0, dtype=None, layer=0):
 def kv_move(cache, path, count, begin):
     """Rows path[s][i] (int32, ascending, >= begin[s] + i) of sequence s become rows begin[s] + i, i < count[s], in
     every layer."""
-    i32, n, ld = _torch().int32, cache.n_seq, path.shape[-1]
-    check(lib().syn_kv_move(cache.ref, _need(path, i32, n * ld, "path"), ld, _need(count, i32, n, "count"),
-                            _need(begin, i32, n, "begin"), _current(cache.device)), "syn_kv_move")
+    i32, dev, n, ld = _torch().int32, _here(), cache.n_seq, path.shape[-1]
+    check(lib().syn_kv_move(cache.ref, _need(path, dev, i32, n * ld, "path"), ld, _need(count, dev, i32, n, "count"),
+                            _need(begin, dev, i32, n, "begin"), _current(cache.device, dev)), "syn_kv_move")
 
 
 def tree_attention_scratch(cache, tree, n_head, max_len=None):
@@ -570,22 +583,22 @@ def _tree_scratch(n, device):
 def tree_attention(cache, q, len, n_head, scale, tree=1, mask=None, max_len=None, out=None, scratch=None, layer=0):
     """Attention of `tree` tokens of every sequence over rows 0 .. len[s] - 1 and the tree's own rows after them that
     their mask bits name (None: a causal chunk); q [n_seq * tree][n_head * head_dim], rotated. See syn_tree_attention."""
-    torch = _torch()
+    torch, dev = _torch(), _here()
     f32, i32 = torch.float32, torch.int32
     cols, rows = n_head * cache.head_dim, cache.n_seq * tree
     max_len = max_len or cache.max_ctx
-    qp, qs = _rows(q, f32, cols, rows, "tree_attention q")
+    qp, qs = _rows(q, dev, f32, cols, rows, "tree_attention q")
     if out is None:
         out = q.new_empty((rows, cols))
     need = _tree_scratch_bytes(cache.n_seq, tree, n_head, cache.n_kv, cache.head_dim, max_len, cache.device)
     if scratch is None:
         scratch = _tree_scratch(need, q.device)
-    elif scratch.numel() * scratch.element_size() < need:
-        raise ValueError(f"tree_attention: scratch of {need} bytes needed")
-    a = TreeAttentionArgs(qp, _need(out, f32, rows * cols, "out"), _need(len, i32, cache.n_seq, "len"),
-                          _need(mask, i32, rows * ((tree + 31) // 32), "mask"), scratch.data_ptr(), qs, tree, n_head,
+    else:
+        _room(scratch, dev, need, "tree_attention")
+    a = TreeAttentionArgs(qp, _need(out, dev, f32, rows * cols, "out"), _need(len, dev, i32, cache.n_seq, "len"),
+                          _need(mask, dev, i32, rows * ((tree + 31) // 32), "mask"), scratch.data_ptr(), qs, tree, n_head,
                           max_len, scale)
-    check(lib().syn_tree_attention(cache.ref, layer, ctypes.byref(a), _current(cache.device)),
+    check(lib().syn_tree_attention(cache.ref, layer, ctypes.byref(a), _current(cache.device, dev)),
           "syn_tree_attention")
     return out
 
@@ -602,23 +615,23 @@ def logits_process(logits, n_seq, penalties=None, history=None, history_len=None
     penalties [n_seq][3] (repeat, presence, frequency), history [n_seq][ld] with history_len [n_seq], the tree's
     tokens draft [n_seq][tree] with mask words, bias (begin [n_seq + 1], tokens, values), allowed [rows][words]. out
     may be logits itself; pick=False leaves the pick out. See syn_logits_process."""
-    torch = _torch()
+    torch, dev = _torch(), _here()
     f32, i32 = torch.float32, torch.int32
     rows, vocab = logits.shape
     tree = rows // n_seq
     if tree * n_seq != rows:
         raise ValueError("logits_process: the same rows for every sequence")
-    xp, ld = _rows(logits, f32, vocab, rows, "logits")
+    xp, ld = _rows(logits, dev, f32, vocab, rows, "logits")
     if out is None:
         out = logits.new_empty((rows, vocab))
-    op, out_ld = _rows(out, f32, vocab, rows, "out")
+    op, out_ld = _rows(out, dev, f32, vocab, rows, "out")
     picks = pp = sp = None
     if pick:
         picks = logits.new_empty(rows, dtype=i32)
         if scratch is None:
             scratch = logits_scratch(rows, logits.device)
-        elif scratch.numel() * scratch.element_size() < (12 * rows + 255) // 256 * 256:  # syn_logits_scratch_bytes
-            raise ValueError("logits_process: the scratch is too small")
+        else:
+            _room(scratch, dev, (12 * rows + 255) // 256 * 256, "logits_process")  # syn_logits_scratch_bytes
         pp, sp = picks.data_ptr(), scratch.data_ptr()
     words = (vocab + 31) // 32
     begin, tokens, values = bias if bias is not None and bias[1].numel() else (None, None, None)
@@ -628,13 +641,13 @@ def logits_process(logits, n_seq, penalties=None, history=None, history_len=None
         if history.dim() != 2:
             raise ValueError("logits_process: history is [n_seq][ld]")
         history_ld = history.shape[1]
-    a = LogitsArgs(xp, op, pp, ld, out_ld, _need(penalties, f32, 3 * n_seq, "penalties"),
-                   _need(history, i32, n_seq * history_ld, "history"), _need(history_len, i32, n_seq, "history_len"),
-                   _need(draft, i32, rows, "draft"), _need(mask, i32, rows * ((tree + 31) // 32), "mask"),
-                   _need(begin, i32, n_seq + 1, "bias begin"), _need(tokens, i32, n, "bias tokens"),
-                   _need(values, f32, n, "bias values"), _need(allowed, i32, rows * words, "allowed"), words, sp,
+    a = LogitsArgs(xp, op, pp, ld, out_ld, _need(penalties, dev, f32, 3 * n_seq, "penalties"),
+                   _need(history, dev, i32, n_seq * history_ld, "history"), _need(history_len, dev, i32, n_seq, "history_len"),
+                   _need(draft, dev, i32, rows, "draft"), _need(mask, dev, i32, rows * ((tree + 31) // 32), "mask"),
+                   _need(begin, dev, i32, n_seq + 1, "bias begin"), _need(tokens, dev, i32, n, "bias tokens"),
+                   _need(values, dev, f32, n, "bias values"), _need(allowed, dev, i32, rows * words, "allowed"), words, sp,
                    n_seq, tree, vocab, history_ld)
-    check(lib().syn_logits_process(ctypes.byref(a), _current(logits.device)), "syn_logits_process")
+    check(lib().syn_logits_process(ctypes.byref(a), _current(logits.device, dev)), "syn_logits_process")
     return out, picks
 
 

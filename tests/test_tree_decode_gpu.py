@@ -767,3 +767,24 @@ def test_refusals():
     with pytest.raises(syn.SynapseError):
         syn.KVCache(syn.Q8_0, 1, 1, 2, 48, 32)
     torch.cuda.synchronize()
+
+
+def test_refuses_tensors_that_are_not_on_the_current_device(monkeypatch):
+    """As with a second GPU current: nothing is launched."""
+    cache = new_cache(syn.Q8_0, 1, 2, 64, 32)
+    i = gpu(np.zeros(1, np.int32))
+    x, q = gpu(np.zeros((1, 128), np.float32)), gpu(np.zeros((1, 256), np.float32))
+    scratch, small = syn.tree_attention_scratch(cache, 1, 4), syn.logits_scratch(1)
+    monkeypatch.setattr(syn, "_here", lambda: 1)
+    for call in (lambda: syn.kv_append(cache, x, x, i), lambda: syn.kv_read(cache, 1), lambda: syn.kv_move(cache, i, i, i),
+                 lambda: syn.tree_attention(cache, q, i, 4, 1.0, scratch=scratch),
+                 lambda: syn.logits_process(x, 1, scratch=small)):
+        with pytest.raises(ValueError, match="current"):
+            call()
+    monkeypatch.undo()
+    for call in (lambda: syn.kv_append(cache, x.cpu(), x, i), lambda: syn.tree_attention(cache, q, i.cpu(), 4, 1.0, scratch=scratch),
+                 lambda: syn.logits_process(x.cpu(), 1), lambda: syn.logits_process(x, 1, scratch=small.cpu()),
+                 lambda: syn.tree_attention(cache, q, i, 4, 1.0, scratch=scratch.cpu()),
+                 lambda: syn.tree_attention(cache, q, i, 4, 1.0, scratch=scratch.new_zeros(2 * scratch.numel())[::2])):
+        with pytest.raises(ValueError, match="current"):
+            call()
