@@ -352,6 +352,14 @@ def test_attention_of_many_ragged_sequences(type_, tree):
 
 
 @pytest.mark.parametrize("type_", TYPES)
+def test_tree_attention_of_many_ragged_sequences(type_):
+    """Trees of 40 tokens in more sequences than the GPU has room for at a time, one of several parts."""
+    lens = [int(x) for x in np.random.default_rng(3).integers(0, 90, 170)]
+    lens[5], lens[169] = 900, 0
+    check_attention(type_, 4, 2, 64, lens, 40, seed=1)
+
+
+@pytest.mark.parametrize("type_", TYPES)
 @pytest.mark.parametrize("lens,tree", [([0], 70), ([100, 37], 9)])
 def test_causal_chunk(type_, lens, tree):
     check_attention(type_, 6, 2, 64, lens, tree, seed=3, mask=None)
