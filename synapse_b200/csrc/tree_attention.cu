@@ -194,6 +194,7 @@ __global__ void __launch_bounds__(kWarps * 32, Plan<TYPE, HDP, STACK>::ctas) tre
     int seq = -1;
     const Cutting cut = tree_cutting(a, kStep, blockIdx.x, seq);
     if (seq < 0) return;
+    note_cut(a, cut, seq);
     const int len = tree_len(a, seq), total = len + a.n_tree;
     const int steps = (total + kStep - 1) / kStep;
     const int s0 = (int(blockIdx.x) - cut.first) * cut.per, s1 = cut.per < steps - s0 ? s0 + cut.per : steps;
@@ -665,16 +666,19 @@ __global__ void __launch_bounds__(kWarps * 32, Plan<TYPE, HDP, STACK>::ctas) tre
     for (int r = warp; r < rows; r += kWarps) join_row<16>(a, row0 + r, kvh, seq, first + r, size_t(gridDim.y) * R, cut.parts);
 }
 
-// Joins the sequences' parts: a warp per row (token, head).
-__global__ void __launch_bounds__(128) tree_join_kernel(const TreeParams a, int R, int step) {
+// Joins the sequences' parts: a warp per row (token, head), whose cutting the first kernel has left in the scratch. The
+// few-row kernel's parts are many, 32 at a time (16 rows of 8192 in Q8_0 18.0 us, against 19.5 with 16); of the other
+// kernel there are few parts and many rows, and more registers mean fewer warps on an SM (16 sequences of 1000, 64 rows,
+// F16: 33 us with 8 at a time, 36 with 16, 56 with 32 and the cutting found again by every warp).
+template <int B>
+__global__ void __launch_bounds__(128) tree_join_kernel(const TreeParams a, int R) {
     pdl_wait();
     const unsigned id = blockIdx.x * 4 + (threadIdx.x >> 5), per_seq = unsigned(a.c.n_kv) * a.rows;
     if (id >= unsigned(a.c.n_seq) * per_seq) return;
-    int seq = int(id / per_seq);
-    const int row = int(id % per_seq) % a.rows, kvh = int(id % per_seq) / a.rows, rb = row / R;
-    const Cutting cut = tree_cutting(a, step, 0, seq);
+    const int seq = int(id / per_seq), row = int(id % per_seq) % a.rows, kvh = int(id % per_seq) / a.rows, rb = row / R;
+    const int2 cut = __ldcg(a.cuts + seq);
     const size_t unit = size_t(a.c.n_kv) * a.row_blocks;
-    join_row<32>(a, row, kvh, seq, (cut.first * unit + size_t(kvh) * a.row_blocks + rb) * R + row - rb * R, unit * R, cut.parts);
+    join_row<B>(a, row, kvh, seq, (cut.x * unit + size_t(kvh) * a.row_blocks + rb) * R + row - rb * R, unit * R, cut.y);
 }
 
 // How a call is cut: rows of a CTA, CTAs over the rows, parts of the contexts
@@ -766,7 +770,7 @@ extern "C" size_t syn_tree_attention_scratch_bytes(int n_seq, int n_tree, int n_
     size_t rows = 0;  // the most of any type
     for (int type : {SYN_F16, SYN_Q8_0, SYN_Q4_0})
         rows = std::max(rows, cut_of(type, n_seq, n_tree, n_head, n_kv, head_dim, max_len).rows);
-    return kCounterBytes + align256(rows * 8) + align256(rows * head_dim * 4);
+    return kCounterBytes + align256(size_t(n_seq) * 8) + align256(rows * 8) + align256(rows * head_dim * 4);
 }
 
 extern "C" int syn_tree_attention(const syn_kv_cache* c, int layer, const syn_tree_attention_args* x, void* stream) {
@@ -786,8 +790,10 @@ extern "C" int syn_tree_attention(const syn_kv_cache* c, int layer, const syn_tr
     a.q = x->q; a.out = x->out; a.len = x->len; a.mask = x->mask;
     char* scratch = static_cast<char*>(x->scratch);
     a.arrived = cut.parts && !cut.join ? reinterpret_cast<unsigned*>(scratch) : nullptr;
-    a.part_ml = reinterpret_cast<float2*>(scratch + kCounterBytes);
-    a.part_o = reinterpret_cast<float*>(scratch + kCounterBytes + align256(cut.rows * 8));
+    a.cuts = cut.join ? reinterpret_cast<int2*>(scratch + kCounterBytes) : nullptr;
+    scratch += kCounterBytes + align256(size_t(c->n_seq) * 8);
+    a.part_ml = reinterpret_cast<float2*>(scratch);
+    a.part_o = reinterpret_cast<float*>(scratch + align256(cut.rows * 8));
     a.q_stride = x->q_stride ? x->q_stride : q_row;
     a.n_tree = x->n_tree; a.n_head = x->n_head;
     a.group = x->n_head / c->n_kv;
@@ -804,5 +810,6 @@ extern "C" int syn_tree_attention(const syn_kv_cache* c, int layer, const syn_tr
     else st = launch_type<SYN_Q4_0>(a, cut, s);
     if (st || !cut.join) return st;
     const size_t rows = size_t(c->n_seq) * c->n_kv * a.rows;
-    return syn_launch_pdl(true, tree_join_kernel, unsigned((rows + 3) / 4), 128, 0, s, a, cut.R, cut.tc ? kTcTile : kStep);
+    if (cut.tc) return syn_launch_pdl(true, tree_join_kernel<8>, unsigned((rows + 3) / 4), 128, 0, s, a, cut.R);
+    return syn_launch_pdl(true, tree_join_kernel<32>, unsigned((rows + 3) / 4), 128, 0, s, a, cut.R);
 }

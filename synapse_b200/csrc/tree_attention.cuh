@@ -15,6 +15,7 @@ struct TreeParams {
     const int32_t* len;
     const uint32_t* mask;
     unsigned* arrived;   // [n_seq][n_kv * row blocks]: parts that are done; zero between calls
+    int2* cuts;          // [n_seq]: a sequence's first part and number of parts, for tree_join_kernel
     float2* part_ml;     // [parts][n_kv * row blocks][R]: a part's maximum and sum of a row
     float* part_o;       // [parts][n_kv * row blocks][R][hd]: its output, not divided
     size_t q_stride;
@@ -146,6 +147,10 @@ __device__ __forceinline__ Cutting tree_cutting(const TreeParams& a, int step, i
         before += __shfl_sync(0xffffffffu, sum, 31);
     }
     return {per, 0, 0};
+}
+// By every CTA of a kernel whose parts tree_join_kernel joins.
+__device__ __forceinline__ void note_cut(const TreeParams& a, const Cutting& cut, int seq) {
+    if (a.cuts && threadIdx.x == 0 && blockIdx.y == 0 && int(blockIdx.x) == cut.first) a.cuts[seq] = make_int2(cut.first, cut.parts);
 }
 // Whether token tk of sequence seq sees the tree's row j >= 0.
 __device__ __forceinline__ bool tree_sees(const TreeParams& a, int seq, int tk, int j) {
