@@ -22,13 +22,13 @@
 // Bound: the products take 16 (F16) or 24 cycles per position and KV head
 // whatever the number of rows up to 128, against 22 (F16), 12 (Q8_0) or 6
 // (Q4_0) for the cache's bytes at head_dim 128. Measured: 64 tokens of 64 heads
-// over 32768 F16 positions 141 us, the tensor cores busy 45 % of it: a tile
+// over 32768 F16 positions 138 us, the tensor cores busy 45 % of it: a tile
 // takes some 2000 cycles of 1024, and leaving out the exponentials, the splitting
 // or the reading of O changes that by 4 to 9 %: the roles wait for one
 // another's latency. Before its first tile a CTA needs 9000 cycles (its 64 KB
 // of q to tensor memory, the first tile), after the last 5000 (64 KB of O), which
 // is most of a short context's time (32 rows of 8192 positions: 20 us).
-// Tried and slower: two groups of softmax warps on alternate tiles (144 us), two
+// Tried and slower: two groups of softmax warps on alternate tiles (3 us more), two
 // threads a row, the products issued by the oldest warp, the exponents by tile
 // with a barrier, polling instead of sleeping waits, rolled loops.
 #include "tcgen05.cuh"
