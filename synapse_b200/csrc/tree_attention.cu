@@ -26,9 +26,13 @@
 // the sum over blocks of scale * (q . quants); for V the block's scale is
 // m * 2^e, 2^e <= 2^5 applied to the integers (exact) and m (in [1, 2) unless
 // the scale is beyond 2^6) to the float probabilities before they are split, so no
-// value is rounded to binary16. Each step's output is added to float registers
-// outside the tensor core, whose accumulation truncates: kept there over 64
-// steps it cost 2e-6.
+// value is rounded to binary16. Probabilities carry 2^8, and 2^8 m is within binary16
+// up to scales of 8188; beyond them a warp's output is NaN, and a warp that ends its
+// steps with NaN goes through them again with m / 16 (m < 2^11). No append writes such
+// scales, and so they cost the other caches nothing in the steps (measured over 17
+// shapes: 0.8 % more time, against 2 to 3 % with the scales tested at every step). Each
+// step's output is added to float registers outside the tensor core, whose accumulation
+// truncates: kept there over 64 steps it cost 2e-6.
 //
 // Up to 8 rows, the usual decode step, the two terms share one product of 16
 // rows: the high terms are rows 0-7, the low ones rows 8-15, and their results
@@ -262,13 +266,17 @@ __global__ void __launch_bounds__(kWarps * 32, Plan<TYPE, HDP, STACK>::ctas) tre
         for (int i = tid; i < P::ring / 16; i += kWarps * 32) reinterpret_cast<uint4*>(ring)[i] = make_uint4(0, 0, 0, 0);
         __syncthreads();
     }
-    int next = s0 + warp;  // the next step to request
+    int next;  // the next step to request
+    auto request_first = [&] {
+        next = s0 + warp;
 #pragma unroll
-    for (int i = 0; i < P::stages - 1; ++i) {
-        if (next < s1) load(next, i);
-        cp_commit();
-        next += kWarps;
-    }
+        for (int i = 0; i < P::stages - 1; ++i) {
+            if (next < s1) load(next, i);
+            cp_commit();
+            next += kWarps;
+        }
+    };
+    request_first();
 
     // --- q: scaled to a row maximum in [2^8, 2^9), split, in the order of the K fragments -------
 #pragma unroll
@@ -315,6 +323,12 @@ __global__ void __launch_bounds__(kWarps * 32, Plan<TYPE, HDP, STACK>::ctas) tre
     for (int u = 0; u < NR; ++u) {
         rs[u] = row_scale[8 * u + g];
         tok[u] = (row0 + 8 * u + g) / a.group;
+    }
+    bool low = false;  // quantised: V's factors m are divided by 16 (a second pass)
+    // --- the steps of this warp ----------------------------------------------------
+[[maybe_unused]] pass:
+#pragma unroll
+    for (int u = 0; u < NR; ++u) {
         m[u] = -INFINITY;
         l[u] = 0.0f;
     }
@@ -322,8 +336,6 @@ __global__ void __launch_bounds__(kWarps * 32, Plan<TYPE, HDP, STACK>::ctas) tre
     for (int n = 0; n < HDP / 8; ++n)
 #pragma unroll
         for (int e = 0; e < 2 * NR; ++e) o[n][e] = 0.0f;
-
-    // --- the steps of this warp ----------------------------------------------------
     int stage = 0;
     for (int step = s0 + warp; step < s1; step += kWarps) {
         cp_wait<P::stages - 2>();
@@ -359,6 +371,9 @@ __global__ void __launch_bounds__(kWarps * 32, Plan<TYPE, HDP, STACK>::ctas) tre
                 vms[id] = finite ? f16_from_bits(uint16_t(dv)) * inv : 0.0f;
                 ves[((r >> 1) * NB + b) * 2 + (r & 1)] = uint16_t(pow);
             }
+            if (low)
+#pragma unroll 1
+                for (int i = 0; i < kStep * NB / 32; ++i) vms[i * 32 + lane] *= 0.0625f;
             __syncwarp();
         }
 
@@ -596,6 +611,25 @@ __global__ void __launch_bounds__(kWarps * 32, Plan<TYPE, HDP, STACK>::ctas) tre
         if (++stage == P::stages) stage = 0;
     }
     cp_wait<0>();
+    if constexpr (kQuant) {  // NaN: a scale above 8188, or values that are not finite
+        bool nan = false;
+#pragma unroll
+        for (int n = 0; n < HDP / 8; ++n)
+#pragma unroll
+            for (int e = 0; e < 2 * NR; ++e) nan |= o[n][e] != o[n][e];
+        if (!low) {
+            if (__any_sync(0xffffffffu, nan)) {
+                low = true;
+                request_first();
+                goto pass;
+            }
+        } else {
+#pragma unroll
+            for (int n = 0; n < HDP / 8; ++n)
+#pragma unroll
+                for (int e = 0; e < 2 * NR; ++e) o[n][e] *= 16.0f;
+        }
+    }
     __syncthreads();  // every warp is done with the ring
 
     // --- the warps' results joined --------------------------------------------------

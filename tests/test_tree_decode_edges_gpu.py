@@ -1,0 +1,71 @@
+"""Tree attention and its caches at the edges of their types. Tolerances are those of test_tree_decode_gpu.py."""
+import numpy as np
+import pytest
+
+pytestmark = pytest.mark.gpu
+torch = pytest.importorskip("torch")
+syn = pytest.importorskip("synapse_b200")
+from tests.test_tree_decode_gpu import exact_attention, fill, gpu, new_cache, random_masks, values  # noqa: E402
+
+# rows of a KV head on either side of every change of kernel: 1, 8, 12, 32 and 36
+ROWS = [(2, 1), (8, 2), (6, 4), (8, 8), (24, 3)]
+
+
+def scales(cache, which):
+    """The scales of a quantised cache of one layer as a view, [n_seq][n_kv][ctx][hd / 32] binary16."""
+    n, kv, hd, ctx = cache.n_seq, cache.n_kv, cache.head_dim, cache.max_ctx
+    at = (kv * ctx * hd // (1 if cache.type == syn.Q8_0 else 2) + 255) // 256 * 256
+    raw = (cache.k if which == 0 else cache.v)[0]
+    return raw[:, at:at + kv * ctx * hd // 16].view(torch.float16).view(n, kv, ctx, hd // 32)
+
+
+def check_against_64_bits(cache, q, lens, tree, words, sees, n_head, scale):
+    got = syn.tree_attention(cache, gpu(q), gpu(np.array(lens, np.int32)), n_head, scale, tree=tree, mask=gpu(words))
+    q64 = q.astype(np.float64).reshape(len(lens), tree, n_head, cache.head_dim)
+    want, bound = exact_attention(q64, values(cache, 0), values(cache, 1), lens, sees, n_head, scale)
+    got = got.cpu().numpy().astype(np.float64).reshape(want.shape)
+    assert np.isfinite(got).all()
+    assert (np.abs(got - want) <= bound[..., None]).all(), np.abs(got - want).max()
+    assert np.linalg.norm(got - want) <= 1e-5 * np.linalg.norm(want)
+
+
+# ---- scales ---------------------------------------------------------------------------------------------------------
+@pytest.mark.parametrize("type_", [syn.Q8_0, syn.Q4_0])
+@pytest.mark.parametrize("hd", [64, 128, 256])
+@pytest.mark.parametrize("n_head,tree", ROWS)
+@pytest.mark.parametrize("where", ["all", "some", "tree"])
+def test_attention_over_scales_of_any_finite_size(type_, hd, n_head, tree, where):
+    """V's scales up to binary16's largest, of both signs, in every row, in a row here and there or in the tree's own."""
+    rng = np.random.default_rng(hd + tree)
+    n_kv, lens = 2, [400, 37]
+    cache = new_cache(type_, 2, n_kv, hd, 400 + tree)
+    fill(cache, rng, 400 + tree)
+    d = scales(cache, 1)
+    big = np.float16(rng.choice([8188, -8188, 8192, -8192, 10000, -16384, 40000, 65504, -65504, 4.0], d.shape))
+    at = np.zeros(d.shape, bool)
+    if where == "all":
+        at[:] = True
+    elif where == "some":
+        at = rng.random(d.shape) < 0.01
+        at[:, :, 5] = True
+    else:
+        for s, n in enumerate(lens):
+            at[s, :, n:n + tree] = True
+    d.copy_(torch.where(gpu(at), gpu(big), d))
+    q = rng.standard_normal((2 * tree, n_head * hd), dtype=np.float32) * np.float32(1.5)
+    words, sees = random_masks(rng, 2, tree)
+    check_against_64_bits(cache, q, lens, tree, words, sees, n_head, hd ** -0.5)
+
+
+@pytest.mark.parametrize("type_", [syn.Q8_0, syn.Q4_0])
+@pytest.mark.parametrize("n_head,tree", ROWS)
+def test_attention_over_large_scales_of_keys(type_, n_head, tree):
+    rng = np.random.default_rng(tree)
+    hd, lens = 64, [90, 300]
+    cache = new_cache(type_, 2, 2, hd, 300 + tree)
+    fill(cache, rng, 300 + tree)
+    d = scales(cache, 0)
+    d.copy_(gpu(np.float16(rng.choice([65504, -65504, 8192, 100], d.shape))))
+    q = rng.standard_normal((2 * tree, n_head * hd), dtype=np.float32) * np.float32(1e-6)
+    words, sees = random_masks(rng, 2, tree)
+    check_against_64_bits(cache, q, lens, tree, words, sees, n_head, hd ** -0.5)
