@@ -27,12 +27,13 @@
 // m * 2^e, 2^e <= 2^5 applied to the integers (exact) and m (in [1, 2) unless
 // the scale is beyond 2^6) to the float probabilities before they are split, so no
 // value is rounded to binary16. Probabilities carry 2^8, and 2^8 m is within binary16
-// up to scales of 8188; beyond them a warp's output is NaN, and a warp that ends its
-// steps with NaN goes through them again with m / 16 (m < 2^11). No append writes such
-// scales, and so they cost the other caches nothing in the steps (measured over 17
-// shapes: 0.8 % more time, against 2 to 3 % with the scales tested at every step). Each
-// step's output is added to float registers outside the tensor core, whose accumulation
-// truncates: kept there over 64 steps it cost 2e-6.
+// up to scales of 8188; beyond them a row's output is NaN, and a warp that ends its
+// steps with such rows goes through them again with those rows' maximum known and
+// raised by 4, for probabilities of up to 2^4 (m < 2^11); the other rows come out the
+// same. No append writes such scales, so the steps themselves do not ask for them
+// (measured over 17 shapes: 1.2 % more time, against 2 to 3 % with the scales tested at
+// every step). Each step's output is added to float registers outside the tensor core,
+// whose accumulation truncates: kept there over 64 steps it cost 2e-6.
 //
 // Up to 8 rows, the usual decode step, the two terms share one product of 16
 // rows: the high terms are rows 0-7, the low ones rows 8-15, and their results
@@ -323,15 +324,14 @@ __global__ void __launch_bounds__(kWarps * 32, Plan<TYPE, HDP, STACK>::ctas) tre
     for (int u = 0; u < NR; ++u) {
         rs[u] = row_scale[8 * u + g];
         tok[u] = (row0 + 8 * u + g) / a.group;
+        m[u] = -INFINITY;
     }
-    bool low = false;  // quantised: V's factors m are divided by 16 (a second pass)
+    bool again = false;
+
     // --- the steps of this warp ----------------------------------------------------
 [[maybe_unused]] pass:
 #pragma unroll
-    for (int u = 0; u < NR; ++u) {
-        m[u] = -INFINITY;
-        l[u] = 0.0f;
-    }
+    for (int u = 0; u < NR; ++u) l[u] = 0.0f;
 #pragma unroll
     for (int n = 0; n < HDP / 8; ++n)
 #pragma unroll
@@ -371,9 +371,6 @@ __global__ void __launch_bounds__(kWarps * 32, Plan<TYPE, HDP, STACK>::ctas) tre
                 vms[id] = finite ? f16_from_bits(uint16_t(dv)) * inv : 0.0f;
                 ves[((r >> 1) * NB + b) * 2 + (r & 1)] = uint16_t(pow);
             }
-            if (low)
-#pragma unroll 1
-                for (int i = 0; i < kStep * NB / 32; ++i) vms[i * 32 + lane] *= 0.0625f;
             __syncwarp();
         }
 
@@ -611,23 +608,25 @@ __global__ void __launch_bounds__(kWarps * 32, Plan<TYPE, HDP, STACK>::ctas) tre
         if (++stage == P::stages) stage = 0;
     }
     cp_wait<0>();
-    if constexpr (kQuant) {  // NaN: a scale above 8188, or values that are not finite
-        bool nan = false;
+    if constexpr (kQuant) {
+        if (!again) {  // NaN in a row: a scale above 8188, or values that are not finite
+            unsigned who[NR], any = 0;
 #pragma unroll
-        for (int n = 0; n < HDP / 8; ++n)
+            for (int u = 0; u < NR; ++u) {
+                bool nan = false;
 #pragma unroll
-            for (int e = 0; e < 2 * NR; ++e) nan |= o[n][e] != o[n][e];
-        if (!low) {
-            if (__any_sync(0xffffffffu, nan)) {
-                low = true;
+                for (int n = 0; n < HDP / 8; ++n) nan |= o[n][2 * u] != o[n][2 * u] || o[n][2 * u + 1] != o[n][2 * u + 1];
+                who[u] = __ballot_sync(0xffffffffu, nan);
+                any |= who[u];
+            }
+            if (any) {  // the other rows come out as before; a maximum to which 4 adds nothing goes up to the next float
+#pragma unroll
+                for (int u = 0; u < NR; ++u)
+                    m[u] = who[u] >> (lane & 28) & 15u ? m[u] + fmaxf(4.0f, fabsf(m[u]) * 0x1p-23f) : -INFINITY;
+                again = true;
                 request_first();
                 goto pass;
             }
-        } else {
-#pragma unroll
-            for (int n = 0; n < HDP / 8; ++n)
-#pragma unroll
-                for (int e = 0; e < 2 * NR; ++e) o[n][e] *= 16.0f;
         }
     }
     __syncthreads();  // every warp is done with the ring

@@ -69,3 +69,22 @@ def test_attention_over_large_scales_of_keys(type_, n_head, tree):
     q = rng.standard_normal((2 * tree, n_head * hd), dtype=np.float32) * np.float32(1e-6)
     words, sees = random_masks(rng, 2, tree)
     check_against_64_bits(cache, q, lens, tree, words, sees, n_head, hd ** -0.5)
+
+
+@pytest.mark.parametrize("type_", [syn.Q8_0, syn.Q4_0])
+@pytest.mark.parametrize("hd", [64, 96, 128, 256])
+@pytest.mark.parametrize("n_head,tree", [(4, 4), (4, 8), (24, 3)])
+def test_large_scales_change_nothing_for_who_does_not_see_them(type_, hd, n_head, tree):
+    rng = np.random.default_rng(hd + tree)
+    n_kv, L = 2, 200
+    cache = new_cache(type_, 1, n_kv, hd, L + tree)
+    fill(cache, rng, L + tree)
+    words, sees = random_masks(rng, 1, tree)
+    q = gpu(rng.standard_normal((tree, n_head * hd), dtype=np.float32))
+    lens = gpu(np.array([L], np.int32))
+    want = syn.tree_attention(cache, q, lens, n_head, 0.125, tree=tree, mask=gpu(words)).view(tree, n_head, hd)
+    scales(cache, 1)[0, 1, L + 1] = 65504.0
+    got = syn.tree_attention(cache, q, lens, n_head, 0.125, tree=tree, mask=gpu(words)).view(tree, n_head, hd)
+    hit = sees[0, :, 1]
+    assert torch.equal(got[~hit], want[~hit]) and torch.equal(got[:, :n_head // 2], want[:, :n_head // 2])
+    assert got.isfinite().all() and (got[hit][:, n_head // 2:] != want[hit][:, n_head // 2:]).any()
