@@ -322,8 +322,10 @@ int syn_kv_move(const syn_kv_cache* c, const int32_t* path, int path_ld, const i
  * or block values of the cache as stored; q, the probabilities and every sum
  * keep 22 bits or more (about 1e-6 relative). A token that sees nothing gets
  * zeros. What masked rows hold, infinities and NaN included, reaches no
- * output; a token that sees a row with a value that is not finite gets NaN in
- * the heads that read it.
+ * output. A token that sees a row with a value of K that is not finite gets
+ * NaN in the heads that read it; so it does for a value of V, but for the
+ * committed rows of an F16 cache: there the dim of the value is infinite or
+ * NaN and the others are as they are.
  * len[s] is clamped to [0, max_len - n_tree]; max_len <= max_ctx bounds
  * len[s] + n_tree and sizes the split of the context over the GPU.
  * scratch: syn_tree_attention_scratch_bytes, 16-byte aligned, its first 4096

@@ -359,15 +359,16 @@ __global__ void __launch_bounds__(kWarps * 32, Plan<TYPE, HDP, STACK>::ctas) tre
 #pragma unroll
             for (int i = 0; i < kStep * NB / 32; ++i) {
                 const int id = i * 32 + lane, r = id / NB, b = id % NB;
-                // a position past the context has scales of 0; one whose V scale is not finite scores NaN (rows
-                // that do not see it mask that)
+                // a position past the context has scales of 0; one with a scale that is not finite scores NaN (rows
+                // that do not see it mask that): of K by an infinity times 0
                 const bool ok = p0 + r < total && b < nb;
                 const uint32_t dk = ok ? reinterpret_cast<const uint16_t*>(st + S::sk_at + scale_off)[r * nb + b] : 0u;
                 const uint32_t dv = ok ? reinterpret_cast<const uint16_t*>(st + S::sv_at + scale_off)[r * nb + b] : 0u;
                 const bool finite = (dv & 0x7c00u) != 0x7c00u;
                 const uint32_t pow = finite ? min(max(dv & 0x7c00u, 0x0400u), 0x5000u) : 0x0400u;  // 2^-14 .. 2^5: 1152 * 2^5 is finite
                 const float inv = __uint_as_float(0x7f000000u - __float_as_uint(f16_from_bits(uint16_t(pow))));
-                kds[id] = finite ? f16_from_bits(uint16_t(dk)) : __uint_as_float(0x7fffffffu);
+                const float kd = f16_from_bits(uint16_t(dk));
+                kds[id] = finite ? __fmaf_rn(kd, 0.0f, kd) : __uint_as_float(0x7fffffffu);
                 vms[id] = finite ? f16_from_bits(uint16_t(dv)) * inv : 0.0f;
                 ves[((r >> 1) * NB + b) * 2 + (r & 1)] = uint16_t(pow);
             }
@@ -460,6 +461,13 @@ __global__ void __launch_bounds__(kWarps * 32, Plan<TYPE, HDP, STACK>::ctas) tre
                 }
             }
         }
+
+        // an infinity in K may score -inf, which would drop its row in silence: NaN
+        if (!kQuant)
+#pragma unroll
+            for (int u = 0; u < 2; ++u)
+#pragma unroll
+                for (int e = 0; e < 2 * NR; e += 2) fma2(s[u][e], s[u][e + 1], 0.0f, 0.0f, s[u][e], s[u][e + 1]);
 
         // the tree's own rows: what a token does not see scores -inf
         const bool edge = p0 + kStep > len;

@@ -279,6 +279,11 @@ __global__ void __launch_bounds__(kTcThreads, 1) tree_attn_tc_kernel(const TreeP
                         fma2(v[0], v[1], c, c, vl.x, vl.y);
                         fma2(v[2], v[3], c, c, vl.z, vl.w);
                     });
+                else  // an infinity in K may score -inf, which would drop its row in silence: NaN (as a quantised one's low term is)
+                    each4([&](float(&v)[4], int) {
+                        fma2(v[0], v[1], 0.0f, 0.0f, v[0], v[1]);
+                        fma2(v[2], v[3], 0.0f, 0.0f, v[2], v[3]);
+                    });
                 if (edge) {
                     const unsigned long long bad = sh.bad[t - edge0], sees = tile_sees(a, seq, tok, t * kTcTile - len);
                     const uint32_t bw[2] = {uint32_t(bad), uint32_t(bad >> 32)}, sw[2] = {uint32_t(sees), uint32_t(sees >> 32)};
@@ -502,8 +507,10 @@ __global__ void __launch_bounds__(kTcThreads, 1) tree_attn_tc_kernel(const TreeP
                 const bool v = i >= NI;
                 const int ii = v ? i - NI : i, p = ii * PS + lp;
                 uint32_t top = d[k] & 0x7fffu;
-                if (__any_sync(0xffffffffu, top >= 0x7c00u)) {  // not finite: a tree row's position is bad, NaN for who sees it
+                bool bad = false;  // the position's row: NaN for who sees it, by its logarithm (V) or its values (K)
+                if (__any_sync(0xffffffffu, top >= 0x7c00u)) {
                     const int t = t0 + j;
+                    bad = __ballot_sync(0xffffffffu, top >= 0x7c00u) >> (lane - ch) & ((1u << CP) - 1u);
                     if (top >= 0x7c00u) {
                         if (t * kTcTile + p >= len) {
                             d[k] = 0;
@@ -521,7 +528,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) tree_attn_tc_kernel(const TreeP
                     if (!v) {
                         sh.k_pow[st][p] = down;
                     } else {
-                        sh.v_log[st][p] = float(int(e) - 23);
+                        sh.v_log[st][p] = bad ? __uint_as_float(0x7fffffffu) : float(int(e) - 23);
                         sh.v_inv[st][p] = up;
                     }
                 }

@@ -7,6 +7,7 @@ torch = pytest.importorskip("torch")
 syn = pytest.importorskip("synapse_b200")
 from tests.test_tree_decode_gpu import exact_attention, fill, gpu, new_cache, random_masks, values  # noqa: E402
 
+TYPES = [syn.F16, syn.Q8_0, syn.Q4_0]
 # rows of a KV head on either side of every change of kernel: 1, 8, 12, 32 and 36
 ROWS = [(2, 1), (8, 2), (6, 4), (8, 8), (24, 3)]
 
@@ -17,6 +18,19 @@ def scales(cache, which):
     at = (kv * ctx * hd // (1 if cache.type == syn.Q8_0 else 2) + 255) // 256 * 256
     raw = (cache.k if which == 0 else cache.v)[0]
     return raw[:, at:at + kv * ctx * hd // 16].view(torch.float16).view(n, kv, ctx, hd // 32)
+
+
+def rows16(cache, which):
+    """An F16 cache of one layer as a view, [n_seq][ctx][n_kv][hd]."""
+    raw = (cache.k if which == 0 else cache.v)[0]
+    return raw.view(torch.float16).view(cache.n_seq, cache.max_ctx, cache.n_kv, cache.head_dim)
+
+
+def copy_of(cache):
+    c = new_cache(cache.type, cache.n_seq, cache.n_kv, cache.head_dim, cache.max_ctx)
+    c.k.copy_(cache.k)
+    c.v.copy_(cache.v)
+    return c
 
 
 def check_against_64_bits(cache, q, lens, tree, words, sees, n_head, scale):
@@ -88,3 +102,42 @@ def test_large_scales_change_nothing_for_who_does_not_see_them(type_, hd, n_head
     hit = sees[0, :, 1]
     assert torch.equal(got[~hit], want[~hit]) and torch.equal(got[:, :n_head // 2], want[:, :n_head // 2])
     assert got.isfinite().all() and (got[hit][:, n_head // 2:] != want[hit][:, n_head // 2:]).any()
+
+
+# ---- values that are not finite -------------------------------------------------------------------------------------
+@pytest.mark.parametrize("type_", TYPES)
+@pytest.mark.parametrize("hd", [64, 96, 128, 256])
+@pytest.mark.parametrize("n_head,tree", [(4, 4), (24, 3)])
+@pytest.mark.parametrize("which", [0, 1])
+def test_one_value_that_is_not_finite(type_, hd, n_head, tree, which):
+    """An infinity or NaN in one value of K (which = 0) or V: tokens that do not see its row and heads that do not read
+    it are as without it. Who sees it gets NaN in the heads that read it, whatever the signs; of V in a committed row of
+    an F16 cache, something that is not finite in the dim concerned, and the others as they were."""
+    rng = np.random.default_rng(hd + tree)
+    n_kv, lens = 2, [70, 200]
+    group = n_head // n_kv
+    cache = new_cache(type_, 2, n_kv, hd, 200 + tree)
+    fill(cache, rng, 200 + tree)
+    words, sees = random_masks(rng, 2, tree)
+    q = gpu(rng.standard_normal((2 * tree, n_head * hd), dtype=np.float32))
+    args = dict(tree=tree, mask=gpu(words))
+    lens_gpu = gpu(np.array(lens, np.int32))
+    want = syn.tree_attention(cache, q, lens_gpu, n_head, 0.125, **args).view(2, tree, n_head, hd)
+    for bad in (float("inf"), -float("inf"), float("nan")):
+        for row in (3, lens[1] + 1):  # committed, and the tree's
+            c = copy_of(cache)
+            dim = int(rng.integers(hd))
+            if type_ == syn.F16:
+                rows16(c, which)[1, row, 1, dim] = bad
+            else:
+                scales(c, which)[1, 1, row, dim // 32] = bad
+            got = syn.tree_attention(c, q, lens_gpu, n_head, 0.125, **args).view(2, tree, n_head, hd)
+            hit = np.ones(tree, bool) if row < lens[1] else sees[1, :, 1]
+            assert torch.equal(got[0], want[0]) and torch.equal(got[:, :, :group], want[:, :, :group])
+            assert torch.equal(got[1, ~hit], want[1, ~hit])
+            heads = got[1, hit][:, group:]
+            if which == 0 or type_ != syn.F16 or row >= lens[1]:
+                assert heads.isnan().all()
+            else:
+                others = torch.arange(hd, device="cuda") != dim
+                assert not heads[..., dim].isfinite().any() and torch.equal(heads[..., others], want[1, hit][:, group:][..., others])
