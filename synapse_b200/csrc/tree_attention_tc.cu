@@ -213,7 +213,8 @@ __global__ void __launch_bounds__(kTcThreads, 1) tree_attn_tc_kernel(const TreeP
             for (int e = 0; e < V; ++e) top = max(top, __float_as_uint(fabsf(x[e])));
             float up, down;
             q_factor(__uint_as_float(__reduce_max_sync(0xffffffffu, top)), up, down);
-            if (lane == 0) sh.q_scale[r] = fabsf(a.scale_log2) * down;
+            const float by = fabsf(a.scale_log2) * down;
+            if (lane == 0) sh.q_scale[r] = by == 0.0f ? 0x1p-126f : by;  // masked scores, -inf, are multiplied by it
             if (a.scale_log2 < 0.0f) up = -up;  // the scores' factor is positive: maxima may be taken before it
             uint32_t hi[V / 2], lo[V / 2];
 #pragma unroll

@@ -141,3 +141,17 @@ def test_one_value_that_is_not_finite(type_, hd, n_head, tree, which):
             else:
                 others = torch.arange(hd, device="cuda") != dim
                 assert not heads[..., dim].isfinite().any() and torch.equal(heads[..., others], want[1, hit][:, group:][..., others])
+
+
+# ---- a scale of zero --------------------------------------------------------------------------------------------------
+@pytest.mark.parametrize("type_", TYPES)
+@pytest.mark.parametrize("hd", [64, 96, 128, 256])
+@pytest.mark.parametrize("n_head,tree", ROWS)
+def test_scale_of_zero_is_the_mean_of_what_is_seen(type_, hd, n_head, tree):
+    rng = np.random.default_rng(hd + tree)
+    lens = [130, 7]
+    cache = new_cache(type_, 2, 2, hd, 130 + tree)
+    fill(cache, rng, 130 + tree)
+    q = rng.standard_normal((2 * tree, n_head * hd), dtype=np.float32)
+    words, sees = random_masks(rng, 2, tree)
+    check_against_64_bits(cache, q, lens, tree, words, sees, n_head, 0.0)
