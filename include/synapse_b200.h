@@ -278,8 +278,9 @@ size_t syn_kv_cache_bytes(int type, int n_kv, int head_dim, int max_ctx);
  * syn_tree_attention takes. A token's RoPE position is pos[s * n + i]
  * (NULL: its slot; in a tree the positions are the committed length plus the
  * node's depth). Quantised types store finite values: an input beyond
- * binary16's range is clamped to +-65504 and NaN stored as 0; F16 stores what
- * the rounding gives. A token whose slot is outside the cache, or whose
+ * binary16's range is clamped to +-65504 and NaN stored as 0, and a Q8_0
+ * scale is at most 515.5, so that the values read back in binary16 are finite
+ * too; F16 stores what the rounding gives. A token whose slot is outside the cache, or whose
  * position is outside the table, is skipped whole (its q_out row too). Two
  * tokens of a call must not share a slot of a sequence. */
 typedef struct {
@@ -300,7 +301,8 @@ int syn_kv_append(const syn_kv_cache* c, int layer, const syn_kv_append_args* a,
 /* Read n rows of every sequence back as values: row i of sequence s is cache
  * row rows[s * n + i] (device), or first + i when rows is NULL. k_out, v_out
  * (either may be NULL): [n_seq][n][n_kv][head_dim] of out_type SYN_F32 or
- * SYN_F16, 16-byte aligned. Rows outside the cache read as zeros. */
+ * SYN_F16 (a value beyond binary16's range, which no append stores, is an
+ * infinity there), 16-byte aligned. Rows outside the cache read as zeros. */
 int syn_kv_read(const syn_kv_cache* c, int layer, const int32_t* rows, int first, int n, int out_type, void* k_out,
                 void* v_out, void* stream);
 

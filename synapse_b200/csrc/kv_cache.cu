@@ -102,7 +102,7 @@ __global__ void __launch_bounds__(THREADS) kv_append_kernel(AppendParams a) {
         uint16_t* scale = reinterpret_cast<uint16_t*>(base + a.c.scale_plane) + block;
         if (TYPE == SYN_Q8_0) {
             const float dd = __fdiv_rn(__uint_as_float(top), 127.0f), id8 = __fdiv_rn(1.0f, dd);
-            const uint16_t dh = f16_bits(dd);
+            const uint16_t dh = min(f16_bits(dd), uint16_t(0x6007));  // 515.5: 127 times the next, 516, is beyond binary16
             uint32_t word = 0;  // a scale that rounds to zero stores zeros (and 1 / d may not be finite)
 #pragma unroll
             for (int e = 0; e < 4; ++e) word |= (dh ? uint32_t(int(roundf(__fmul_rn(x[e], id8)))) & 255u : 0u) << (8 * e);

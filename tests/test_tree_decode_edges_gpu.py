@@ -155,3 +155,22 @@ def test_scale_of_zero_is_the_mean_of_what_is_seen(type_, hd, n_head, tree):
     q = rng.standard_normal((2 * tree, n_head * hd), dtype=np.float32)
     words, sees = random_masks(rng, 2, tree)
     check_against_64_bits(cache, q, lens, tree, words, sees, n_head, 0.0)
+
+
+# ---- what an append stores --------------------------------------------------------------------------------------------
+@pytest.mark.parametrize("type_", [syn.Q8_0, syn.Q4_0])
+def test_clamped_rows_read_back_finite_in_binary16(type_):
+    """Values around and beyond binary16's range, of both signs, read back in both formats."""
+    tops = [65400.0, 65469.0, 65499.0, 65500.25, 65500.5, 65503.0, 65504.0, 65519.0, 65520.0, 1e6, 3e38, float("inf")]
+    tops += [-t for t in tops]
+    cache = new_cache(type_, 1, 1, 64, len(tops))
+    x = np.ones((len(tops), 64), np.float32)
+    x[:, 5] = tops
+    syn.kv_append(cache, gpu(x), gpu(x), gpu(np.arange(len(tops), dtype=np.int32)))
+    f, _ = syn.kv_read(cache, len(tops))
+    h, hv = syn.kv_read(cache, len(tops), dtype=torch.float16)
+    assert f.isfinite().all() and h.isfinite().all() and torch.equal(h, hv)
+    want = np.clip(np.array(tops), -65504.0, 65504.0)
+    got = f[0, :, 0, 5].cpu().numpy()
+    # the scale's rounding: 2^-11 of it, or from 516 down to 515.5
+    assert (np.abs(got - want) <= 1.01 * 2.0 ** -10 * np.abs(want)).all()
