@@ -90,8 +90,11 @@ class TreeDecoder:
         return self.torch.from_numpy(np.ascontiguousarray(a)).to(self.cache.device)
 
     def forward(self, tokens, parents):
-        """Logits [n_seq * nodes][n_vocab] of one tree per sequence appended after its committed rows, and the mask."""
+        """Logits [n_seq * nodes][n_vocab] of one tree per sequence appended after its committed rows, and the mask.
+        Raises ValueError when a tree does not fit its sequence's cache."""
         c, w, n = self.cfg, self.w, tokens.shape[1]
+        if self.lens.max() + n > self.max_ctx:
+            raise ValueError(f"{n} rows after {self.lens.max()} do not fit a cache of {self.max_ctx}")
         masks, depths = zip(*(tree_mask(p) for p in parents))
         mask = self.dev(np.stack(masks))
         slot = self.dev((self.lens[:, None] + np.arange(n, dtype=np.int32)).reshape(-1))
@@ -149,6 +152,13 @@ class TreeDecoder:
             self.histories[s] += new
         return out
 
+    def keep(self, n):
+        """Takes the tokens past the first n of every sequence back; their rows are written again."""
+        for s, h in enumerate(self.histories):
+            if len(h) > n:
+                del h[n:]
+                self.lens[s] = n - 1
+
     def start(self, prompts):
         """Prompts of one length: all but the last token are run as a chain through the cache."""
         self.histories = [list(map(int, p)) for p in prompts]
@@ -160,11 +170,13 @@ class TreeDecoder:
 
 
 def decode(model, prompts, steps, size, rules):
-    """`steps` tokens per sequence by trees of `size` nodes: (tokens [n_seq][steps], forward passes)."""
+    """`steps` tokens per sequence by trees of `size` nodes: (tokens [n_seq][steps], forward passes). The caches need room
+    for the prompt, the steps and a tree; a sequence that is done waits for the others."""
     model.start(prompts)
     first, passes = len(prompts[0]), 0
     while min(len(h) for h in model.histories) < first + steps:
         model.step(size, rules)
+        model.keep(first + steps)
         passes += 1
     return [h[first:first + steps] for h in model.histories], passes
 
