@@ -23,6 +23,7 @@ from . import F16, F32, LAYOUT_PLANAR, Q4_0, Q8_0, KVCache, embed, kv_append, kv
 from .model import random_llama_weights
 
 CACHES = {"f16": F16, "q8_0": Q8_0, "q4_0": Q4_0}
+MOST_NODES = 1024  # of a tree (syn_tree_attention)
 
 
 def tree_mask(parents):
@@ -160,13 +161,14 @@ class TreeDecoder:
                 self.lens[s] = n - 1
 
     def start(self, prompts):
-        """Prompts of one length: all but the last token are run as a chain through the cache."""
+        """Prompts of one length: all but the last token are run as chains through the cache."""
         self.histories = [list(map(int, p)) for p in prompts]
         self.lens[:] = 0
-        n = len(prompts[0]) - 1
-        if n > 0:
-            self.forward(np.array([p[:-1] for p in prompts], np.int32), [list(range(-1, n - 1))] * self.n_seq)
-            self.lens += n
+        tokens = np.array([p[:-1] for p in prompts], np.int32)
+        for i in range(0, tokens.shape[1], MOST_NODES):
+            part = tokens[:, i:i + MOST_NODES]
+            self.forward(part, [list(range(-1, part.shape[1] - 1))] * self.n_seq)
+            self.lens += part.shape[1]
 
 
 def decode(model, prompts, steps, size, rules):

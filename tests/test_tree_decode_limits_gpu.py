@@ -11,9 +11,10 @@ from synapse_b200 import tree_decode as td  # noqa: E402
 CFG = dict(n_layer=1, n_embd=128, n_ff=256, n_head=4, n_head_kv=2, head_dim=32, n_vocab=256, rms_eps=1e-5, rope_base=10000.0)
 
 
-def decoder(n_seq, max_ctx, tree, cache=syn.F16):
-    weights = synmodel.random_llama_weights(CFG, seed=3, type_layers=syn.F32, type_embd=syn.F32, tied=True, sigma=0.05)
-    return td.TreeDecoder(CFG, weights, cache, n_seq, max_ctx, tree)
+def decoder(n_seq, max_ctx, tree, cache=syn.F16, n_layer=1):
+    cfg = dict(CFG, n_layer=n_layer)
+    weights = synmodel.random_llama_weights(cfg, seed=3, type_layers=syn.F32, type_embd=syn.F32, tied=True, sigma=0.05)
+    return td.TreeDecoder(cfg, weights, cache, n_seq, max_ctx, tree)
 
 
 def prompts(n_seq, n):
@@ -41,3 +42,20 @@ def test_decode_fills_the_cache_to_its_last_row_and_no_further():
     many, passes = td.decode(m, p, steps, tree, {})
     assert many == one and passes <= steps
     assert [len(h) for h in m.histories] == [5 + steps] * 3 and m.lens.tolist() == [4 + steps] * 3
+
+
+@pytest.mark.parametrize("n", [1, 2, 1025, 1026, 2500])
+def test_prompts_of_any_length(n):
+    """A prompt of more tokens than a tree may have leaves the rows that its tokens leave in chains of 100."""
+    m, by_100 = decoder(2, n + 4, 4, n_layer=2), decoder(2, n + 4, 4, n_layer=2)
+    p = prompts(2, n)
+    m.start(p)
+    assert m.lens.tolist() == [n - 1] * 2
+    for i in range(0, n - 1, 100):
+        part = np.array([x[i:min(i + 100, n - 1)] for x in p], np.int32)
+        by_100.forward(part, [list(range(-1, part.shape[1] - 1))] * 2)
+        by_100.lens += part.shape[1]
+    if n > 1:
+        for x, y in zip(syn.kv_read(m.cache, n - 1, layer=1), syn.kv_read(by_100.cache, n - 1, layer=1)):
+            assert (x - y).abs().max() <= 2.0 ** -10 * x.abs().max()  # a value may round to the neighbouring binary16
+    assert all(len(new) >= 1 for new in m.step(4, {}))
