@@ -119,7 +119,8 @@ class TreeDecoder:
         return mm("output" if "output" in w else "token_embd", h), mask
 
     def step(self, size, rules):
-        """One step of a tree of `size` nodes per sequence: the tokens that it commits, for every sequence."""
+        """One step of a tree of `size` nodes per sequence: the tokens that it commits, for every sequence. Raises ValueError,
+        with nothing committed, where the rules leave a sequence no token."""
         drafts = [draft_pairs(h, size, c) for h, c in zip(self.histories, self.corpus)]
         tokens = np.array([d[0] for d in drafts], np.int32)
         logits, mask = self.forward(tokens, [d[1] for d in drafts])
@@ -144,6 +145,8 @@ class TreeDecoder:
                     break
                 kept.append(node)
                 new.append(int(picks[s, node]))
+            if min(new) < 0:
+                raise ValueError(f"no logit of sequence {s} is above -inf: no token to go on with")
             path[s, :len(kept)] = self.lens[s] + np.array(kept)
             count[s] = len(kept)
             out.append(new)

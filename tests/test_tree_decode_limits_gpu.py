@@ -59,3 +59,13 @@ def test_prompts_of_any_length(n):
         for x, y in zip(syn.kv_read(m.cache, n - 1, layer=1), syn.kv_read(by_100.cache, n - 1, layer=1)):
             assert (x - y).abs().max() <= 2.0 ** -10 * x.abs().max()  # a value may round to the neighbouring binary16
     assert all(len(new) >= 1 for new in m.step(4, {}))
+
+
+def test_rules_that_leave_no_token_raise():
+    m = decoder(2, 40, 4)
+    m.start(prompts(2, 6))
+    before = [list(h) for h in m.histories], m.lens.copy()
+    with pytest.raises(ValueError, match="no token"):
+        m.step(4, {"allowed": torch.zeros(1, CFG["n_vocab"] // 32, dtype=torch.int32, device="cuda")})
+    assert m.histories == before[0] and (m.lens == before[1]).all()
+    assert all(0 <= t < CFG["n_vocab"] for new in m.step(4, {}) for t in new)
