@@ -359,8 +359,9 @@ int syn_tree_attention(const syn_kv_cache* c, int layer, const syn_tree_attentio
  *             (NaN is never picked).
  * Everything but logits, out or pick, and the sizes may be NULL. Tokens
  * outside the vocabulary count nowhere. A token that a sequence's bias list
- * names several times gets their sum, added in the list's order. Calls that overlap on the GPU need scratches of
- * their own. */
+ * names several times gets their sum, added in the list's order; entries
+ * outside [0, n_bias) that bias_begin names are left out. Calls that overlap
+ * on the GPU need scratches of their own. */
 typedef struct {
     const float* logits;
     float* out;                 /* NULL: only picks; may be logits itself */
@@ -379,6 +380,7 @@ typedef struct {
     void* scratch;              /* with pick: syn_logits_scratch_bytes, 8-byte aligned, zeroed once before its
                                    first use (each call leaves it zero) */
     int n_seq, n_tree, n_vocab, history_ld;
+    int n_bias;                 /* entries of bias_token and bias_value (0: as many as bias_begin names) */
 } syn_logits_args;
 size_t syn_logits_scratch_bytes(int n_rows);
 int syn_logits_process(const syn_logits_args* a, void* stream);

@@ -418,7 +418,7 @@ class LogitsArgs(ctypes.Structure):
                [(n, ctypes.c_void_p) for n in ("penalties", "history", "history_len", "draft", "mask", "bias_begin",
                                                 "bias_token", "bias_value", "allowed")] + \
                [("allowed_ld", ctypes.c_size_t), ("scratch", ctypes.c_void_p)] + \
-               [(n, ctypes.c_int) for n in ("n_seq", "n_tree", "n_vocab", "history_ld")]
+               [(n, ctypes.c_int) for n in ("n_seq", "n_tree", "n_vocab", "history_ld", "n_bias")]
 
 
 def kv_cache_bytes(type_, n_kv, head_dim, max_ctx):
@@ -646,7 +646,7 @@ def logits_process(logits, n_seq, penalties=None, history=None, history_len=None
                    _need(draft, dev, i32, rows, "draft"), _need(mask, dev, i32, rows * ((tree + 31) // 32), "mask"),
                    _need(begin, dev, i32, n_seq + 1, "bias begin"), _need(tokens, dev, i32, n, "bias tokens"),
                    _need(values, dev, f32, n, "bias values"), _need(allowed, dev, i32, rows * words, "allowed"), words, sp,
-                   n_seq, tree, vocab, history_ld)
+                   n_seq, tree, vocab, history_ld, n)
     check(lib().syn_logits_process(ctypes.byref(a), _current(logits.device, dev)), "syn_logits_process")
     return out, picks
 

@@ -24,6 +24,7 @@
 #include "common.cuh"
 
 #include <algorithm>
+#include <climits>
 
 using namespace syn;
 
@@ -48,7 +49,7 @@ struct LogitParams {
     const uint32_t* allowed;
     unsigned long long* key;  // [rows] best of the chunks seen so far, 0 = none
     unsigned* arrived;        // [rows]
-    int n_tree, n_vocab, history_ld, rows_per_cta;
+    int n_tree, n_vocab, history_ld, n_bias, rows_per_cta;
 };
 
 // Counts: 32 bits in the short chunks, 16 (two to a word) in the long ones,
@@ -136,6 +137,9 @@ __global__ void __launch_bounds__(kThreads, 4) logits_kernel(const LogitParams a
     };
     load(0);  // on its way while the counts are made
 
+    // both in [0, n_bias], which leaves room for a CTA's steps below the largest int
+    const int bias0 = a.bias_begin ? min(max(a.bias_begin[seq], 0), a.n_bias) : 0;
+    const int bias1 = a.bias_begin ? min(max(a.bias_begin[seq + 1], 0), a.n_bias) : 0;
     auto touch = [&](int at) { atomicOr(&sh.touched[at >> 5], 1u << (at & 31)); };
     if (a.history) {
         const int n = min(a.history_len[seq], a.history_ld);
@@ -152,15 +156,12 @@ __global__ void __launch_bounds__(kThreads, 4) logits_kernel(const LogitParams a
                 }
         }
     }
-    if (a.bias_begin) {
-        const int end = a.bias_begin[seq + 1];
-        for (int i = a.bias_begin[seq] + tid; i < end; i += kThreads) {
-            const int tok = a.bias_token[i];
-            if (tok >= v0 && tok - v0 < span) {
-                atomicAdd(&sh.bias[tok - v0], a.bias_value[i]);
-                if (atomicAdd(reinterpret_cast<unsigned*>(sh.x) + tok - v0, 1u) == 2) sh.thrice = 1;
-                touch(tok - v0);
-            }
+    for (int i = bias0 + tid; i < bias1; i += kThreads) {
+        const int tok = a.bias_token[i];
+        if (tok >= v0 && tok - v0 < span) {
+            atomicAdd(&sh.bias[tok - v0], a.bias_value[i]);
+            if (atomicAdd(reinterpret_cast<unsigned*>(sh.x) + tok - v0, 1u) == 2) sh.thrice = 1;
+            touch(tok - v0);
         }
     }
     const int32_t* draft = a.draft ? a.draft + size_t(seq) * a.n_tree : nullptr;
@@ -178,7 +179,7 @@ __global__ void __launch_bounds__(kThreads, 4) logits_kernel(const LogitParams a
         for (int at = tid; at < CHUNK; at += kThreads)
             if (__float_as_uint(sh.x[at]) > 2) {
                 float sum = 0.0f;
-                for (int i = a.bias_begin[seq]; i < a.bias_begin[seq + 1]; ++i)
+                for (int i = bias0; i < bias1; ++i)
                     if (a.bias_token[i] == v0 + at) sum += a.bias_value[i];
                 sh.bias[at] = sum;
             }
@@ -314,12 +315,13 @@ extern "C" int syn_logits_process(const syn_logits_args* x, void* stream) {
     if (a.ld < size_t(x->n_vocab) || a.out_ld < size_t(x->n_vocab) || a.allowed_ld < words) return SYN_ERR_INVALID;
     if (x->out == x->logits && a.ld != a.out_ld) return SYN_ERR_INVALID;
     if (x->history && (!x->history_len || x->history_ld <= 0)) return SYN_ERR_INVALID;
-    if (x->bias_begin && (!x->bias_token || !x->bias_value)) return SYN_ERR_INVALID;
+    if (x->bias_begin && (!x->bias_token || !x->bias_value || x->n_bias < 0)) return SYN_ERR_INVALID;
     if (x->pick && (!x->scratch || (reinterpret_cast<uintptr_t>(x->scratch) & 7))) return SYN_ERR_INVALID;
     a.penalties = x->penalties;
     a.history = x->history; a.history_len = x->history_len; a.history_ld = x->history_ld;
     a.draft = x->draft; a.mask = x->mask;
     a.bias_begin = x->bias_begin; a.bias_token = x->bias_token; a.bias_value = x->bias_value;
+    a.n_bias = x->n_bias && x->n_bias < INT_MAX - kThreads ? x->n_bias : INT_MAX - kThreads;
     a.allowed = x->allowed;
     const size_t rows = size_t(x->n_seq) * x->n_tree;
     a.key = static_cast<unsigned long long*>(x->scratch);
