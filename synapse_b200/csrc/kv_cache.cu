@@ -237,12 +237,13 @@ __device__ __forceinline__ void move_column(T* col, size_t pitch, const int32_t*
 #pragma unroll
         for (int j = 0; j < kMoveBatch; ++j) {
             const int i = i0 + j, src = i < n ? path[i] : -1;
-            ok[j] = src >= 0 && src < max_ctx && begin + i >= 0 && begin + i < max_ctx && src != begin + i;
+            const unsigned to = unsigned(begin) + unsigned(i);  // a begin near the largest int wraps past max_ctx
+            ok[j] = src >= 0 && src < max_ctx && to < unsigned(max_ctx) && unsigned(src) != to;
             if (ok[j]) x[j] = col[size_t(src) * pitch];
         }
 #pragma unroll
         for (int j = 0; j < kMoveBatch; ++j)
-            if (ok[j]) col[size_t(begin + i0 + j) * pitch] = x[j];
+            if (ok[j]) col[size_t(unsigned(begin) + unsigned(i0 + j)) * pitch] = x[j];
     }
 }
 

@@ -174,3 +174,17 @@ def test_clamped_rows_read_back_finite_in_binary16(type_):
     got = f[0, :, 0, 5].cpu().numpy()
     # the scale's rounding: 2^-11 of it, or from 516 down to 515.5
     assert (np.abs(got - want) <= 1.01 * 2.0 ** -10 * np.abs(want)).all()
+
+
+@pytest.mark.parametrize("type_", TYPES)
+def test_move_to_rows_near_the_largest_int(type_):
+    """Rows begin + i outside the cache are skipped, wherever begin is; those inside are moved."""
+    cache = new_cache(type_, 3, 2, 64, 16)
+    fill(cache, np.random.default_rng(1), 16)
+    k, v = syn.kv_read(cache, 16)
+    path = np.array([[9, 10, 11], [9, 10, 11], [9, 10, 11]], np.int32)
+    begin = np.array([2**31 - 2, -2, -2**31], np.int32)  # the second: rows -2, -1 and 0
+    syn.kv_move(cache, gpu(path), gpu(np.array([3, 3, 3], np.int32)), gpu(begin))
+    for x, y in zip((k, v), syn.kv_read(cache, 16)):
+        x[1, 0] = x[1, 11]
+        assert torch.equal(x, y)
