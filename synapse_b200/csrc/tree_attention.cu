@@ -15,9 +15,10 @@
 // their own (one pass over K and V); the warps' results are joined at the end.
 // The contexts of all sequences are cut into parts of one length, as many as
 // fill the GPU whatever the sequences' own lengths; each CTA leaves (max, sum,
-// output) in the scratch, and the last of a sequence's to be done joins them,
-// in their order. (tree_attention_tc.cu leaves that to tree_join_kernel, which
-// starts early and waits for the first kernel to end: its parts are larger.)
+// output) in the scratch. With few rows (cut_of) the last of a sequence's CTAs to
+// be done joins them, in their order; with more, and always of
+// tree_attention_tc.cu's parts, tree_join_kernel does, which starts early and
+// waits for the first kernel to end.
 //
 // Precision: the products run on binary16 tensor-core instructions with float
 // accumulators. q is scaled by a power of two per row and split into two
@@ -196,10 +197,10 @@ __global__ void __launch_bounds__(kWarps * 32, Plan<TYPE, HDP, STACK>::ctas) tre
 
     pdl_launch_dependents();
     pdl_wait();
-    int seq = -1;
-    const Cutting cut = tree_cutting(a, kStep, blockIdx.x, seq);
+    const Cutting cut = tree_cutting(a, kStep, blockIdx.x);
+    const int seq = cut.seq;
     if (seq < 0) return;
-    note_cut(a, cut, seq);
+    note_cut(a, cut);
     const int len = tree_len(a, seq), total = len + a.n_tree;
     const int steps = (total + kStep - 1) / kStep;
     const int s0 = (int(blockIdx.x) - cut.first) * cut.per, s1 = cut.per < steps - s0 ? s0 + cut.per : steps;
@@ -774,7 +775,7 @@ Cut cut_of(int type, int n_seq, int n_tree, int n_head, int n_kv, int head_dim, 
         const size_t most = std::max((turns + 1) / 2, std::min<size_t>(turns, 16)) * n_seq;
         c.parts = int(std::min(per_sm * sms / units, most));
     }
-    if (c.parts <= n_seq && !(n_seq == 1 && c.parts > 1)) c.parts = 0;
+    if (c.parts <= n_seq) c.parts = 0;
     // The last CTA has a row a warp to join, or two of a few parts, in less time than a launch; with more it has them
     // one after another. Measured for one sequence of 8192, last CTA / kernel, us: 4 rows (of 4096) 10.8 / 11.7, 8 rows
     // 18.3 / 16.2, 16 rows 27.0 / 18.4; 4 sequences of 8192, 8 rows 27.5 / 28.4, 16 rows 33.2 / 31.5.

@@ -15,12 +15,12 @@ struct TreeParams {
     const int32_t* len;
     const uint32_t* mask;
     unsigned* arrived;   // [n_seq][n_kv * row blocks]: parts that are done; zero between calls
-    int2* cuts;          // [n_seq]: a sequence's first part and number of parts, for tree_join_kernel
+    int2* cuts;          // [n_seq]: a sequence's first part and number of parts, for tree_join_kernel; or NULL
     float2* part_ml;     // [parts][n_kv * row blocks][R]: a part's maximum and sum of a row
     float* part_o;       // [parts][n_kv * row blocks][R][hd]: its output, not divided
     size_t q_stride;
     int n_tree, n_head, group, rows, row_blocks, max_len, mask_words;
-    int parts;           // that the contexts may be cut into, more than n_seq (n_seq = 1: or 1); 0: not cut
+    int parts;           // that the contexts may be cut into, more than n_seq; 0: not cut
     float scale_log2;    // scale * log2(e)
 };
 
@@ -90,6 +90,7 @@ __device__ __forceinline__ void q_factor(float m, float& up, float& down) {
 // whatever the sequences' lengths, numbered through the sequences, and the
 // shortest of which there are at most a.parts (0: a part is a sequence).
 struct Cutting {
+    int seq;    // the part's sequence, -1: there are not so many parts
     int per;    // steps of a part
     int first;  // the sequence's first part
     int parts;  // and its number of parts
@@ -100,19 +101,13 @@ __device__ __forceinline__ int tree_len(const TreeParams& a, int seq) {
 __device__ __forceinline__ int tree_steps(const TreeParams& a, int seq, int step) {
     return (tree_len(a, seq) + a.n_tree + step - 1) / step;
 }
-// For a warp: the cutting of sequence seq, or, with seq = -1, of the sequence
-// that holds part `part` (seq = -1 stays when there is none).
-__device__ __forceinline__ Cutting tree_cutting(const TreeParams& a, int step, int part, int& seq) {
+// For a warp: the sequence that holds part `part`, and its cutting.
+__device__ __forceinline__ Cutting tree_cutting(const TreeParams& a, int step, int part) {
     const int lane = threadIdx.x & 31, n = a.c.n_seq;
-    if (a.parts == 0) {
-        if (seq < 0) seq = part;
-        return {0x3fffffff, seq, 1};
-    }
+    if (a.parts == 0) return {part, 0x3fffffff, part, 1};
     if (n == 1) {
-        seq = 0;
         const int steps = tree_steps(a, 0, step), per = (steps + a.parts - 1) / a.parts, parts = (steps + per - 1) / per;
-        if (part >= parts) seq = -1;
-        return {per, 0, parts};
+        return {part < parts ? 0 : -1, per, 0, parts};
     }
     const int own = lane < n ? tree_steps(a, lane, step) : 0;
     int total = own;
@@ -137,20 +132,18 @@ __device__ __forceinline__ Cutting tree_cutting(const TreeParams& a, int step, i
             const int x = __shfl_up_sync(0xffffffffu, sum, o);
             if (lane >= o) sum += x;
         }
-        const bool here = seq >= 0 ? s0 + lane == seq : s0 + lane < n && part < before + sum;
-        const unsigned who = __ballot_sync(0xffffffffu, here);
+        const unsigned who = __ballot_sync(0xffffffffu, s0 + lane < n && part < before + sum);
         if (who) {
             const int l = __ffs(who) - 1;
-            seq = s0 + l;
-            return {per, before + __shfl_sync(0xffffffffu, sum - mine, l), __shfl_sync(0xffffffffu, mine, l)};
+            return {s0 + l, per, before + __shfl_sync(0xffffffffu, sum - mine, l), __shfl_sync(0xffffffffu, mine, l)};
         }
         before += __shfl_sync(0xffffffffu, sum, 31);
     }
-    return {per, 0, 0};
+    return {-1, per, 0, 0};
 }
 // By every CTA of a kernel whose parts tree_join_kernel joins.
-__device__ __forceinline__ void note_cut(const TreeParams& a, const Cutting& cut, int seq) {
-    if (a.cuts && threadIdx.x == 0 && blockIdx.y == 0 && int(blockIdx.x) == cut.first) a.cuts[seq] = make_int2(cut.first, cut.parts);
+__device__ __forceinline__ void note_cut(const TreeParams& a, const Cutting& cut) {
+    if (a.cuts && threadIdx.x == 0 && blockIdx.y == 0 && int(blockIdx.x) == cut.first) a.cuts[cut.seq] = make_int2(cut.first, cut.parts);
 }
 // Whether token tk of sequence seq sees the tree's row j >= 0.
 __device__ __forceinline__ bool tree_sees(const TreeParams& a, int seq, int tk, int j) {

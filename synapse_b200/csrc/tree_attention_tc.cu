@@ -141,10 +141,10 @@ __global__ void __launch_bounds__(kTcThreads, 1) tree_attn_tc_kernel(const TreeP
 
     pdl_launch_dependents();
     pdl_wait();
-    int seq = -1;
-    const Cutting cut = tree_cutting(a, kTcTile, blockIdx.x, seq);
+    const Cutting cut = tree_cutting(a, kTcTile, blockIdx.x);
+    const int seq = cut.seq;
     if (seq < 0) return;
-    note_cut(a, cut, seq);
+    note_cut(a, cut);
     const int len = tree_len(a, seq), total = len + a.n_tree;
     const int n_tiles = (total + kTcTile - 1) / kTcTile;
     const int t0 = (int(blockIdx.x) - cut.first) * cut.per, n = min(cut.per, n_tiles - t0);  // tiles t0 .. t0 + n - 1
