@@ -237,13 +237,12 @@ __device__ __forceinline__ void move_column(T* col, size_t pitch, const int32_t*
 #pragma unroll
         for (int j = 0; j < kMoveBatch; ++j) {
             const int i = i0 + j, src = i < n ? path[i] : -1;
-            const unsigned to = unsigned(begin) + unsigned(i);  // a begin near the largest int wraps past max_ctx
-            ok[j] = src >= 0 && src < max_ctx && to < unsigned(max_ctx) && unsigned(src) != to;
+            ok[j] = src >= 0 && src < max_ctx && begin + i >= 0 && begin + i < max_ctx && src != begin + i;
             if (ok[j]) x[j] = col[size_t(src) * pitch];
         }
 #pragma unroll
         for (int j = 0; j < kMoveBatch; ++j)
-            if (ok[j]) col[size_t(unsigned(begin) + unsigned(i0 + j)) * pitch] = x[j];
+            if (ok[j]) col[size_t(begin + i0 + j) * pitch] = x[j];
     }
 }
 
@@ -253,7 +252,8 @@ __global__ void __launch_bounds__(128) kv_move_kernel(MoveParams a) {
     pdl_wait();
     const int s = blockIdx.y, layer = blockIdx.z >> 1;
     char* base = ((blockIdx.z & 1) ? a.c.v : a.c.k) + size_t(layer) * a.layer_stride + size_t(s) * a.c.seq_stride;
-    const int n = min(a.count[s], a.path_ld), begin = a.begin[s];
+    // from past the cache or n and more before it no row is moved: begin + i stays an int
+    const int n = min(a.count[s], a.path_ld), begin = min(max(a.begin[s], -max(n, 0)), a.c.max_ctx);
     const int32_t* path = a.path + size_t(s) * a.path_ld;
     int col = blockIdx.x * blockDim.x + threadIdx.x;
     if (col < a.cols16) {
