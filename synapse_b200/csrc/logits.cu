@@ -137,9 +137,7 @@ __global__ void __launch_bounds__(kThreads, 4) logits_kernel(const LogitParams a
     };
     load(0);  // on its way while the counts are made
 
-    // both in [0, n_bias], which leaves room for a CTA's steps below the largest int
-    const int bias0 = a.bias_begin ? min(max(a.bias_begin[seq], 0), a.n_bias) : 0;
-    const int bias1 = a.bias_begin ? min(max(a.bias_begin[seq + 1], 0), a.n_bias) : 0;
+    const int named0 = a.bias_begin ? __ldg(a.bias_begin + seq) : 0, named1 = a.bias_begin ? __ldg(a.bias_begin + seq + 1) : 0;
     auto touch = [&](int at) { atomicOr(&sh.touched[at >> 5], 1u << (at & 31)); };
     if (a.history) {
         const int n = min(a.history_len[seq], a.history_ld);
@@ -156,6 +154,8 @@ __global__ void __launch_bounds__(kThreads, 4) logits_kernel(const LogitParams a
                 }
         }
     }
+    // both in [0, n_bias], which leaves room for a CTA's steps below the largest int
+    const int bias0 = min(max(named0, 0), a.n_bias), bias1 = min(max(named1, 0), a.n_bias);
     for (int i = bias0 + tid; i < bias1; i += kThreads) {
         const int tok = a.bias_token[i];
         if (tok >= v0 && tok - v0 < span) {
