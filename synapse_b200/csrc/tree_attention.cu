@@ -59,6 +59,7 @@ constexpr int kStep = 16;            // positions per step of a warp
 // F16 scores: products summed in the tensor core, which truncates, before a float add. The outputs' error (3000 positions)
 // with all of them summed there is 1.4e-6 at 128 dims and 2.0e-6 at 256, with two 5e-7, in the same time.
 constexpr int kChain = 2;
+constexpr int kMostLen = 0x7fffffff - kMaxTree;  // of max_len: positions rounded up to a tile are still ints
 constexpr size_t kCounterBytes = 4096;  // counters of parts that are done, at the start of the scratch
 __device__ __forceinline__ void ldsm4(uint32_t (&r)[4], uint32_t addr) {
     asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
@@ -807,7 +808,7 @@ int launch_type(const TreeParams& a, const Cut& c, cudaStream_t s) {
 extern "C" size_t syn_tree_attention_scratch_bytes(int n_seq, int n_tree, int n_head, int n_kv, int head_dim,
                                                    int max_len) {
     if (n_seq <= 0 || n_tree <= 0 || n_tree > kMaxTree || n_kv <= 0 || n_head <= 0 || n_head % n_kv || head_dim <= 0 ||
-        head_dim > 256 || max_len < n_tree)
+        head_dim > 256 || max_len < n_tree || max_len > kMostLen)
         return 0;
     size_t rows = 0;  // the most of any type
     for (int type : {SYN_F16, SYN_Q8_0, SYN_Q4_0})
@@ -821,7 +822,7 @@ extern "C" int syn_tree_attention(const syn_kv_cache* c, int layer, const syn_tr
     if (!x || !x->q || !x->out || !x->len || !x->scratch) return SYN_ERR_INVALID;
     if (x->n_head <= 0 || x->n_head % c->n_kv || x->n_tree <= 0) return SYN_ERR_INVALID;
     if (x->max_len < x->n_tree || x->max_len > c->max_ctx) return SYN_ERR_INVALID;
-    if (x->n_tree > kMaxTree || c->n_seq > 65535) return SYN_ERR_UNSUPPORTED;
+    if (x->n_tree > kMaxTree || c->n_seq > 65535 || x->max_len > kMostLen) return SYN_ERR_UNSUPPORTED;
     const size_t q_row = size_t(x->n_head) * c->head_dim;
     if (x->q_stride && x->q_stride < q_row) return SYN_ERR_INVALID;
     if ((reinterpret_cast<uintptr_t>(x->scratch) | reinterpret_cast<uintptr_t>(x->out)) & 15) return SYN_ERR_INVALID;
