@@ -322,8 +322,8 @@ int syn_kv_move(const syn_kv_cache* c, const int32_t* path, int path_ld, const i
  *   own row included).
  * Query head h reads KV head h / (n_head / n_kv). Products use the binary16
  * or block values of the cache as stored; q, the probabilities and every sum
- * keep 22 bits or more (about 1e-6 relative). A token that sees nothing gets
- * zeros. What masked rows hold, infinities and NaN included, reaches no
+ * keep 22 bits or more (about 1e-6 of the largest value of V that a token
+ * sees). A token that sees nothing gets zeros. What masked rows hold, infinities and NaN included, reaches no
  * output. A token that sees a row with a value of K that is not finite gets
  * NaN in the heads that read it; so it does for a value of V, but for the
  * committed rows of an F16 cache: there the dim of the value is infinite or

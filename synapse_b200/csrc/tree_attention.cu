@@ -42,10 +42,12 @@
 // that takes 60 us in Q8_0, against 92 with a product for each term.
 //
 // Bound: an F16 cache's bytes (16 sequences of 8192: 76 us, 5.4 TB/s, 83 % of
-// the copy rate). A quantised cache's instructions: its bytes become binary16
-// in some 600 instructions of a warp per 16 positions, whatever their width (60
-// us in Q8_0, 57 % of the copy rate, 59 in Q4_0, 30 %). One short sequence: the
-// steps' latencies and the join (4096 positions: 10.8 us).
+// the copy rate). A quantised cache's steps: some 600 instructions of a warp per
+// 16 positions whatever the bytes' width (170 make binary16 of the bytes, 32 are
+// products, the rest adds, splits, scales and addresses), issued in 57 % of the
+// schedulers' active cycles, and uneven parts (60 us in Q8_0, 57 % of the copy rate,
+// 61 in Q4_0, 30 %). One short sequence: the steps' latencies and the join (4096
+// positions: 12.5 us).
 #include "tree_attention.cuh"
 
 #include <algorithm>
@@ -731,7 +733,8 @@ struct Cut {
     int R, row_blocks, parts;
     size_t rows;  // of all parts in the scratch
 };
-// CTAs of the few-row kernel on an SM.
+// CTAs of the few-row kernel on an SM (heads of more than 128 dims in F16 and Q8_0: shared memory lets one on it, and the
+// parts take two waves).
 template <int TYPE>
 constexpr int slots(int hd, bool stack) {
     return hd <= 64    ? (stack ? Plan<TYPE, 64, true>::ctas : Plan<TYPE, 64, false>::ctas)

@@ -9,8 +9,9 @@ decode of the same prompts, a fifth of its tokens changed), appends the drafted 
 (syn_kv_append), attends with the tree's mask (syn_tree_attention), picks a
 token at every node under penalties, biases and a grammar mask
 (syn_logits_process), keeps the longest path that the picks confirm and moves
-its rows together (syn_kv_move). The tokens are those of decoding one at a time;
-the command decodes both ways and compares.
+its rows together (syn_kv_move). The tokens are those of decoding one at a time,
+up to near ties that the orders of summing decide; the command decodes both ways
+and compares.
 """
 import argparse
 import json
@@ -41,8 +42,8 @@ def tree_mask(parents):
 
 def draft_pairs(history, size, corpus=(), branch=2):
     """A tree of `size` nodes from the last token on: what followed each token earlier, in the history or the corpus,
-    most recent first. (tokens, parents); node 0 is the last token itself. The tree is filled up with nodes that nothing
-    confirms."""
+    most recent first. (tokens, parents); node 0 is the last token itself. The tree is filled up with copies of it under
+    the root."""
     follow = {}
     for a, b in [*zip(corpus, corpus[1:]), *zip(history, history[1:])]:
         f = follow.setdefault(int(a), [])
